@@ -4,6 +4,7 @@
 #pragma once
 #include <math.h>
 
+#include "cache_int4.h"
 #include "common.h"
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
@@ -37,15 +38,26 @@ struct PrefillLds {
   uint32_t table[AP_TABLE_MAX];
 };
 
+// What the pages hold: bfloat16 values, which go from memory straight into LDS, or codes of 4 bits and their steps
+// (cache_int4.h), which pass through registers and lie in LDS as the bfloat16 values that they stand for.
+struct Bf16Pages {
+  typedef bf16_t Element;
+  static constexpr bool INT4 = false;
+};
+struct Int4Pages {
+  typedef uint8_t Element;
+  static constexpr bool INT4 = true;
+};
+
 // The work of one block: one head of one tile of queries.  The caller provides the block's LDS
 // (the kernel below its own; a kernel that runs blocks of several kinds in one launch a share
 // of what all of them need).
 // head_dim / 16; waves along the keys; waves along the queries; runs of 32 keys per wave and tile
-template <int NDB, int KS, int QW = 2, int KR = 1>
+template <int NDB, int KS, int QW = 2, int KR = 1, typename Pages = Bf16Pages>
 __device__ __forceinline__ void attention_prefill_block(
     PrefillLds<NDB, KS, QW, KR>& lds, const int head, const int tile_index,
-    const bf16_t* __restrict__ q, int64_t q_stride, const bf16_t* __restrict__ k_pool,
-    const bf16_t* __restrict__ v_pool, bf16_t* __restrict__ out, int64_t out_stride,
+    const bf16_t* __restrict__ q, int64_t q_stride, const typename Pages::Element* __restrict__ k_pool,
+    const typename Pages::Element* __restrict__ v_pool, bf16_t* __restrict__ out, int64_t out_stride,
     const int* __restrict__ tile_item, const int* __restrict__ tile_q0,
     const int* __restrict__ cu_tokens, const int* __restrict__ kv_lens,
     const int* __restrict__ tables, int table_width, int heads, int kv_heads, int page_size,
@@ -161,35 +173,130 @@ __device__ __forceinline__ void attention_prefill_block(
     load_piece[j] = (slot + CH - (key_local / SPREAD) % CH) % CH;
   }
   const int page_mask = page_size - 1;                // where the page size is a power of two
-  auto issue = [&](int tile_number, int k0) {
-    unsigned char* stage = stages + (tile_number % STAGES) * STAGE_BYTES;
-    // the rows first (their table entries are then on their way together), then the loads
-    uint32_t row[PER_OPERAND];
-#pragma unroll
-    for (int j = 0; j < PER_OPERAND; ++j) {
-      // keys outside the tile's visible range are fetched from a visible key instead: they
-      // are masked below, and whatever lies in pages that were given back is never read
-      int key = k0 + load_key[j];
-      key = key < key_begin ? key_begin : (key >= key_end ? key_end - 1 : key);
-      int logical, within;
-      if (page_shift >= 0) {
-        logical = key >> page_shift;
-        within = key & page_mask;
-      } else {
-        logical = key / page_size;
-        within = key - logical * page_size;
-      }
-      row[j] = s_table[logical - first_logical] + (uint32_t)within;
+  // the page's first row and the key's place in the page, for a lane's piece j of the tile at k0
+  auto place_of = [&](int j, int k0, uint32_t& page_row, int& within) {
+    // keys outside the tile's visible range are fetched from a visible key instead: they
+    // are masked below, and whatever lies in pages that were given back is never read
+    int key = k0 + load_key[j];
+    key = key < key_begin ? key_begin : (key >= key_end ? key_end - 1 : key);
+    int logical;
+    if (page_shift >= 0) {
+      logical = key >> page_shift;
+      within = key & page_mask;
+    } else {
+      logical = key / page_size;
+      within = key - logical * page_size;
     }
+    page_row = s_table[logical - first_logical];
+  };
+  auto issue = [&](int tile_number, int k0) {
+    if constexpr (!Pages::INT4) {
+      unsigned char* stage = stages + (tile_number % STAGES) * STAGE_BYTES;
+      // the rows first (their table entries are then on their way together), then the loads
+      uint32_t row[PER_OPERAND];
 #pragma unroll
-    for (int j = 0; j < PER_OPERAND; ++j) {
-      const uint64_t offset = (uint64_t)row[j] * (uint32_t)HD + (uint32_t)(load_piece[j] * 8);
-      const int number = wave * PER_OPERAND + j < INSTRUCTIONS ? wave * PER_OPERAND + j : INSTRUCTIONS - 1;
-      const int dst = number * 1024;
-      __builtin_amdgcn_global_load_lds((ap_global_ptr)(k_pool + offset), (ap_lds_ptr)(stage + dst),
-                                       16, 0, 0);
-      __builtin_amdgcn_global_load_lds((ap_global_ptr)(v_pool + offset),
-                                       (ap_lds_ptr)(stage + TILE_BYTES + dst), 16, 0, 0);
+      for (int j = 0; j < PER_OPERAND; ++j) {
+        uint32_t page_row;
+        int within;
+        place_of(j, k0, page_row, within);
+        row[j] = page_row + (uint32_t)within;
+      }
+#pragma unroll
+      for (int j = 0; j < PER_OPERAND; ++j) {
+        const uint64_t offset = (uint64_t)row[j] * (uint32_t)HD + (uint32_t)(load_piece[j] * 8);
+        const int number = wave * PER_OPERAND + j < INSTRUCTIONS ? wave * PER_OPERAND + j : INSTRUCTIONS - 1;
+        const int dst = number * 1024;
+        __builtin_amdgcn_global_load_lds((ap_global_ptr)(k_pool + offset), (ap_lds_ptr)(stage + dst),
+                                         16, 0, 0);
+        __builtin_amdgcn_global_load_lds((ap_global_ptr)(v_pool + offset),
+                                         (ap_lds_ptr)(stage + TILE_BYTES + dst), 16, 0, 0);
+      }
+    }
+  };
+  // Codes: a lane's pieces of a tile are asked for two tiles ahead, and one tile ahead they become values in LDS.
+  constexpr int GROUPS = (HD + PS_INT4_GROUP - 1) / PS_INT4_GROUP;
+  uint32_t k_codes[PER_OPERAND], v_codes[PER_OPERAND][4];
+  uint16_t k_steps[PER_OPERAND], v_steps[PER_OPERAND];
+  auto fetch = [&](int k0) {
+    if constexpr (Pages::INT4) {
+      const uint8_t* k_at[PER_OPERAND];
+      const uint8_t* v_at[PER_OPERAND];
+      int rows[PER_OPERAND];
+#pragma unroll
+      for (int j = 0; j < PER_OPERAND; ++j) {
+        uint32_t page_row;
+        int within;
+        place_of(j, k0, page_row, within);
+        const uint64_t at = (uint64_t)page_row * (18 * GROUPS);
+        k_at[j] = k_pool + at;
+        v_at[j] = v_pool + at;
+        rows[j] = within;
+      }
+#pragma unroll
+      for (int j = 0; j < PER_OPERAND; ++j) {
+        const int g = load_piece[j] >> 2, c = load_piece[j] & 3;
+        const int row = rows[j] * (16 * GROUPS);
+        const int steps = page_size * (16 * GROUPS) + 2 * (rows[j] * GROUPS + g);
+        k_codes[j] = *reinterpret_cast<const uint32_t*>(k_at[j] + row + 4 * (c * GROUPS + g));
+        k_steps[j] = *reinterpret_cast<const uint16_t*>(k_at[j] + steps);
+        const uint8_t* from = v_at[j] + row + 4 * c * GROUPS;
+        if constexpr (GROUPS == 1) {
+          v_codes[j][0] = *reinterpret_cast<const uint32_t*>(from);
+        } else if constexpr (GROUPS == 2) {
+          const uint2 both = *reinterpret_cast<const uint2*>(from);
+          v_codes[j][0] = both.x;
+          v_codes[j][1] = both.y;
+        } else if constexpr (GROUPS == 4) {
+          const uint4 all = *reinterpret_cast<const uint4*>(from);
+          v_codes[j][0] = all.x;
+          v_codes[j][1] = all.y;
+          v_codes[j][2] = all.z;
+          v_codes[j][3] = all.w;
+        } else {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) v_codes[j][b] = from[b * GROUPS + g];
+        }
+        v_steps[j] = *reinterpret_cast<const uint16_t*>(v_at[j] + steps);
+      }
+    }
+  };
+  // eight codes as the bfloat16 values that they stand for, exactly
+  auto values_of = [&](uint32_t codes, float step) {
+    const float base = -8.f * step;
+    const uint32_t even = codes & 0x0f0f0f0fu, odd = codes >> 4 & 0x0f0f0f0fu;
+    u32x4 words;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      words[i] = pack2_bf16(fmaf((float)(even >> (8 * i) & 0xffu), step, base),
+                            fmaf((float)(odd >> (8 * i) & 0xffu), step, base));
+    return words;
+  };
+  auto store = [&](int tile_number) {
+    if constexpr (Pages::INT4) {
+      unsigned char* stage = stages + (tile_number % STAGES) * STAGE_BYTES;
+#pragma unroll
+      for (int j = 0; j < PER_OPERAND; ++j) {
+        const int number = wave * PER_OPERAND + j < INSTRUCTIONS ? wave * PER_OPERAND + j : INSTRUCTIONS - 1;
+        const int g = load_piece[j] >> 2;
+        uint32_t v_word;
+        if constexpr (GROUPS == 1) v_word = v_codes[j][0];
+        else if constexpr (GROUPS == 2) v_word = __builtin_amdgcn_perm(v_codes[j][1], v_codes[j][0], g ? 0x07050301u : 0x06040200u);
+        else if constexpr (GROUPS == 4) {
+          const uint32_t pick = 0x0c0c0400u + 0x0101u * g;
+          v_word = __builtin_amdgcn_perm(v_codes[j][1], v_codes[j][0], pick) |
+                   __builtin_amdgcn_perm(v_codes[j][3], v_codes[j][2], pick) << 16;
+        } else {
+          v_word = v_codes[j][0] | v_codes[j][1] << 8 | v_codes[j][2] << 16 | v_codes[j][3] << 24;
+        }
+        // A value that is no number must not reach the queries that do not see its key, whose weight of 0 would
+        // still make it one: it is 0 here, and the key takes its place, whose scores are masked.
+        const uint32_t k_bits = k_steps[j], v_bits = v_steps[j];
+        const bool number_held = (v_bits & 0x7fffu) <= 0x7f80u;
+        const float k_step = __uint_as_float((number_held ? k_bits : v_bits) << 16);
+        const float v_step = __uint_as_float(number_held ? v_bits << 16 : 0u);
+        *reinterpret_cast<u32x4*>(stage + number * 1024 + lane * 16) = values_of(k_codes[j], k_step);
+        *reinterpret_cast<u32x4*>(stage + TILE_BYTES + number * 1024 + lane * 16) = values_of(v_word, v_step);
+      }
     }
   };
 
@@ -257,9 +364,15 @@ __device__ __forceinline__ void attention_prefill_block(
   // (and with them for every tile in flight) inside the loop
 #pragma unroll
   for (int step = 0; step < NDB; ++step) asm volatile("" : "+v"(qf[step]));
+  if constexpr (Pages::INT4) {
+    fetch(k_first);
+    store(0);
+    if (tiles > 1) fetch(k_first + AP_KEYS);
+  } else {
 #pragma unroll
-  for (int d = 0; d < STAGES - 1; ++d)
-    if (d < tiles) issue(d, k_first + d * AP_KEYS);
+    for (int d = 0; d < STAGES - 1; ++d)
+      if (d < tiles) issue(d, k_first + d * AP_KEYS);
+  }
 
   // ---- the parts of an iteration
   typedef u32x4 KeyRegs[KR][NDB];
@@ -406,13 +519,20 @@ __device__ __forceinline__ void attention_prefill_block(
 
   for (int t = 0; t < tiles; ++t) {
     const int k0 = k_first + t * AP_KEYS;
-    const int ahead = tiles - 1 - t < STAGES - 2 ? tiles - 1 - t : STAGES - 2;
-    if (ahead <= 0) ap_wait_loads_and_sync<0>();
-    else if (ahead == 1) ap_wait_loads_and_sync<LOADS>();
-    else ap_wait_loads_and_sync<2 * LOADS>();
-    // the stage that the tile before this one lay in is free since the barrier: the tile that
-    // is STAGES - 1 ahead is asked for at once
-    if (t + STAGES - 1 < tiles) issue(t + STAGES - 1, k0 + (STAGES - 1) * AP_KEYS);
+    if constexpr (Pages::INT4) {
+      // this tile's values have been written by every wave, and the tile before it has been read
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (t + 1 < tiles) store(t + 1);
+      if (t + 2 < tiles) fetch(k0 + 2 * AP_KEYS);
+    } else {
+      const int ahead = tiles - 1 - t < STAGES - 2 ? tiles - 1 - t : STAGES - 2;
+      if (ahead <= 0) ap_wait_loads_and_sync<0>();
+      else if (ahead == 1) ap_wait_loads_and_sync<LOADS>();
+      else ap_wait_loads_and_sync<2 * LOADS>();
+      // the stage that the tile before this one lay in is free since the barrier: the tile that
+      // is STAGES - 1 ahead is asked for at once
+      if (t + STAGES - 1 < tiles) issue(t + STAGES - 1, k0 + (STAGES - 1) * AP_KEYS);
+    }
     const int kw = wave_keys(t);
     if (!sees(kw)) continue;
     const uint32_t stage_base = stage_of(t);

@@ -288,6 +288,42 @@ int ps_attention_prefill_table_max(void);
 int ps_sample(const float* logits, int64_t ld, const float* inv_temperature, const float* uniform,
               int* tokens, int rows, int vocab, void* stream);
 
+// ---- a cache in 4 bits (cache_int4.h: groups of 32 dimensions with a step each, 18 bytes a group) ----
+// Pools: bytes [pages, kv_heads, page_size, 18 * ceil(head_dim / 32)], pages of a multiple of 8 keys, from a multiple of 16
+// bytes on.  k, v: [tokens, kv_heads * head_dim] of `dtype` with row strides of their own.  head_dim: 1 to 256.
+// Tokens whose position has no page in the pool are passed over.
+int ps_kv_write_int4(const void* k, const void* v, int64_t k_stride, int64_t v_stride, void* k_pool,
+                     void* v_pool, const int* tok_item, const int* tok_pos, const int* tables,
+                     int table_width, int tokens, int kv_heads, int head_dim, int page_size,
+                     int num_pages, int dtype, void* stream);
+int ps_kv_read_int4(const void* k_pool, const void* v_pool, void* k, void* v, int64_t k_stride,
+                    int64_t v_stride, const int* tok_item, const int* tok_pos, const int* tables,
+                    int table_width, int tokens, int kv_heads, int head_dim, int page_size,
+                    int num_pages, int dtype, void* stream);
+// ps_attention_decode over such a cache (q and out of `dtype`; no gate, no logistic weights): `partial` is scratch of
+// count * heads * splits * (head_dim + 2) floats, unused with one range.  A token that sees nothing gets zeros.
+int ps_attention_decode_int4(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool,
+                             void* out, int64_t out_stride, float* partial, int64_t partial_floats,
+                             const int* tok_list, const int* tok_item, const int* tok_pos,
+                             const int* tables, int table_width, int count, int heads, int kv_heads,
+                             int head_dim, int page_size, int num_pages, float scale, int window,
+                             int splits, const float* sink, float softcap, int dtype, void* stream);
+// ps_attention_prefill over such a cache (bfloat16 q and out).
+int ps_attention_prefill_int4(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool,
+                              void* out, int64_t out_stride, const int* tile_item, const int* tile_q0,
+                              int tiles, const int* cu_tokens, const int* kv_lens, const int* tables,
+                              int table_width, int heads, int kv_heads, int head_dim, int page_size,
+                              int num_pages, float scale, int window, int max_kv_len, int query_tile,
+                              const float* sink, float softcap, void* stream);
+
+// logprobs[r] = log softmax(logits[r])[tokens[r]] of rows `ld` apart, of `dtype`.  entropy, ranks, top_ids, top_logprobs: null, or what
+// is wanted of them (the two last [rows, top], top up to 32).  A token of -1: none (0, rank -1); others outside the vocabulary: NaN, -1.
+// partial: scratch of ps_logprob_scratch(rows, vocab, top) floats.
+int ps_token_logprobs(const void* logits, int64_t ld, int rows, int vocab, const int* tokens,
+                      float* logprobs, float* entropy, int* ranks, int* top_ids, float* top_logprobs,
+                      int top, float* partial, int64_t partial_floats, int dtype, void* stream);
+int64_t ps_logprob_scratch(int rows, int vocab, int top);
+
 // Record the launches issued on `stream` between begin and end into an executable graph.
 int ps_graph_begin(void* stream);
 int ps_graph_end(void* stream, void** exec_out, int* node_count);

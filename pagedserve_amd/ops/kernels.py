@@ -147,6 +147,18 @@ _SIGNATURES = {
     "ps_state_output": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
                         c_void_p, c_int, c_float, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int,
                         c_void_p],
+    "ps_kv_write_int4": [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                         c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    "ps_kv_read_int4": [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int,
+                        c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    "ps_attention_decode_int4": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                 c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                 c_float, c_int, c_int, c_void_p, c_float, c_int, c_void_p],
+    "ps_attention_prefill_int4": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int,
+                                  c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
+                                  c_int, c_int, c_int, c_void_p, c_float, c_void_p],
+    "ps_token_logprobs": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                          c_int, c_void_p, c_int64, c_int, c_void_p],
     "ps_sample": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
 }
 
@@ -1271,6 +1283,159 @@ def attention_mixed(q, k_pool, v_pool, out, tok_list, tok_item, positions, tile_
     return out
 
 
+# ---- a cache in 4 bits (csrc/cache_int4.h says how a page holds its keys and values)
+INT4_GROUP = 32          # head dimensions that share a step
+INT4_PAGE_KEYS = 8       # a page's keys are a multiple of this many
+
+
+def int4_row_bytes(head_dim: int) -> int:
+    """Bytes of one key (or value) of one head: 16 of codes and a step of 2 for every group of 32 dimensions."""
+    return 18 * -(-head_dim // INT4_GROUP)
+
+
+def _one_device(what, *tensors):
+    """All tensors lie on one device, which is the current one: kernels are launched on its stream."""
+    devices = {tensor.device for tensor in tensors if tensor is not None}
+    if len(devices) != 1:
+        raise KernelError(f"{what}: tensors on {', '.join(sorted(map(str, devices)))}; one device is needed")
+    device = devices.pop()
+    if device.type == "cuda" and device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensors on {device}, the current device is {torch.cuda.current_device()}")
+
+
+def _check_int4_pools(k_pool, v_pool, columns, heads=None):
+    """(pages, key/value heads, page size, head size) of pools ``[pages, kv_heads, page_size,
+    int4_row_bytes(head_dim)]`` of bytes, for rows of ``columns`` values of ``heads`` heads (None: of the pools' own)."""
+    _check(k_pool, "k_pool", torch.uint8, 4)
+    _check(v_pool, "v_pool", torch.uint8, 4)
+    if k_pool.shape != v_pool.shape or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise KernelError("key and value pools must be contiguous and of one shape")
+    pages, kv_heads, page_size, row = k_pool.shape
+    if 0 in k_pool.shape:
+        raise KernelError(f"the pools of a cache in 4 bits are empty: {tuple(k_pool.shape)}")
+    if (k_pool.data_ptr() | v_pool.data_ptr()) % 16:
+        raise KernelError("the pools of a cache in 4 bits must begin at multiples of 16 bytes")
+    if page_size % INT4_PAGE_KEYS:
+        raise KernelError(f"pages of a cache in 4 bits hold a multiple of {INT4_PAGE_KEYS} keys, not {page_size}")
+    count = kv_heads if heads is None else heads
+    if count <= 0 or columns % count or not 0 < columns // count <= 256 or row != int4_row_bytes(columns // count):
+        raise KernelError(f"rows of {columns} values of {count} heads do not fit pools of {row} bytes a key "
+                          f"({INT4_GROUP} dimensions take 18)")
+    return pages, kv_heads, page_size, columns // count
+
+
+def _int4_rows(what, k, v, k_pool, v_pool, tok_item, tok_pos, tables):
+    _check(k, "k", ndim=2)
+    _check(v, "v", k.dtype, 2)
+    if v.shape != k.shape:
+        raise KernelError(f"{what}: k and v must share a shape")
+    pages, kv_heads, page_size, head_dim = _check_int4_pools(k_pool, v_pool, k.shape[1])
+    _check_step_index(tok_item, tok_pos, tables, k.shape[0])
+    _one_device(what, k, v, k_pool, v_pool, tok_item, tok_pos, tables)
+    return (_rows(k, "k"), _rows(v, "v"), k_pool.data_ptr(), v_pool.data_ptr(), tok_item.data_ptr(), tok_pos.data_ptr(),
+            tables.data_ptr(), tables.shape[1], k.shape[0], kv_heads, head_dim, page_size, pages, dtype_code(k.dtype))
+
+
+def kv_write_int4(k, v, k_pool, v_pool, tok_item, tok_pos, tables):
+    """Store rows of k and v ([tokens, kv_heads*head_dim], float or bfloat16, row strides of their own) at their positions' pages
+    in 4 bits: per 32 dimensions a step ``d`` (an eighth of the largest magnitude, rounded to five bits) and codes
+    ``clamp(rint(x / d), -8, 7) + 8``.  ``(code - 8) d`` is a bfloat16 number exactly.  A group with an infinity or a NaN in it is
+    held as NaN.  Tokens without a page (a table entry outside the pool) are not stored, as in ``kv_write``; no two
+    tokens of a call may have one place."""
+    k_stride, v_stride, k_at, v_at, *index = _int4_rows("kv_write_int4", k, v, k_pool, v_pool, tok_item, tok_pos, tables)
+    _call("ps_kv_write_int4", k.data_ptr(), v.data_ptr(), k_stride, v_stride, k_at, v_at, *index, _stream())
+
+
+def kv_read_int4(k_pool, v_pool, k, v, tok_item, tok_pos, tables):
+    """The values that a cache in 4 bits holds for tokens, into rows of k and v ([tokens, kv_heads*head_dim]); rows of
+    tokens without a page are left as they were."""
+    k_stride, v_stride, k_at, v_at, *index = _int4_rows("kv_read_int4", k, v, k_pool, v_pool, tok_item, tok_pos, tables)
+    _call("ps_kv_read_int4", k_at, v_at, k.data_ptr(), v.data_ptr(), k_stride, v_stride, *index, _stream())
+
+
+def int4_decode_splits(dtype, count, heads, kv_heads, head_dim, visible) -> int:
+    """Ranges per request that ``attention_decode_int4`` best cuts its keys into: ``count`` tokens, none of which sees more
+    than ``visible`` keys."""
+    units = compute_units()
+    blocks = max(1, count * heads)
+    return max(1, min(-(-4 * units // blocks), -(-visible // 128), 64))
+
+
+def attention_decode_int4(q, k_pool, v_pool, out, tok_item, tok_pos, tables, heads, scale, splits, partial=None,
+                          window=0, tok_list=None, sink=None, softcap=0.0):
+    """``attention_decode`` over a cache in 4 bits, any head size up to 256, float or bfloat16 queries: the same attention over
+    the values that the cache stands for.  ``partial``: float scratch of ``count * heads * splits * (head_dim + 2)``
+    values when ``splits > 1``.  A token that sees no key gets zeros."""
+    _check(q, "q", ndim=2)
+    _check(out, "out", q.dtype, 2)
+    pages, kv_heads, page_size, head_dim = _check_int4_pools(k_pool, v_pool, q.shape[1], heads)
+    if out.shape != q.shape:
+        raise KernelError("attention_decode_int4: q and out rows must hold heads x head_dim values")
+    _check_step_index(tok_item, tok_pos, tables, q.shape[0], direct_items=True)
+    count = q.shape[0]
+    if tok_list is not None:
+        _check(tok_list, "tok_list", torch.int32, 1)
+        if not tok_list.is_contiguous():
+            raise KernelError("attention_decode_int4: tok_list must be contiguous")
+        count = tok_list.numel()
+    floats = 0
+    if splits > 1:
+        _check(partial, "partial", torch.float32)
+        if not partial.is_contiguous():
+            raise KernelError("attention_decode_int4: scratch must be contiguous")
+        floats = partial.numel()
+    _one_device("attention_decode_int4", q, k_pool, v_pool, out, tok_item, tok_pos, tables, tok_list, sink,
+                partial if splits > 1 else None)
+    _call("ps_attention_decode_int4", q.data_ptr(), _rows(q, "q"), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(),
+          _rows(out, "out"), _ptr(partial if splits > 1 else None), floats, _ptr(tok_list), _ptr(tok_item),
+          tok_pos.data_ptr(), tables.data_ptr(), tables.shape[1], count, heads, kv_heads, head_dim, page_size, pages,
+          float(scale), int(window), int(splits), _check_sink(sink, heads), _check_cap(softcap), dtype_code(q.dtype),
+          _stream())
+    return out
+
+
+def prefill_int4_supported(dtype, head_dim, table_width=0) -> bool:
+    """Whether ``attention_prefill_int4`` takes this type, head size and width of the block tables; what it does not take
+    goes through ``attention_decode_int4``, token by token."""
+    return prefill_supported(dtype, head_dim, table_width)
+
+
+def prefill_int4_tile(heads, head_dim, tiles, max_kv_len=0) -> int:
+    """Queries per tile for ``attention_prefill_int4``: ``tiles`` maps each size (64, 32, 128) to the number of tiles
+    that a step's portions make of it.  The lines are those of the other cache's kernel."""
+    if prefill_small_tile_pays(heads, head_dim, tiles[PREFILL_TILE]):
+        return PREFILL_SMALL_TILE
+    if prefill_large_tile_pays(heads, head_dim, tiles[PREFILL_LARGE_TILE], max_kv_len):
+        return PREFILL_LARGE_TILE
+    return PREFILL_TILE
+
+
+def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_lens, tables, heads, scale,
+                           window=0, max_kv_len=0, query_tile=PREFILL_TILE, sink=None, softcap=0.0):
+    """``attention_prefill`` over a cache in 4 bits (bfloat16 queries, head sizes in multiples of 16)."""
+    _check_prefill_constants()
+    _check(q, "q", torch.bfloat16, 2)
+    _check(out, "out", torch.bfloat16, 2)
+    pages, kv_heads, page_size, head_dim = _check_int4_pools(k_pool, v_pool, q.shape[1], heads)
+    if out.shape != q.shape:
+        raise KernelError("attention_prefill_int4: q and out rows must hold heads x head_dim values")
+    for name, tensor in (("tile_item", tile_item), ("tile_q0", tile_q0), ("cu_tokens", cu_tokens), ("kv_lens", kv_lens)):
+        _check(tensor, name, torch.int32, 1)
+        if not tensor.is_contiguous():
+            raise KernelError(f"attention_prefill_int4: {name} must be contiguous")
+    _check(tables, "tables", torch.int32, 2)
+    tiles, items = tile_item.numel(), kv_lens.numel()
+    if tile_q0.numel() != tiles or cu_tokens.numel() != items + 1 or tables.shape[0] != items \
+            or not tables.is_contiguous():
+        raise KernelError("attention_prefill_int4: inconsistent tile or item arrays")
+    _one_device("attention_prefill_int4", q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_lens, tables, sink)
+    _call("ps_attention_prefill_int4", q.data_ptr(), _rows(q, "q"), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(),
+          _rows(out, "out"), tile_item.data_ptr(), tile_q0.data_ptr(), tiles, cu_tokens.data_ptr(), kv_lens.data_ptr(),
+          tables.data_ptr(), tables.shape[1], heads, kv_heads, head_dim, page_size, pages, float(scale), int(window),
+          int(max_kv_len), int(query_tile), _check_sink(sink, heads), _check_cap(softcap), _stream())
+    return out
+
+
 def _float_rows(tensor, name, rows, columns):
     _check(tensor, name, torch.float32, 2)
     if tensor.shape[0] < rows or tensor.shape[1] != columns or not tensor.is_contiguous():
@@ -2382,6 +2547,62 @@ def sample(logits, inv_temperature, uniform, out):
             raise KernelError("sample: one temperature and one uniform number per row are needed")
     _call("ps_sample", logits.data_ptr(), ld, _ptr(inv_temperature), _ptr(uniform),
           out.data_ptr(), rows, vocab, _stream())
+    return out
+
+
+MAX_TOP = 32     # alternatives that ``token_logprobs`` gives, at most
+
+
+def logprob_scratch(rows, vocab, top) -> int:
+    """Floats of scratch that ``token_logprobs`` needs for rows of that size (0: none)."""
+    fn = load_library().ps_logprob_scratch
+    fn.argtypes, fn.restype = [c_int, c_int, c_int], c_int64
+    return fn(rows, vocab, top)
+
+
+def token_logprobs(logits, tokens, out, entropy=None, ranks=None, top_ids=None, top_logprobs=None, partial=None):
+    """out[r] = log softmax(logits[r])[tokens[r]] (float or bfloat16 logits, rows of any stride, one token each).
+
+    ``entropy``: the entropy of each row's distribution, in natural units.  ``ranks``: how many tokens of the row are
+    more likely than the given one (among equals the lower ids are).  ``top_ids`` and ``top_logprobs`` ([rows, top], int32 and float, top
+    up to 32): the row's most likely tokens and their log probabilities, the lower id first among equals.  ``partial``: float
+    scratch of ``logprob_scratch(rows, vocab, top)`` values.
+
+    A row whose token is -1 has none: log probability 0, rank -1.  Any other token outside the vocabulary gives NaN and -1.
+    Logits of minus infinity are tokens that cannot come; a row of nothing else, or with a NaN or an infinity above, has NaN
+    for its log probabilities and its entropy."""
+    _check(logits, "logits", ndim=2)
+    rows, vocab = logits.shape
+    ld = _rows(logits, "logits")
+    for name, tensor, dtype in (("tokens", tokens, torch.int32), ("out", out, torch.float32),
+                                ("entropy", entropy, torch.float32), ("ranks", ranks, torch.int32)):
+        if tensor is None and name in ("entropy", "ranks"):
+            continue
+        _check(tensor, name, dtype, 1)
+        if tensor.numel() < rows or not tensor.is_contiguous():
+            raise KernelError(f"token_logprobs: {name} needs an entry per row ({rows}), contiguous")
+    if (top_ids is None) != (top_logprobs is None):
+        raise KernelError("token_logprobs: alternatives are ids and log probabilities, both or neither")
+    top = 0
+    if top_ids is not None:
+        _check(top_ids, "top_ids", torch.int32, 2)
+        _check(top_logprobs, "top_logprobs", torch.float32, 2)
+        top = top_ids.shape[1]
+        if top_ids.shape != top_logprobs.shape or top_ids.shape[0] != rows \
+                or not (top_ids.is_contiguous() and top_logprobs.is_contiguous()):
+            raise KernelError(f"token_logprobs: alternatives must be contiguous [{rows}, top]")
+        if top > min(MAX_TOP, vocab):
+            raise KernelError(f"token_logprobs: {top} alternatives out of {vocab} tokens; at most {MAX_TOP}")
+    floats = 0
+    if partial is not None:
+        _check(partial, "partial", torch.float32)
+        if not partial.is_contiguous():
+            raise KernelError("token_logprobs: scratch must be contiguous")
+        floats = partial.numel()
+    _one_device("token_logprobs", logits, tokens, out, entropy, ranks, top_ids, top_logprobs, partial)
+    _call("ps_token_logprobs", logits.data_ptr(), ld, rows, vocab, tokens.data_ptr(), out.data_ptr(), _ptr(entropy),
+          _ptr(ranks), _ptr(top_ids) if top else 0, _ptr(top_logprobs) if top else 0, top, _ptr(partial), floats,
+          dtype_code(logits.dtype), _stream())
     return out
 
 
