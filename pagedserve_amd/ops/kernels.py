@@ -192,7 +192,8 @@ _STREAM_HANDLE = None
 def _stream():
     if _STREAM_HANDLE is not None:
         return _STREAM_HANDLE
-    return torch.cuda.current_stream().cuda_stream
+    # (the handle that torch.cuda.current_stream().cuda_stream gives, without the objects around it: 0.3 of 2.5 us)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 class on_stream:
@@ -1293,27 +1294,53 @@ def int4_row_bytes(head_dim: int) -> int:
     return 18 * -(-head_dim // INT4_GROUP)
 
 
-def _one_device(what, *tensors):
-    """All tensors lie on one device, which is the current one: kernels are launched on its stream."""
-    devices = {tensor.device for tensor in tensors if tensor is not None}
-    if len(devices) != 1:
-        raise KernelError(f"{what}: tensors on {', '.join(sorted(map(str, devices)))}; one device is needed")
-    device = devices.pop()
-    if device.type == "cuda" and device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: tensors on {device}, the current device is {torch.cuda.current_device()}")
+def _one_device(what, first):
+    """The device of a call's first tensor, which must be the current one: kernels are launched on its stream."""
+    device = first.get_device()
+    if device >= 0 and device != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: tensors on {first.device}, the current device is {torch.cuda.current_device()}")
+    return device
 
 
-def _check_int4_pools(k_pool, v_pool, columns, heads=None):
-    """(pages, key/value heads, page size, head size) of pools ``[pages, kv_heads, page_size,
+def _dense(tensor, name, dtype, ndim, device):
+    """A contiguous tensor of this type on a call's device; its address.  (One question after the other costs a decode
+    step's launches more than the GPU needs for them: what is wrong is found out only where something is.)"""
+    try:
+        if tensor.dtype is dtype and tensor.dim() == ndim and tensor.is_contiguous() and tensor.get_device() == device:
+            return tensor.data_ptr()
+    except AttributeError:
+        pass
+    _check(tensor, name, dtype, ndim)
+    if tensor.get_device() != device:
+        raise KernelError(f"{name} is on {tensor.device}, not on the device of the call's other tensors")
+    raise KernelError(f"{name} must be contiguous")
+
+
+def _rows_on(tensor, name, dtype, device):
+    """Rows of this type on a call's device; (address, row stride)."""
+    try:
+        if tensor.dtype is dtype and tensor.dim() == 2 and tensor.get_device() == device:
+            if tensor.is_contiguous():
+                return tensor.data_ptr(), max(1, tensor.size(1))
+            return tensor.data_ptr(), _rows(tensor, name)
+    except AttributeError:
+        pass
+    _check(tensor, name, dtype, 2)
+    raise KernelError(f"{name} is on {tensor.device}, not on the device of the call's other tensors")
+
+
+def _int4_pools(k_pool, v_pool, columns, heads, device):
+    """(addresses, pages, key/value heads, page size, head size) of pools ``[pages, kv_heads, page_size,
     int4_row_bytes(head_dim)]`` of bytes, for rows of ``columns`` values of ``heads`` heads (None: of the pools' own)."""
-    _check(k_pool, "k_pool", torch.uint8, 4)
-    _check(v_pool, "v_pool", torch.uint8, 4)
-    if k_pool.shape != v_pool.shape or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+    k_at = _dense(k_pool, "k_pool", torch.uint8, 4, device)
+    v_at = _dense(v_pool, "v_pool", torch.uint8, 4, device)
+    shape = k_pool.shape
+    if shape != v_pool.shape:
         raise KernelError("key and value pools must be contiguous and of one shape")
-    pages, kv_heads, page_size, row = k_pool.shape
-    if 0 in k_pool.shape:
-        raise KernelError(f"the pools of a cache in 4 bits are empty: {tuple(k_pool.shape)}")
-    if (k_pool.data_ptr() | v_pool.data_ptr()) % 16:
+    pages, kv_heads, page_size, row = shape
+    if not (pages and kv_heads and page_size and row):
+        raise KernelError(f"the pools of a cache in 4 bits are empty: {tuple(shape)}")
+    if (k_at | v_at) & 15:
         raise KernelError("the pools of a cache in 4 bits must begin at multiples of 16 bytes")
     if page_size % INT4_PAGE_KEYS:
         raise KernelError(f"pages of a cache in 4 bits hold a multiple of {INT4_PAGE_KEYS} keys, not {page_size}")
@@ -1321,19 +1348,41 @@ def _check_int4_pools(k_pool, v_pool, columns, heads=None):
     if count <= 0 or columns % count or not 0 < columns // count <= 256 or row != int4_row_bytes(columns // count):
         raise KernelError(f"rows of {columns} values of {count} heads do not fit pools of {row} bytes a key "
                           f"({INT4_GROUP} dimensions take 18)")
-    return pages, kv_heads, page_size, columns // count
+    return k_at, v_at, pages, kv_heads, page_size, columns // count
+
+
+def _token_index(tok_item, tok_pos, tables, tokens, device, direct_items=False):
+    """Addresses of a step's index arrays and the tables' width; as ``_check_step_index``."""
+    pos_at = _dense(tok_pos, "tok_pos", torch.int32, 1, device)
+    tables_at = _dense(tables, "tables", torch.int32, 2, device)
+    items, width = tables.shape
+    if tok_item is None:
+        if not direct_items:
+            raise KernelError("this kernel needs the item index of every token")
+        if items < tokens:
+            raise KernelError("without item indices the block table needs a row per token")
+        item_at = 0
+    else:
+        item_at = _dense(tok_item, "tok_item", torch.int32, 1, device)
+        if tok_item.size(0) < tokens:
+            raise KernelError("one item index per token is needed, contiguous")
+    if tok_pos.size(0) < tokens:
+        raise KernelError("one position per token is needed")
+    return item_at, pos_at, tables_at, width
 
 
 def _int4_rows(what, k, v, k_pool, v_pool, tok_item, tok_pos, tables):
     _check(k, "k", ndim=2)
-    _check(v, "v", k.dtype, 2)
+    device = _one_device(what, k)
+    dtype = k.dtype
+    k_rows, v_rows = _rows_on(k, "k", dtype, device), _rows_on(v, "v", dtype, device)
+    tokens, columns = k.shape
     if v.shape != k.shape:
         raise KernelError(f"{what}: k and v must share a shape")
-    pages, kv_heads, page_size, head_dim = _check_int4_pools(k_pool, v_pool, k.shape[1])
-    _check_step_index(tok_item, tok_pos, tables, k.shape[0])
-    _one_device(what, k, v, k_pool, v_pool, tok_item, tok_pos, tables)
-    return (_rows(k, "k"), _rows(v, "v"), k_pool.data_ptr(), v_pool.data_ptr(), tok_item.data_ptr(), tok_pos.data_ptr(),
-            tables.data_ptr(), tables.shape[1], k.shape[0], kv_heads, head_dim, page_size, pages, dtype_code(k.dtype))
+    k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, columns, None, device)
+    item_at, pos_at, tables_at, width = _token_index(tok_item, tok_pos, tables, tokens, device)
+    return (k_rows, v_rows, k_at, v_at, item_at, pos_at, tables_at, width, tokens, kv_heads, head_dim, page_size, pages,
+            dtype_code(dtype))
 
 
 def kv_write_int4(k, v, k_pool, v_pool, tok_item, tok_pos, tables):
@@ -1342,15 +1391,17 @@ def kv_write_int4(k, v, k_pool, v_pool, tok_item, tok_pos, tables):
     ``clamp(rint(x / d), -8, 7) + 8``.  ``(code - 8) d`` is a bfloat16 number exactly.  A group with an infinity or a NaN in it is
     held as NaN.  Tokens without a page (a table entry outside the pool) are not stored, as in ``kv_write``; no two
     tokens of a call may have one place."""
-    k_stride, v_stride, k_at, v_at, *index = _int4_rows("kv_write_int4", k, v, k_pool, v_pool, tok_item, tok_pos, tables)
-    _call("ps_kv_write_int4", k.data_ptr(), v.data_ptr(), k_stride, v_stride, k_at, v_at, *index, _stream())
+    (k_from, k_stride), (v_from, v_stride), k_at, v_at, *index = _int4_rows("kv_write_int4", k, v, k_pool, v_pool, tok_item,
+                                                                            tok_pos, tables)
+    _call("ps_kv_write_int4", k_from, v_from, k_stride, v_stride, k_at, v_at, *index, _stream())
 
 
 def kv_read_int4(k_pool, v_pool, k, v, tok_item, tok_pos, tables):
     """The values that a cache in 4 bits holds for tokens, into rows of k and v ([tokens, kv_heads*head_dim]); rows of
     tokens without a page are left as they were."""
-    k_stride, v_stride, k_at, v_at, *index = _int4_rows("kv_read_int4", k, v, k_pool, v_pool, tok_item, tok_pos, tables)
-    _call("ps_kv_read_int4", k_at, v_at, k.data_ptr(), v.data_ptr(), k_stride, v_stride, *index, _stream())
+    (k_to, k_stride), (v_to, v_stride), k_at, v_at, *index = _int4_rows("kv_read_int4", k, v, k_pool, v_pool, tok_item,
+                                                                        tok_pos, tables)
+    _call("ps_kv_read_int4", k_at, v_at, k_to, v_to, k_stride, v_stride, *index, _stream())
 
 
 def int4_decode_splits(dtype, count, heads, kv_heads, head_dim, visible) -> int:
@@ -1367,30 +1418,29 @@ def attention_decode_int4(q, k_pool, v_pool, out, tok_item, tok_pos, tables, hea
     the values that the cache stands for.  ``partial``: float scratch of ``count * heads * splits * (head_dim + 2)``
     values when ``splits > 1``.  A token that sees no key gets zeros."""
     _check(q, "q", ndim=2)
-    _check(out, "out", q.dtype, 2)
-    pages, kv_heads, page_size, head_dim = _check_int4_pools(k_pool, v_pool, q.shape[1], heads)
+    device = _one_device("attention_decode_int4", q)
+    dtype = q.dtype
+    q_at, q_stride = _rows_on(q, "q", dtype, device)
+    out_at, out_stride = _rows_on(out, "out", dtype, device)
+    tokens, columns = q.shape
+    k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, columns, heads, device)
     if out.shape != q.shape:
         raise KernelError("attention_decode_int4: q and out rows must hold heads x head_dim values")
-    _check_step_index(tok_item, tok_pos, tables, q.shape[0], direct_items=True)
-    count = q.shape[0]
+    item_at, pos_at, tables_at, width = _token_index(tok_item, tok_pos, tables, tokens, device, direct_items=True)
+    list_at, count = 0, tokens
     if tok_list is not None:
-        _check(tok_list, "tok_list", torch.int32, 1)
-        if not tok_list.is_contiguous():
-            raise KernelError("attention_decode_int4: tok_list must be contiguous")
-        count = tok_list.numel()
-    floats = 0
+        list_at, count = _dense(tok_list, "tok_list", torch.int32, 1, device), tok_list.size(0)
+    partial_at = floats = 0
     if splits > 1:
         _check(partial, "partial", torch.float32)
-        if not partial.is_contiguous():
-            raise KernelError("attention_decode_int4: scratch must be contiguous")
-        floats = partial.numel()
-    _one_device("attention_decode_int4", q, k_pool, v_pool, out, tok_item, tok_pos, tables, tok_list, sink,
-                partial if splits > 1 else None)
-    _call("ps_attention_decode_int4", q.data_ptr(), _rows(q, "q"), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(),
-          _rows(out, "out"), _ptr(partial if splits > 1 else None), floats, _ptr(tok_list), _ptr(tok_item),
-          tok_pos.data_ptr(), tables.data_ptr(), tables.shape[1], count, heads, kv_heads, head_dim, page_size, pages,
-          float(scale), int(window), int(splits), _check_sink(sink, heads), _check_cap(softcap), dtype_code(q.dtype),
-          _stream())
+        partial_at, floats = _dense(partial, "partial", torch.float32, partial.dim(), device), partial.numel()
+    sink_at = 0
+    if sink is not None:
+        sink_at = _check_sink(sink, heads)
+        _dense(sink, "sink", torch.float32, 1, device)
+    _call("ps_attention_decode_int4", q_at, q_stride, k_at, v_at, out_at, out_stride, partial_at, floats, list_at, item_at,
+          pos_at, tables_at, width, count, heads, kv_heads, head_dim, page_size, pages, float(scale), int(window),
+          int(splits), sink_at, _check_cap(softcap), dtype_code(dtype), _stream())
     return out
 
 
@@ -1415,24 +1465,25 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
     """``attention_prefill`` over a cache in 4 bits (bfloat16 queries, head sizes in multiples of 16)."""
     _check_prefill_constants()
     _check(q, "q", torch.bfloat16, 2)
-    _check(out, "out", torch.bfloat16, 2)
-    pages, kv_heads, page_size, head_dim = _check_int4_pools(k_pool, v_pool, q.shape[1], heads)
+    device = _one_device("attention_prefill_int4", q)
+    q_at, q_stride = _rows_on(q, "q", torch.bfloat16, device)
+    out_at, out_stride = _rows_on(out, "out", torch.bfloat16, device)
+    k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, q.size(1), heads, device)
     if out.shape != q.shape:
         raise KernelError("attention_prefill_int4: q and out rows must hold heads x head_dim values")
-    for name, tensor in (("tile_item", tile_item), ("tile_q0", tile_q0), ("cu_tokens", cu_tokens), ("kv_lens", kv_lens)):
-        _check(tensor, name, torch.int32, 1)
-        if not tensor.is_contiguous():
-            raise KernelError(f"attention_prefill_int4: {name} must be contiguous")
-    _check(tables, "tables", torch.int32, 2)
-    tiles, items = tile_item.numel(), kv_lens.numel()
-    if tile_q0.numel() != tiles or cu_tokens.numel() != items + 1 or tables.shape[0] != items \
-            or not tables.is_contiguous():
+    index = [_dense(tensor, name, torch.int32, 1, device)
+             for name, tensor in (("tile_item", tile_item), ("tile_q0", tile_q0), ("cu_tokens", cu_tokens), ("kv_lens", kv_lens))]
+    tables_at = _dense(tables, "tables", torch.int32, 2, device)
+    tiles, items = tile_item.size(0), kv_lens.size(0)
+    if tile_q0.size(0) != tiles or cu_tokens.size(0) != items + 1 or tables.size(0) != items:
         raise KernelError("attention_prefill_int4: inconsistent tile or item arrays")
-    _one_device("attention_prefill_int4", q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_lens, tables, sink)
-    _call("ps_attention_prefill_int4", q.data_ptr(), _rows(q, "q"), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(),
-          _rows(out, "out"), tile_item.data_ptr(), tile_q0.data_ptr(), tiles, cu_tokens.data_ptr(), kv_lens.data_ptr(),
-          tables.data_ptr(), tables.shape[1], heads, kv_heads, head_dim, page_size, pages, float(scale), int(window),
-          int(max_kv_len), int(query_tile), _check_sink(sink, heads), _check_cap(softcap), _stream())
+    sink_at = 0
+    if sink is not None:
+        sink_at = _check_sink(sink, heads)
+        _dense(sink, "sink", torch.float32, 1, device)
+    _call("ps_attention_prefill_int4", q_at, q_stride, k_at, v_at, out_at, out_stride, index[0], index[1], tiles, index[2],
+          index[3], tables_at, tables.size(1), heads, kv_heads, head_dim, page_size, pages, float(scale), int(window),
+          int(max_kv_len), int(query_tile), sink_at, _check_cap(softcap), _stream())
     return out
 
 
@@ -2572,37 +2623,38 @@ def token_logprobs(logits, tokens, out, entropy=None, ranks=None, top_ids=None, 
     Logits of minus infinity are tokens that cannot come; a row of nothing else, or with a NaN or an infinity above, has NaN
     for its log probabilities and its entropy."""
     _check(logits, "logits", ndim=2)
+    device = _one_device("token_logprobs", logits)
+    dtype = logits.dtype
+    logits_at, ld = _rows_on(logits, "logits", dtype, device)
     rows, vocab = logits.shape
-    ld = _rows(logits, "logits")
-    for name, tensor, dtype in (("tokens", tokens, torch.int32), ("out", out, torch.float32),
-                                ("entropy", entropy, torch.float32), ("ranks", ranks, torch.int32)):
-        if tensor is None and name in ("entropy", "ranks"):
-            continue
-        _check(tensor, name, dtype, 1)
-        if tensor.numel() < rows or not tensor.is_contiguous():
-            raise KernelError(f"token_logprobs: {name} needs an entry per row ({rows}), contiguous")
+
+    def per_row(tensor, name, kind):
+        at = _dense(tensor, name, kind, 1, device)
+        if tensor.size(0) < rows:
+            raise KernelError(f"token_logprobs: {name} needs an entry per row ({rows})")
+        return at
+
+    tokens_at = per_row(tokens, "tokens", torch.int32)
+    out_at = per_row(out, "out", torch.float32)
+    entropy_at = 0 if entropy is None else per_row(entropy, "entropy", torch.float32)
+    ranks_at = 0 if ranks is None else per_row(ranks, "ranks", torch.int32)
     if (top_ids is None) != (top_logprobs is None):
         raise KernelError("token_logprobs: alternatives are ids and log probabilities, both or neither")
-    top = 0
+    top = ids_at = best_at = 0
     if top_ids is not None:
-        _check(top_ids, "top_ids", torch.int32, 2)
-        _check(top_logprobs, "top_logprobs", torch.float32, 2)
-        top = top_ids.shape[1]
-        if top_ids.shape != top_logprobs.shape or top_ids.shape[0] != rows \
-                or not (top_ids.is_contiguous() and top_logprobs.is_contiguous()):
+        ids_at = _dense(top_ids, "top_ids", torch.int32, 2, device)
+        best_at = _dense(top_logprobs, "top_logprobs", torch.float32, 2, device)
+        top = top_ids.size(1)
+        if top_ids.shape != top_logprobs.shape or top_ids.size(0) != rows:
             raise KernelError(f"token_logprobs: alternatives must be contiguous [{rows}, top]")
         if top > min(MAX_TOP, vocab):
             raise KernelError(f"token_logprobs: {top} alternatives out of {vocab} tokens; at most {MAX_TOP}")
-    floats = 0
+    partial_at = floats = 0
     if partial is not None:
         _check(partial, "partial", torch.float32)
-        if not partial.is_contiguous():
-            raise KernelError("token_logprobs: scratch must be contiguous")
-        floats = partial.numel()
-    _one_device("token_logprobs", logits, tokens, out, entropy, ranks, top_ids, top_logprobs, partial)
-    _call("ps_token_logprobs", logits.data_ptr(), ld, rows, vocab, tokens.data_ptr(), out.data_ptr(), _ptr(entropy),
-          _ptr(ranks), _ptr(top_ids) if top else 0, _ptr(top_logprobs) if top else 0, top, _ptr(partial), floats,
-          dtype_code(logits.dtype), _stream())
+        partial_at, floats = _dense(partial, "partial", torch.float32, partial.dim(), device), partial.numel()
+    _call("ps_token_logprobs", logits_at, ld, rows, vocab, tokens_at, out_at, entropy_at, ranks_at,
+          ids_at if top else 0, best_at if top else 0, top, partial_at, floats, dtype_code(dtype), _stream())
     return out
 
 

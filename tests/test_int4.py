@@ -83,7 +83,7 @@ def test_what_they_take(on_gpu):
     ({"tables": _ints(1, 5).long()}, "int32"), ({"tables": _ints(5, 2).t()}, "contiguous"),
     ({"k": torch.zeros(128, 3).t(), "v": torch.zeros(128, 3).t()}, "contiguous rows"),
     ({"k": torch.zeros(3, 128, dtype=torch.float16), "v": torch.zeros(3, 128, dtype=torch.float16)}, "not supported"),
-    ({"tables": torch.zeros(1, 5, dtype=torch.int32, device="meta")}, "one device")])
+    ({"k_pool": None}, "must be a tensor"), ({"v": [1.0]}, "must be a tensor"), ({"tok_pos": _ints(6)[::2]}, "contiguous")])
 @pytest.mark.parametrize("function", [kernels.kv_write_int4, kernels.kv_read_int4])
 def test_rows_refused(on_gpu, function, changed, message):
     if message is None:                                  # 63 dimensions take as many bytes as 64
@@ -92,6 +92,33 @@ def test_rows_refused(on_gpu, function, changed, message):
     with pytest.raises(kernels.KernelError, match=message):
         function(**_write(**changed))
     assert not on_gpu
+
+
+def test_tensors_on_two_devices(on_gpu):
+    """One tensor after the other claims another device than the first one's."""
+    for function, args in ((kernels.kv_write_int4, _write()), (kernels.kv_read_int4, _write()),
+                           (kernels.attention_decode_int4, _decode(tok_list=_ints(2), sink=torch.zeros(4), splits=2,
+                                                                   partial=torch.zeros(4000))),
+                           (kernels.attention_prefill_int4, _prompt(sink=torch.zeros(4))),
+                           (kernels.token_logprobs, _logprobs(entropy=torch.zeros(3), ranks=_ints(3), top_ids=_ints(3, 2),
+                                                              top_logprobs=torch.zeros(3, 2), partial=torch.zeros(9)))):
+        names = [name for name, value in args.items() if isinstance(value, torch.Tensor)]
+        for name in names[1:]:
+            other = args[name]
+            with mock.patch.object(torch.Tensor, "get_device", lambda tensor: -2 if tensor is other else -1):
+                with pytest.raises(kernels.KernelError, match="device"):
+                    function(**args)
+        assert not on_gpu
+        function(**args)
+        on_gpu.clear()
+
+
+def test_tensors_that_are_not_on_the_current_device(on_gpu):
+    with mock.patch.object(torch.Tensor, "get_device", lambda tensor: 1), \
+            mock.patch.object(torch._C, "_cuda_getDevice", lambda: 0, create=True), \
+            mock.patch.object(torch.cuda, "current_device", lambda: 0):
+        with pytest.raises(kernels.KernelError, match="current device is 0"):
+            kernels.kv_write_int4(**_write())
 
 
 @pytest.mark.parametrize("changed,message", [
