@@ -45,6 +45,7 @@ HIPCC_FLAGS = [
 # a tile are level (270 products of 1 to 300 rows 1.000 plain and with GELU, 1.004 added to rows).
 EXTRA_FLAGS = {
     "attention_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "attention_decode_int4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attention_prefill_int4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attention_mixed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attention_tiled_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],

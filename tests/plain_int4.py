@@ -80,11 +80,20 @@ def visible(position, key, window):
     return True
 
 
+def _largest(x):
+    """Every element of [.., dim] replaced by the largest magnitude of its group of 32."""
+    return torch.cat([part.abs().amax(-1, keepdim=True).expand_as(part) for part in x.split(GROUP, dim=-1)], -1)
+
+
 def attention(q, k, v, positions, heads, scale, window=0, sink=None, softcap=0.0):
     """(out, size, shift) in 64 bits for queries [n, heads * dim] at ``positions`` over the keys 0 .. of one request
-    ([length, kv_heads * dim]).  ``size``: the weighted mean of the values' magnitudes; ``shift``: how far float evaluation may
+    ([length, kv_heads * dim]).  ``size``: the weighted mean of the values' magnitudes and, for bfloat16 queries, 2^-7 of the weighted mean
+    of their groups' largest ones: the kernels sum codes with an offset there, 16 + code less 24, at most 40 steps in any partial sum,
+    where a group's largest value has 7 or more.  64 additions of a tile, rounded to 2^-24 of that, are
+    64 * 40 / 7 * 2^-24 = 2^-15.5 of the largest value's share, and ``allowed`` takes 2^-8 of ``size``.  ``shift``: how far float evaluation may
     move a score (a sum of dim products, its scaling and the change to units of log 2), as an exponent."""
     n, length = q.shape[0], k.shape[0]
+    offset = q.dtype == torch.bfloat16
     dim = q.shape[1] // heads
     kv_heads = k.shape[1] // dim
     q = q.double().cpu().view(n, heads, dim)
@@ -97,6 +106,8 @@ def attention(q, k, v, positions, heads, scale, window=0, sink=None, softcap=0.0
         vh = v[:, h // (heads // kv_heads)]
         s = q[:, h] @ kh.T * scale
         absolute = q[:, h].abs() @ kh.nan_to_num(0.0).abs().T * abs(scale)
+        if offset:      # (the same for the scores: partial sums of 40 steps to a query's element, a seventh of its group's largest key)
+            absolute = absolute + q[:, h].abs() @ _largest(kh.nan_to_num(0.0)).T * abs(scale) * 40 / 7
         if softcap:
             s = softcap * torch.tanh(s / softcap)
         s = s.masked_fill(~mask, -math.inf)
@@ -108,6 +119,9 @@ def attention(q, k, v, positions, heads, scale, window=0, sink=None, softcap=0.0
         seen = torch.where(mask.T[None], vh.T[:, :, None], torch.zeros(()).double())          # [dim, length, n]
         out[:, h] = torch.einsum("nl,dln->nd", p, seen)
         size[:, h] = torch.einsum("nl,dln->nd", p, seen.abs())
+        if offset:
+            large = torch.where(mask.T[None], _largest(vh).T[:, :, None], torch.zeros(()).double())
+            size[:, h] += 2.0 ** -7 * torch.einsum("nl,dln->nd", p, large)
         shift[:, h] = moved[:, None]
     if sink is None:
         out[~mask.any(-1)] = 0.0
