@@ -37,47 +37,76 @@ typedef uint32_t int4_u32x4 __attribute__((ext_vector_type(4)));
 #define I4_OFFSET 24.f       // what a code is held as, less what it stands for
 #define I4_SLACK 8.f         // how far (in units of log 2) a score may pass the exponentials' reference
 
-// Words of W consecutive bytes (a power of two) at a multiple of W.
-template <int W>
-__device__ inline void int4_load(const uint8_t* p, uint32_t* words) {
-  if constexpr (W == 1) words[0] = *p;
-  else if constexpr (W == 2) words[0] = *reinterpret_cast<const uint16_t*>(p);
-  else if constexpr (W == 4) words[0] = *reinterpret_cast<const uint32_t*>(p);
-  else if constexpr (W == 8) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    words[0] = v.x;
-    words[1] = v.y;
-  } else {
+// Reads from LDS, at constant distances from an address, that have arrived when they return.  (Written as assembly: the
+// compiler would wait for every load on its way to LDS before a read of its own.)
+typedef __attribute__((address_space(3))) void* int4_lds_ptr;
+typedef const __attribute__((address_space(1))) void* int4_global_ptr;
+typedef uint32_t int4_u32x2 __attribute__((ext_vector_type(2)));
+#define I4_READ2(OP, X, Y, AT, A, B)                                                                              \
+  asm volatile(OP " %0, %2 offset:%3\n\t" OP " %1, %2 offset:%4\n\ts_waitcnt lgkmcnt(0)"                           \
+               : "=&v"(X), "=&v"(Y)                                                                               \
+               : "v"(AT), "n"(A), "n"(B)                                                                          \
+               : "memory")
+#define I4_READ8(OP, X, AT, D, SUB)                                                                               \
+  asm volatile(OP " %0, %8 offset:%9\n\t" OP " %1, %8 offset:%10\n\t" OP " %2, %8 offset:%11\n\t" OP              \
+                  " %3, %8 offset:%12\n\t" OP " %4, %8 offset:%13\n\t" OP " %5, %8 offset:%14\n\t" OP             \
+                  " %6, %8 offset:%15\n\t" OP " %7, %8 offset:%16\n\ts_waitcnt lgkmcnt(0)"                       \
+               : "=&v"(X[0]), "=&v"(X[1]), "=&v"(X[2]), "=&v"(X[3]), "=&v"(X[4]), "=&v"(X[5]), "=&v"(X[6]),       \
+                 "=&v"(X[7])                                                                                      \
+               : "v"(AT), "n"(0), "n"(D), "n"(2 * (D)), "n"(3 * (D)), "n"(SUB), "n"((SUB) + (D)),                 \
+                 "n"((SUB) + 2 * (D)), "n"((SUB) + 3 * (D))                                                       \
+               : "memory")
+// BYTES at `at` and at `at` + SUB, into words of two rows.
+template <int BYTES, int SUB, int FROM = 0>
+__device__ inline void int4_read_pair(uint32_t at, uint32_t* first, uint32_t* second) {
+  if constexpr (BYTES - FROM >= 16 && BYTES % 16 == 0) {
+    int4_u32x4 x, y;
+    I4_READ2("ds_read_b128", x, y, at, FROM, SUB + FROM);
 #pragma unroll
-    for (int i = 0; i < W / 16; ++i) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + 16 * i);
-      words[4 * i] = v.x;
-      words[4 * i + 1] = v.y;
-      words[4 * i + 2] = v.z;
-      words[4 * i + 3] = v.w;
+    for (int i = 0; i < 4; ++i) {
+      first[FROM / 4 + i] = x[i];
+      second[FROM / 4 + i] = y[i];
     }
+    int4_read_pair<BYTES, SUB, FROM + 16>(at, first, second);
+  } else if constexpr (BYTES - FROM >= 8 && BYTES % 8 == 0) {
+    int4_u32x2 x, y;
+    I4_READ2("ds_read_b64", x, y, at, FROM, SUB + FROM);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      first[FROM / 4 + i] = x[i];
+      second[FROM / 4 + i] = y[i];
+    }
+    int4_read_pair<BYTES, SUB, FROM + 8>(at, first, second);
+  } else if constexpr (BYTES - FROM >= 4) {
+    I4_READ2("ds_read_b32", first[FROM / 4], second[FROM / 4], at, FROM, SUB + FROM);
+    int4_read_pair<BYTES, SUB, FROM + 4>(at, first, second);
   }
 }
-// The largest power of two that divides n, 16 at most.
-constexpr int int4_piece(int n) { return n % 16 == 0 ? 16 : n % 8 == 0 ? 8 : n % 4 == 0 ? 4 : n % 2 == 0 ? 2 : 1; }
 
-// Nibbles i and i + 4 of a word as the bfloat16 numbers 16 + nibble, in the low and the high half.
+// Nibbles i and i + 4 of a word as the bfloat16 numbers 16 + nibble, in the low and the high half.  (mask and sixteens:
+// 0x00780078 and 0x41804180 in registers; written out, they would cost an instruction more.)
 template <int I>
-__device__ inline uint32_t int4_pair(uint32_t word) {
+__device__ inline uint32_t int4_pair(uint32_t word, uint32_t mask, uint32_t sixteens) {
   const uint32_t at = I == 0 ? word << 3 : word >> (4 * I - 3);
-  return (at & 0x00780078u) | 0x41804180u;
+  return (at & mask) | sixteens;
 }
 
-// What a wave loads of 32 keys.  Lane (16 c + n): keys n and 16 + n, words c G ..; of keys 4 c .. + 3 and 16 + 4 c .. + 3 their
-// bytes n G .. and all their steps.
+// The largest of three, in one instruction (the library's maxima quiet every operand first).
+__device__ inline float int4_max3(float x, float y, float z) {
+  float high;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(high) : "v"(x), "v"(y), "v"(z));
+  return high;
+}
+
+// A tile of 32 keys in LDS: the rows of the keys' codes, those of the values', the keys' steps and the values'.  It comes there
+// from the pages by loads that pass no register: 16 bytes of codes, 4 of steps to a lane.
 template <int G>
-struct Int4Keys {
-  uint32_t codes[2][G], steps[2][2 * G];
-};
-template <int G>
-struct Int4Values {
-  static constexpr int PIECE = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;       // bytes of a load
-  uint32_t codes[8][G / PIECE], steps[2][2 * G];
+struct Int4Stage {
+  static constexpr int CODES = I4_TILE * 16 * G;               // bytes of the keys' codes, and of the values'
+  static constexpr int STEPS = I4_TILE * 2 * G;                // bytes of the keys' steps, and of the values'
+  static constexpr int STEP_LOADS = (2 * STEPS + 255) / 256;
+  static constexpr int LOADS = G + STEP_LOADS;                 // instructions of a wave
+  static constexpr int BYTES = 2 * CODES + 256 * STEP_LOADS;
 };
 __device__ inline float int4_step_at(const uint32_t* steps, int i) {
   return __uint_as_float(i & 1 ? steps[i / 2] & 0xffff0000u : steps[i / 2] << 16);
@@ -100,17 +129,19 @@ struct Int4Decode {
   const float* sink;
 };
 
-// EVEN: 16 keys from a multiple of 16 on lie in one page (else 8 from a multiple of 8), whose place the scalar unit
-// works out for the wave.
-// dynamic LDS: the waves' maxima and sums [WAVES][16] each, the block's maxima [16], the waves' accumulators
-// [WAVES][heads of the block][32 G]
-template <int G, int WAVES, bool EVEN>
+// EVEN: pages of a power of two, 16 or more: 16 keys from a multiple of 16 on lie in one page (else 8 from a multiple of 8), whose
+// place the scalar unit works out for the wave.
+// dynamic LDS: the waves' maxima and sums [WAVES][16] each, the block's maxima [16], then the waves' rings of DEPTH tiles, in
+// whose place the accumulators [WAVES][heads of the block][32 G] meet at the end
+template <int G, int WAVES, bool EVEN, int DEPTH>
 __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel(const Int4Decode a) {
-  extern __shared__ __attribute__((aligned(16))) float lds[];
+  typedef Int4Stage<G> Stage;
+  extern __shared__ __attribute__((aligned(1024))) float lds[];
   float* s_m = lds;
   float* s_l = lds + WAVES * I4_HEADS;
   float* s_block = lds + 2 * WAVES * I4_HEADS;
   float* s_acc = s_block + I4_HEADS;
+  unsigned char* stages = reinterpret_cast<unsigned char*>(s_acc);      // (the accumulators come when no tile is left)
   const int index = blockIdx.x, split = blockIdx.z;
   const int kv_head = blockIdx.y / a.parts, part = blockIdx.y - kv_head * a.parts;
   const int t = a.tok_list ? a.tok_list[index] : index;
@@ -123,118 +154,11 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
   const int head0 = kv_head * kv_group + part * a.block_heads;
   const int left = kv_group - part * a.block_heads, count = left < a.block_heads ? left : a.block_heads;
 
-  const int first = pos < 0 ? 0 : first_visible_key(pos, a.window);
-  const int64_t room = (int64_t)a.table_width * a.page_size;
-  const int end_key = pos + 1 < room ? pos + 1 : (int)room;
-  int begin = first & ~(I4_TILE - 1), end = end_key;
-  if (a.splits > 1) {
-    int chunk = (end - begin + a.splits - 1) / a.splits;
-    chunk = (chunk + I4_TILE * WAVES - 1) / (I4_TILE * WAVES) * (I4_TILE * WAVES);
-    begin += split * chunk;
-    if (begin + chunk < end) end = begin + chunk;
-  }
-
-  // the pages of a tile's units of 8 (EVEN: 16) keys, and which of them exist
-  constexpr int UNITS = EVEN ? 2 : 4, UNIT = I4_TILE / UNITS;
-  struct Entries {
-    int page[UNITS];
-  };
-  auto logical_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size; };
-  auto unit_key = [&](int base, int u) { return base + UNIT * u < end ? base + UNIT * u : (end - 1) & ~(UNIT - 1); };
-  auto ask = [&](int base) {
-    Entries e;
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) e.page[u] = scalar_load(table + logical_of(unit_key(base, u)));
-    return e;
-  };
-  auto units_of = [&](const Entries& e) {
-    unsigned units = 0;
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) units |= (unsigned)((unsigned)e.page[u] < (unsigned)a.num_pages) << u;
-    return units;
-  };
-  const int64_t page_bytes = (int64_t)a.page_size * (18 * G);
-  // a unit's first row of codes, and of steps, in bytes from the pool's beginning
-  auto places = [&](const Entries& e, int base, int u, int64_t& code_at, int64_t& step_at) {
-    const int key = unit_key(base, u);
-    const int within = key - logical_of(key) * a.page_size;
-    const int page = (unsigned)e.page[u] < (unsigned)a.num_pages ? e.page[u] : 0;     // a place that exists
-    const int64_t at = ((int64_t)page * a.kv_heads + kv_head) * page_bytes;
-    code_at = at + within * (16 * G);
-    step_at = at + (int64_t)a.page_size * (16 * G) + within * (2 * G);
-  };
-  // where a lane's rows lie within its unit; `half`: which of two units of 8
-  const int key_row = EVEN ? n : n & 7, value_row = EVEN ? 4 * c : 4 * (c & 1);
-  const uint32_t key_lane = key_row * (16 * G) + c * (4 * G), value_lane = value_row * (16 * G) + n * G;
-  const uint32_t step_lane = value_row * (2 * G);
-  auto load_keys = [&](Int4Keys<G>& keys, const Entries& e, int base) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      int64_t code_at, step_at;
-      const uint8_t *codes, *steps;
-      if constexpr (EVEN) {
-        places(e, base, s, code_at, step_at);
-        codes = a.k_pool + code_at;
-        steps = a.k_pool + step_at;
-      } else {
-        int64_t code_2, step_2;
-        places(e, base, 2 * s, code_at, step_at);
-        places(e, base, 2 * s + 1, code_2, step_2);
-        codes = a.k_pool + (n & 8 ? code_2 : code_at);
-        steps = a.k_pool + (c & 2 ? step_2 : step_at);
-      }
-      constexpr int W = int4_piece(4 * G), SW = int4_piece(8 * G);
-#pragma unroll
-      for (int i = 0; i < 4 * G; i += W) int4_load<W>(codes + key_lane + i, keys.codes[s] + i / 4);
-#pragma unroll
-      for (int i = 0; i < 8 * G; i += SW) int4_load<SW>(steps + step_lane + i, keys.steps[s] + i / 4);
-    }
-  };
-  auto load_values = [&](Int4Values<G>& values, const Entries& e, int base) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      int64_t code_at, step_at;
-      const uint8_t *codes, *steps;
-      if constexpr (EVEN) {
-        places(e, base, s, code_at, step_at);
-        codes = a.v_pool + code_at;
-        steps = a.v_pool + step_at;
-      } else {
-        int64_t code_2, step_2;
-        places(e, base, 2 * s, code_at, step_at);
-        places(e, base, 2 * s + 1, code_2, step_2);
-        codes = a.v_pool + (c & 2 ? code_2 : code_at);
-        steps = a.v_pool + (c & 2 ? step_2 : step_at);
-      }
-      constexpr int W = Int4Values<G>::PIECE, SW = int4_piece(8 * G);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int i = 0; i < G / W; ++i) int4_load<W>(codes + value_lane + r * (16 * G) + i * W, values.codes[4 * s + r] + i);
-#pragma unroll
-      for (int i = 0; i < 8 * G; i += SW) int4_load<SW>(steps + step_lane + i, values.steps[s] + i / 4);
-    }
-  };
-
-  int base = begin + wave * I4_TILE;
-  Int4Keys<G> keys;
-  Int4Values<G> values;
-  Entries entries = {};
-  unsigned units = 0;
-  if (base < end) {
-    entries = ask(base);
-    units = units_of(entries);
-    load_keys(keys, entries, base);
-    load_values(values, entries, base);
-    if (base + I4_TILE * WAVES < end) entries = ask(base + I4_TILE * WAVES);
-  }
-
-  // the queries, column n of the products: dimensions 32 g + 8 c + (0, 4, 1, 5, ..), the order of a word's nibbles
-  int4_bf16x8 query[G];
-  int4_f32x4 start[G];
+  uint32_t raw_query[G][4];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    uint32_t raw[4] = {0u, 0u, 0u, 0u};
+    uint32_t (&raw)[4] = raw_query[g];
+    raw[0] = raw[1] = raw[2] = raw[3] = 0u;
     const int d0 = 32 * g + 8 * c;
     if (n < count) {
       const bf16_t* from = a.q + t * a.q_stride + (int64_t)(head0 + n) * a.head_dim + d0;
@@ -252,6 +176,116 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
           if (d0 + i < a.head_dim) raw[i / 2] |= (uint32_t)from[i].bits << (16 * (i & 1));
       }
     }
+  }
+
+  const int first = pos < 0 ? 0 : first_visible_key(pos, a.window);
+  const int64_t room = (int64_t)a.table_width * a.page_size;
+  const int end_key = pos + 1 < room ? pos + 1 : (int)room;
+  int begin = first & ~(I4_TILE - 1), end = end_key;
+  if (a.splits > 1) {
+    int chunk = (end - begin + a.splits - 1) / a.splits;
+    chunk = (chunk + I4_TILE * WAVES - 1) / (I4_TILE * WAVES) * (I4_TILE * WAVES);
+    begin += split * chunk;
+    if (begin + chunk < end) end = begin + chunk;
+  }
+
+  // the pages of a tile's units of 8 (EVEN: 16) keys, and which of them exist
+  constexpr int UNITS = EVEN ? 2 : 4, UNIT = I4_TILE / UNITS;
+  struct Entries {
+    int page[UNITS];
+  };
+  auto logical_of = [&](int key) { return EVEN ? key >> a.page_shift : key / a.page_size; };
+  auto unit_key = [&](int base, int u) { return base + UNIT * u < end ? base + UNIT * u : (end - 1) & ~(UNIT - 1); };
+  auto ask = [&](int base) __attribute__((always_inline)) {
+    Entries e;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) e.page[u] = scalar_load(table + logical_of(unit_key(base, u)));
+    return e;
+  };
+  auto units_of = [&](const Entries& e) {
+    unsigned units = 0;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) units |= (unsigned)((unsigned)e.page[u] < (unsigned)a.num_pages) << u;
+    return units;
+  };
+  const uint64_t page_stride = (uint64_t)a.kv_heads * (unsigned)a.page_size * (18 * G);
+  const int64_t head_at = (int64_t)kv_head * a.page_size * (18 * G), steps_at = (int64_t)a.page_size * (16 * G);
+  // a unit's first row of codes, and of steps, in bytes from the pool's beginning
+  struct Places {
+    int64_t codes[UNITS], steps[UNITS];
+  };
+  auto places = [&](const Entries& e, int base) __attribute__((always_inline)) {
+    Places at;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int key = unit_key(base, u);
+      const int within = EVEN ? key & (a.page_size - 1) : key - logical_of(key) * a.page_size;
+      const unsigned page = (unsigned)e.page[u] < (unsigned)a.num_pages ? e.page[u] : 0u;     // a place that exists
+      const int64_t first_byte = (int64_t)((uint64_t)page * page_stride) + head_at;
+      at.codes[u] = first_byte + within * (16 * G);
+      at.steps[u] = first_byte + steps_at + within * (2 * G);
+    }
+    return at;
+  };
+  auto of_unit = [&](const int64_t (&at)[UNITS], int u) __attribute__((always_inline)) {
+    // (by masks: differences are the scalar unit's, and a selection would keep the array in memory)
+    int64_t found = at[0];
+#pragma unroll
+    for (int i = 1; i < UNITS; ++i) found += (at[i] - at[0]) & -(int64_t)(u == i);
+    return found;
+  };
+  unsigned char* ring = stages + wave * (DEPTH * Stage::BYTES);
+  auto issue = [&](int slot, const Entries& e, int base) __attribute__((always_inline)) {
+    const Places at = places(e, base);
+    unsigned char* stage = ring + slot * Stage::BYTES;
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int piece = j * 64 + lane;
+      const bool is_value = piece >= 32 * G;
+      const int p = is_value ? piece - 32 * G : piece;
+      const int key = p / G, within = p - key * G;
+      const uint8_t* from = (is_value ? a.v_pool : a.k_pool) + of_unit(at.codes, key / UNIT) +
+                            ((key % UNIT) * (16 * G) + within * 16);
+      __builtin_amdgcn_global_load_lds((int4_global_ptr)from, (int4_lds_ptr)(stage + j * 1024), 16, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < Stage::STEP_LOADS; ++j) {
+      const int word = j * 64 + lane < 32 * G ? j * 64 + lane : 32 * G - 1;      // (what is left over repeats the last one)
+      const bool is_value = word >= 16 * G;
+      const int p = is_value ? word - 16 * G : word;
+      constexpr int UNIT_WORDS = UNIT * G / 2;
+      const uint8_t* from =
+          (is_value ? a.v_pool : a.k_pool) + of_unit(at.steps, p / UNIT_WORDS) + 4 * (p % UNIT_WORDS);
+      __builtin_amdgcn_global_load_lds((int4_global_ptr)from, (int4_lds_ptr)(stage + 2 * Stage::CODES + j * 256), 4, 0, 0);
+    }
+  };
+
+  // DEPTH - 1 tiles are on their way while one is worked on; the table's entries are asked for one tile earlier still
+  int base = begin + wave * I4_TILE, ahead = base;
+  constexpr int STRIDE = I4_TILE * WAVES;
+  Entries entries = {};
+  unsigned exist = 0;         // which units of the tiles on their way have a page, four bits a tile, the nearest lowest
+  int on_way = 0;
+  auto send = [&](int slot) __attribute__((always_inline)) {
+    exist |= units_of(entries) << (4 * on_way);
+    issue(slot, entries, ahead);
+    ++on_way;
+    ahead += STRIDE;
+    if (ahead < end) entries = ask(ahead);
+  };
+  if (base < end) {
+    entries = ask(base);
+#pragma unroll
+    for (int i = 0; i < DEPTH - 1; ++i)
+      if (ahead < end) send(i);
+  }
+
+  // the queries, column n of the products: dimensions 32 g + 8 c + (0, 4, 1, 5, ..), the order of a word's nibbles
+  int4_bf16x8 query[G];
+  int4_f32x4 start[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const uint32_t (&raw)[4] = raw_query[g];
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum += __uint_as_float(raw[i] << 16) + __uint_as_float(raw[i] & 0xffff0000u);
@@ -266,30 +300,42 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
   int4_f32x4 acc[G][2];
 #pragma unroll
   for (int g = 0; g < G; ++g) acc[g][0] = acc[g][1] = int4_f32x4{0.f, 0.f, 0.f, 0.f};
+  uint32_t mask = 0x00780078u, sixteens = 0x41804180u;
+  asm volatile("" : "+s"(mask));
+  asm volatile("" : "+v"(sixteens));
   // -24 in all places
   const int4_bf16x8 offsets =
       __builtin_bit_cast(int4_bf16x8, (int4_u32x4){0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u});
 
-  // scores of the lane's 8 keys: 4 c .. + 3 and 16 + 4 c .. + 3, head n; unscaled
-  auto score = [&](float (&s)[8]) {
+  // Lane (16 c + n) reads the words c G .. of keys n and 16 + n, and of keys 4 c .. + 3 and 16 + 4 c .. + 3 the bytes n G .. of
+  // the values and all steps.
+  const uint32_t ring_at = (uint32_t)(uintptr_t)(int4_lds_ptr)ring;
+  const uint32_t key_lane = n * (16 * G) + c * (4 * G), value_lane = Stage::CODES + 4 * c * (16 * G) + n * G;
+  const uint32_t step_lane = 2 * Stage::CODES + 4 * c * (2 * G);
+  // scores of those 8 keys, head n; unscaled
+  auto score = [&](float (&s)[8], uint32_t stage) {
+    uint32_t codes[2][G], steps[2][2 * G];
+    int4_read_pair<4 * G, 256 * G>(stage + key_lane, codes[0], codes[1]);
+    int4_read_pair<8 * G, 32 * G>(stage + step_lane, steps[0], steps[1]);
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const uint32_t w = keys.codes[sub][g];
-        const int4_u32x4 row = {int4_pair<0>(w), int4_pair<1>(w), int4_pair<2>(w), int4_pair<3>(w)};
+        const uint32_t w = codes[sub][g];
+        const int4_u32x4 row = {int4_pair<0>(w, mask, sixteens), int4_pair<1>(w, mask, sixteens), int4_pair<2>(w, mask, sixteens), int4_pair<3>(w, mask, sixteens)};
         const int4_f32x4 dot = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(int4_bf16x8, row), query[g],
                                                                        start[g], 0, 0, 0);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float step = int4_step_at(keys.steps[sub], r * G + g);
+          const float step = int4_step_at(steps[sub], r * G + g);
           s[4 * sub + r] = g == 0 ? dot[r] * step : fmaf(dot[r], step, s[4 * sub + r]);
         }
       }
   };
-  // their weights, and the state that these are relative to
+  // their weights, and the state that these are relative to; capped scores are scaled already
+  const float factor = a.softcap_log2 > 0.f ? 1.f : a.scale_log2;
   auto weigh = [&](float (&s)[8]) {
-    float high = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    const float high = int4_max3(int4_max3(s[0], s[1], s[2]), int4_max3(s[3], s[4], s[5]), int4_max3(s[6], s[7], s[7])) * factor;
     if (__builtin_amdgcn_ballot_w64(high > m + I4_SLACK)) {
       const float m_new = fmaxf(m, halves_max(xor_max<16>(high)));
       reference = m_new == -INFINITY ? 0.f : m_new;
@@ -306,21 +352,27 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(s[i] - reference);
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], factor, -reference));
       l += s[i];
     }
   };
-  auto mix = [&](const float (&p)[8], const bool whole, const unsigned seen) {
+  auto mix = [&](const float (&p)[8], uint32_t stage) {
     // two keys' codes side by side, of as many groups as a half word has bytes
-    constexpr int PIECE = Int4Values<G>::PIECE, BYTES = PIECE >= 2 ? 2 : 1;
+    constexpr int PIECE = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1, BYTES = PIECE >= 2 ? 2 : 1;
+    uint32_t steps[2][2 * G];
+    int4_read_pair<8 * G, 32 * G>(stage + Stage::STEPS + step_lane, steps[0], steps[1]);
+    uint32_t codes[8];
 #pragma unroll
     for (int g0 = 0; g0 < G; g0 += BYTES) {
+      if (g0 % PIECE == 0) {
+        if constexpr (PIECE == 4) I4_READ8("ds_read_b32", codes, stage + value_lane + g0, 16 * G, 256 * G);
+        else if constexpr (PIECE == 2) I4_READ8("ds_read_u16", codes, stage + value_lane + g0, 16 * G, 256 * G);
+        else I4_READ8("ds_read_u8", codes, stage + value_lane + g0, 16 * G, 256 * G);
+      }
       uint32_t both[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t lo = values.codes[2 * j][g0 / PIECE], hi = values.codes[2 * j + 1][g0 / PIECE];
-        both[j] = __builtin_amdgcn_perm(hi, lo, PIECE == 4 && (g0 & 2) ? 0x07060302u : 0x05040100u);
-      }
+      for (int j = 0; j < 4; ++j)
+        both[j] = __builtin_amdgcn_perm(codes[2 * j + 1], codes[2 * j], PIECE == 4 && (g0 & 2) ? 0x07060302u : 0x05040100u);
 #pragma unroll
       for (int b = 0; b < BYTES; ++b) {
         const int g = g0 + b;
@@ -331,13 +383,11 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int i = 2 * j + h;
-            w[h] = p[i] * int4_step_at(values.steps[i >> 2], (i & 3) * G + g);
-            // (what a masked key's step is, nobody knows)
-            if (!whole) w[h] = seen >> i & 1u ? w[h] : 0.f;
+            w[h] = p[i] * int4_step_at(steps[i >> 2], (i & 3) * G + g);
           }
           weights[j] = pack2_bf16(w[0], w[1]);
-          low[j] = b == 0 ? int4_pair<0>(both[j]) : int4_pair<2>(both[j]);
-          high[j] = b == 0 ? int4_pair<1>(both[j]) : int4_pair<3>(both[j]);
+          low[j] = b == 0 ? int4_pair<0>(both[j], mask, sixteens) : int4_pair<2>(both[j], mask, sixteens);
+          high[j] = b == 0 ? int4_pair<1>(both[j], mask, sixteens) : int4_pair<3>(both[j], mask, sixteens);
         }
         const int4_bf16x8 column = __builtin_bit_cast(int4_bf16x8, weights);
         const int4_f32x4 shifted[2] = {__builtin_amdgcn_mfma_f32_16x16x32_bf16(offsets, column, acc[g][0], 0, 0, 0),
@@ -348,41 +398,42 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
     }
   };
 
-  // The keys of the next tile are asked for when this one's scores are made, its values when these are used: each then has
-  // the other half of the work to arrive in, and one set of registers serves.
+  int slot = 0;
   while (base < end) {
-    const int after = base + I4_TILE * WAVES;
+    // the tile in the stage that was read last is on its way again
+    if (ahead < end) send(slot == 0 ? DEPTH - 1 : slot - 1);
+    // the loads of this tile have landed; those behind it are on their way
+    if (on_way == DEPTH) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * Stage::LOADS) : "memory");
+    else if (DEPTH > 2 && on_way == DEPTH - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 2) * Stage::LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const unsigned units = exist & 15u;
     const bool whole = base >= first && base + I4_TILE <= end && units == (1u << UNITS) - 1;
+    const uint32_t stage = ring_at + slot * Stage::BYTES;
     float s[8];
-    score(s);
-    if (after < end) load_keys(keys, entries, after);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] *= a.scale_log2;
+    score(s, stage);
     if (a.softcap_log2 > 0.f) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = capped_score_fast(s[i], a.softcap_log2);
+      for (int i = 0; i < 8; ++i) s[i] = capped_score_fast(s[i] * a.scale_log2, a.softcap_log2);
     }
-    if (whole) {
-      weigh(s);
-      mix(s, true, 0);
-    } else {
-      unsigned seen = 0;
+    if (!whole) {
+      auto visible = [&](int within) {
+        return (base + within >= first) & (base + within < end) & ((units >> (within / UNIT) & 1u) != 0);
+      };
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int within = 16 * (i >> 2) + 4 * c + (i & 3);
-        const bool visible = base + within >= first && base + within < end && (units >> (within / UNIT) & 1u);
-        seen |= (unsigned)visible << i;
-        s[i] = visible ? s[i] : -INFINITY;
+      for (int i = 0; i < 8; ++i) s[i] = visible(16 * (i >> 2) + 4 * c + (i & 3)) ? s[i] : -INFINITY;
+      // nobody knows what a masked key's steps are, and 0 times a NaN is none: the values' steps become 0 where they lie
+      if (lane < I4_TILE && !visible(lane)) {
+        uint16_t* steps = reinterpret_cast<uint16_t*>(ring + slot * Stage::BYTES + 2 * Stage::CODES + Stage::STEPS) + lane * G;
+#pragma unroll
+        for (int g = 0; g < G; ++g) steps[g] = 0;
       }
-      weigh(s);
-      mix(s, false, seen);
     }
-    if (after < end) {
-      units = units_of(entries);
-      load_values(values, entries, after);
-      if (after + I4_TILE * WAVES < end) entries = ask(after + I4_TILE * WAVES);
-    }
-    base = after;
+    weigh(s);
+    mix(s, stage);
+    base += STRIDE;
+    exist >>= 4;
+    --on_way;
+    slot = slot == DEPTH - 1 ? 0 : slot + 1;
   }
 
   // the waves' states meet: maxima first, then sums and accumulators scaled to the block's
@@ -433,22 +484,38 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
   }
 }
 
+// (beyond the 64 KB that a kernel may ask for without saying so)
+static void int4_allow_lds(const void* kernel, int bytes) {
+  if (bytes > 64 * 1024)
+    (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
 template <int G>
 static void launch_heads(const Int4Decode& a, int count, int waves, hipStream_t s) {
+  // tiles in a wave's ring: as many as leave room for the waves that the registers allow
+  constexpr int DEPTH = G <= 2 ? 4 : G <= 4 ? 3 : 2;
   const dim3 grid(count, a.kv_heads * a.parts, a.splits);
-  const int bytes = (I4_HEADS + waves * (2 * I4_HEADS + a.block_heads * 32 * G)) * 4;      // 64 KB at most
-  const bool even = a.page_size % 16 == 0;
-#define PS_LAUNCH_H4(WAVES, EVEN) \
-  hipLaunchKernelGGL((attention_decode_int4_heads_kernel<G, WAVES, EVEN>), grid, dim3(64 * WAVES), bytes, s, a)
+  const int ring = waves * DEPTH * Int4Stage<G>::BYTES, meet = waves * a.block_heads * 32 * G * 4;
+  const int bytes = (I4_HEADS + waves * 2 * I4_HEADS) * 4 + (ring > meet ? ring : meet);
+  const bool even = a.page_size >= 16 && a.page_shift >= 0;
+#define PS_LAUNCH_H4E(WAVES, EVEN)                                                                              \
+  do {                                                                                                          \
+    int4_allow_lds(reinterpret_cast<const void*>(attention_decode_int4_heads_kernel<G, WAVES, EVEN, DEPTH>), bytes); \
+    hipLaunchKernelGGL((attention_decode_int4_heads_kernel<G, WAVES, EVEN, DEPTH>), grid, dim3(64 * WAVES), bytes, s, a); \
+  } while (0)
+#define PS_LAUNCH_H4(WAVES)                \
+  do {                                     \
+    if (even) PS_LAUNCH_H4E(WAVES, true);  \
+    else PS_LAUNCH_H4E(WAVES, false);      \
+  } while (0)
   if constexpr (G <= 4) {
     if (waves == 8) {
-      if (even) PS_LAUNCH_H4(8, true);
-      else PS_LAUNCH_H4(8, false);
+      PS_LAUNCH_H4(8);
       return;
     }
   }
-  if (even) PS_LAUNCH_H4(4, true);
-  else PS_LAUNCH_H4(4, false);
+  PS_LAUNCH_H4(4);
+#undef PS_LAUNCH_H4E
 #undef PS_LAUNCH_H4
 }
 
@@ -604,27 +671,53 @@ __global__ __launch_bounds__(256) void attention_decode_int4_kernel(
   }
 }
 
-// The records of a token's ranges joined: a block per (token, head), a thread per dimension.
-template <typename T>
-__global__ __launch_bounds__(256) void attention_decode_int4_merge_kernel(const float* __restrict__ partial,
-                                                                          const int* __restrict__ tok_list, int heads,
-                                                                          int head_dim, int splits,
-                                                                          T* __restrict__ out, int64_t out_stride) {
-  const int n = blockIdx.x, head = blockIdx.y, d = threadIdx.x;
+// The records of a token's ranges joined, a wave per (token, head): lane s fetches maximum and sum of range s (64 at most),
+// and with them the first eight ranges' values leave, so that a merge of eight is one trip to memory.  A lane owns dimensions
+// lane, lane + 64, .. (DIMS of them).
+template <typename T, int DIMS>
+__global__ __launch_bounds__(64) void attention_decode_int4_merge_kernel(const float* __restrict__ partial,
+                                                                         const int* __restrict__ tok_list, int heads,
+                                                                         int head_dim, int splits,
+                                                                         T* __restrict__ out, int64_t out_stride) {
+  const int n = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
   const int stride = head_dim + 2;
   const float* records = partial + ((int64_t)n * heads + head) * splits * stride;
-  float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, records[s * stride + head_dim]);
-  float sum = 0.f, total = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float m_s = records[s * stride + head_dim];
-    const float c = m_s == -INFINITY ? 0.f : exp2_fast<T>(m_s - m);
-    total += records[s * stride + head_dim + 1] * c;
-    if (d < head_dim) sum += records[s * stride + d] * c;
-  }
+  const int own = lane < splits ? lane : 0;
+  float m = records[own * stride + head_dim], l = records[own * stride + head_dim + 1];
+  float part[8][DIMS], value[DIMS];
+  auto ask = [&](int from) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int k = 0; k < DIMS; ++k)
+        part[j][k] = records[(from + j < splits ? from + j : 0) * stride + (64 * k + lane < head_dim ? 64 * k + lane : 0)];
+  };
+  ask(0);
   const int t = tok_list ? tok_list[n] : n;
-  if (d < head_dim)
-    out[t * out_stride + (int64_t)head * head_dim + d] = from_float<T>(total == 0.f ? 0.f : sum / total);
+  if (lane >= splits) {
+    m = -INFINITY;
+    l = 0.f;
+  }
+  const float high = wave_max(m);
+  const float weight = m == -INFINITY ? 0.f : exp2_fast<T>(m - high);
+  const float total = wave_sum(l * weight);
+#pragma unroll
+  for (int k = 0; k < DIMS; ++k) value[k] = 0.f;
+  for (int from = 0; from < splits; from += 8) {
+    if (from > 0) ask(from);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float w = read_lane(weight, (from + j) & 63);        // (0 for ranges beyond the last)
+#pragma unroll
+      for (int k = 0; k < DIMS; ++k) value[k] = from + j < splits ? fmaf(part[j][k], w, value[k]) : value[k];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < DIMS; ++k) {
+    const int d = 64 * k + lane;
+    if (d < head_dim)
+      out[t * out_stride + (int64_t)head * head_dim + d] = from_float<T>(total == 0.f ? 0.f : value[k] / total);
+  }
 }
 
 extern "C" int ps_attention_decode_int4(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool,
@@ -679,7 +772,7 @@ extern "C" int ps_attention_decode_int4(const void* q, int64_t q_stride, const v
                        (kv_group + block_heads - 1) / block_heads, block_heads, head_dim, page_size, page_shift, num_pages, window, splits,
                        wide_q, scale * 1.4426950408889634f, softcap * 1.4426950408889634f, sink};
     const int64_t blocks = (int64_t)count * kv_heads * a.parts;
-    const int waves = splits == 1 && blocks <= ps_compute_units() && groups <= 4 && block_heads * groups <= 32 ? 8 : 4;
+    int waves = splits == 1 && blocks <= ps_compute_units() && groups <= 4 && block_heads * groups <= 32 ? 8 : 4;
     switch (groups) {
       case 1: launch_heads<1>(a, count, waves, s); break;
       case 2: launch_heads<2>(a, count, waves, s); break;
@@ -696,12 +789,19 @@ extern "C" int ps_attention_decode_int4(const void* q, int64_t q_stride, const v
 #undef PS_LAUNCH_D4
   PS_CHECK_LAUNCH("ps_attention_decode_int4");
   if (splits > 1) {
-    if (dtype == PS_F32)
-      hipLaunchKernelGGL(attention_decode_int4_merge_kernel<float>, dim3(count, heads), dim3(256), 0, s, partial,
-                         tok_list, heads, head_dim, splits, (float*)out, out_stride);
-    else
-      hipLaunchKernelGGL(attention_decode_int4_merge_kernel<bf16_t>, dim3(count, heads), dim3(256), 0, s, partial,
-                         tok_list, heads, head_dim, splits, (bf16_t*)out, out_stride);
+#define PS_LAUNCH_M4(T, DIMS)                                                                                      \
+  hipLaunchKernelGGL((attention_decode_int4_merge_kernel<T, DIMS>), dim3(count, heads), dim3(64), 0, s, partial, \
+                     tok_list, heads, head_dim, splits, (T*)out, out_stride)
+#define PS_LAUNCH_M4T(T)                        \
+  do {                                          \
+    if (head_dim <= 64) PS_LAUNCH_M4(T, 1);     \
+    else if (head_dim <= 128) PS_LAUNCH_M4(T, 2); \
+    else PS_LAUNCH_M4(T, 4);                    \
+  } while (0)
+    if (dtype == PS_F32) PS_LAUNCH_M4T(float);
+    else PS_LAUNCH_M4T(bf16_t);
+#undef PS_LAUNCH_M4T
+#undef PS_LAUNCH_M4
     PS_CHECK_LAUNCH("ps_attention_decode_int4(merge)");
   }
   return 0;

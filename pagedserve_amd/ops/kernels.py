@@ -1406,10 +1406,24 @@ def kv_read_int4(k_pool, v_pool, k, v, tok_item, tok_pos, tables):
 
 def int4_decode_splits(dtype, count, heads, kv_heads, head_dim, visible) -> int:
     """Ranges per request that ``attention_decode_int4`` best cuts its keys into: ``count`` tokens, none of which sees more
-    than ``visible`` keys."""
+    than ``visible`` keys.  A block takes up to 16 heads that share keys (in float one head), four waves of 32 keys a turn.
+
+    * Up to 384 keys one range, whose block has eight waves where the blocks leave units idle (us in one range and in
+      two or three: 1 and 8 requests of 12 heads over 144 and 300 keys 4.9 / 6.3 and 5.7 / 7.1).
+    * Up to half a block per unit, ranges until three blocks come to a unit, of a turn or more, eight at most, sixteen where
+      even these leave units idle (1 request of 12 heads over 900 keys in 1, 4 and 8 ranges 8.4, 7.3 and 6.3, over 4,096 in 8,
+      16 and 32 9.4, 8.1 and 8.3; 8 over 1,000 in 1 and 8 9.3 and 8.5, over 4,000 in 8 and 16 14.1 and 15.0; 24 of 16 heads of 128 over 2, up
+      to 6,000 keys, in 4, 8 and 16 24.2, 19.2 and 21.4).
+    * More blocks: one range up to 2,048 keys (20 of 12 heads over 1,000 in 1 and 2 10.2 and 12.2), beyond ranges until six come
+      to a unit (32 of 12 over 8,192 keys in 1, 2 and 4 68, 59.7 and 57.3)."""
     units = compute_units()
-    blocks = max(1, count * heads)
-    return max(1, min(-(-4 * units // blocks), -(-visible // 128), 64))
+    group = 1 if dtype == torch.float32 else heads // kv_heads
+    blocks = max(1, count * (heads // group) * -(-group // (16 if head_dim <= 128 else 8)))
+    if visible <= 384:
+        return 1
+    if 2 * blocks > units:
+        return 1 if visible <= 2048 else max(1, min(-(-6 * units // blocks), 64))
+    return max(1, min(16 if 16 * blocks <= units else 8, 3 * units // blocks, -(-visible // 128)))
 
 
 def attention_decode_int4(q, k_pool, v_pool, out, tok_item, tok_pos, tables, heads, scale, splits, partial=None,
