@@ -1294,94 +1294,114 @@ def int4_row_bytes(head_dim: int) -> int:
     return 18 * -(-head_dim // INT4_GROUP)
 
 
-def _one_device(what, first):
-    """The device of a call's first tensor, which must be the current one: kernels are launched on its stream."""
-    device = first.get_device()
-    if device >= 0 and device != torch._C._cuda_getDevice():
-        raise KernelError(f"{what}: tensors on {first.device}, the current device is {torch.cuda.current_device()}")
-    return device
+# The faces below ask all that a launch assumes in one expression per group of arguments and find out what is wrong only
+# where something is: one question after the other cost a call 6 us on the host, as much as the GPU needs for most of them.
+def _first(what, tensor, name):
+    """(dtype, device) of a call's first rows, which lie on the current device: kernels are launched on its stream."""
+    try:
+        device = tensor.get_device()
+        if tensor.dim() == 2 and (device == torch._C._cuda_getDevice() if device >= 0 else tensor.is_cuda):
+            return tensor.dtype, device
+    except AttributeError:
+        pass
+    _check(tensor, name, ndim=2)
+    raise KernelError(f"{what}: tensors on {tensor.device}, the current device is {torch.cuda.current_device()}")
+
+
+def _elsewhere(tensor, name, device):
+    if tensor.get_device() != device:
+        raise KernelError(f"{name} is on {tensor.device}, not on the device of the call's other tensors")
 
 
 def _dense(tensor, name, dtype, ndim, device):
-    """A contiguous tensor of this type on a call's device; its address.  (One question after the other costs a decode
-    step's launches more than the GPU needs for them: what is wrong is found out only where something is.)"""
+    """The address of a contiguous tensor of this type (and of so many dimensions) on a call's device."""
     try:
-        if tensor.dtype is dtype and tensor.dim() == ndim and tensor.is_contiguous() and tensor.get_device() == device:
+        if (tensor.dtype is dtype and (ndim is None or tensor.dim() == ndim) and tensor.is_contiguous()
+                and tensor.get_device() == device):
             return tensor.data_ptr()
     except AttributeError:
         pass
     _check(tensor, name, dtype, ndim)
-    if tensor.get_device() != device:
-        raise KernelError(f"{name} is on {tensor.device}, not on the device of the call's other tensors")
+    _elsewhere(tensor, name, device)
     raise KernelError(f"{name} must be contiguous")
 
 
 def _rows_on(tensor, name, dtype, device):
-    """Rows of this type on a call's device; (address, row stride)."""
+    """(address, row stride) of rows of this type on a call's device."""
     try:
         if tensor.dtype is dtype and tensor.dim() == 2 and tensor.get_device() == device:
-            if tensor.is_contiguous():
-                return tensor.data_ptr(), max(1, tensor.size(1))
+            stride, step = tensor.stride()
+            if step == 1 and tensor.size(0) > 1:
+                return tensor.data_ptr(), stride
             return tensor.data_ptr(), _rows(tensor, name)
     except AttributeError:
         pass
     _check(tensor, name, dtype, 2)
-    raise KernelError(f"{name} is on {tensor.device}, not on the device of the call's other tensors")
+    _elsewhere(tensor, name, device)
+    raise KernelError(f"{name} must be 2-D")
 
 
 def _int4_pools(k_pool, v_pool, columns, heads, device):
     """(addresses, pages, key/value heads, page size, head size) of pools ``[pages, kv_heads, page_size,
     int4_row_bytes(head_dim)]`` of bytes, for rows of ``columns`` values of ``heads`` heads (None: of the pools' own)."""
+    try:
+        shape = pages, kv_heads, page_size, row = k_pool.shape
+        count = kv_heads if heads is None else heads
+        head_dim = columns // count
+        k_at, v_at = k_pool.data_ptr(), v_pool.data_ptr()
+        if (k_pool.dtype is torch.uint8 is v_pool.dtype and v_pool.shape == shape and pages and kv_heads and page_size
+                and not page_size % INT4_PAGE_KEYS and not (k_at | v_at) & 15 and count > 0 and 0 < head_dim <= 256
+                and head_dim * count == columns and row == 18 * (head_dim + 31 >> 5) and k_pool.is_contiguous()
+                and v_pool.is_contiguous() and k_pool.get_device() == device == v_pool.get_device()):
+            return k_at, v_at, pages, kv_heads, page_size, head_dim
+    except (AttributeError, TypeError, ValueError, ZeroDivisionError):
+        pass
     k_at = _dense(k_pool, "k_pool", torch.uint8, 4, device)
     v_at = _dense(v_pool, "v_pool", torch.uint8, 4, device)
-    shape = k_pool.shape
-    if shape != v_pool.shape:
+    if k_pool.shape != v_pool.shape:
         raise KernelError("key and value pools must be contiguous and of one shape")
-    pages, kv_heads, page_size, row = shape
-    if not (pages and kv_heads and page_size and row):
-        raise KernelError(f"the pools of a cache in 4 bits are empty: {tuple(shape)}")
+    if 0 in k_pool.shape:
+        raise KernelError(f"the pools of a cache in 4 bits are empty: {tuple(k_pool.shape)}")
     if (k_at | v_at) & 15:
         raise KernelError("the pools of a cache in 4 bits must begin at multiples of 16 bytes")
-    if page_size % INT4_PAGE_KEYS:
-        raise KernelError(f"pages of a cache in 4 bits hold a multiple of {INT4_PAGE_KEYS} keys, not {page_size}")
-    count = kv_heads if heads is None else heads
-    if count <= 0 or columns % count or not 0 < columns // count <= 256 or row != int4_row_bytes(columns // count):
-        raise KernelError(f"rows of {columns} values of {count} heads do not fit pools of {row} bytes a key "
-                          f"({INT4_GROUP} dimensions take 18)")
-    return k_at, v_at, pages, kv_heads, page_size, columns // count
+    if k_pool.size(2) % INT4_PAGE_KEYS:
+        raise KernelError(f"pages of a cache in 4 bits hold a multiple of {INT4_PAGE_KEYS} keys, not {k_pool.size(2)}")
+    raise KernelError(f"rows of {columns} values of {k_pool.size(1) if heads is None else heads} heads do not fit pools of "
+                      f"{k_pool.size(3)} bytes a key ({INT4_GROUP} dimensions take 18)")
 
 
 def _token_index(tok_item, tok_pos, tables, tokens, device, direct_items=False):
     """Addresses of a step's index arrays and the tables' width; as ``_check_step_index``."""
-    pos_at = _dense(tok_pos, "tok_pos", torch.int32, 1, device)
-    tables_at = _dense(tables, "tables", torch.int32, 2, device)
-    items, width = tables.shape
-    if tok_item is None:
-        if not direct_items:
-            raise KernelError("this kernel needs the item index of every token")
-        if items < tokens:
-            raise KernelError("without item indices the block table needs a row per token")
-        item_at = 0
-    else:
-        item_at = _dense(tok_item, "tok_item", torch.int32, 1, device)
-        if tok_item.size(0) < tokens:
-            raise KernelError("one item index per token is needed, contiguous")
-    if tok_pos.size(0) < tokens:
-        raise KernelError("one position per token is needed")
-    return item_at, pos_at, tables_at, width
+    try:
+        items, width = tables.shape
+        if (tables.dtype is torch.int32 is tok_pos.dtype and tok_pos.dim() == 1 and tok_pos.size(0) >= tokens
+                and tables.is_contiguous() and tok_pos.is_contiguous()
+                and tables.get_device() == device == tok_pos.get_device()):
+            if tok_item is None:
+                if direct_items and items >= tokens:
+                    return 0, tok_pos.data_ptr(), tables.data_ptr(), width
+            elif (tok_item.dtype is torch.int32 and tok_item.dim() == 1 and tok_item.size(0) >= tokens
+                    and tok_item.is_contiguous() and tok_item.get_device() == device):
+                return tok_item.data_ptr(), tok_pos.data_ptr(), tables.data_ptr(), width
+    except (AttributeError, ValueError):
+        pass
+    _check_step_index(tok_item, tok_pos, tables, tokens, direct_items)
+    for name, tensor in (("tok_item", tok_item), ("tok_pos", tok_pos), ("tables", tables)):
+        if tensor is not None:
+            _elsewhere(tensor, name, device)
+    raise KernelError("step index tensors must be contiguous")
 
 
 def _int4_rows(what, k, v, k_pool, v_pool, tok_item, tok_pos, tables):
-    _check(k, "k", ndim=2)
-    device = _one_device(what, k)
-    dtype = k.dtype
+    """What the launches on a step's rows of keys and values take, checked."""
+    dtype, device = _first(what, k, "k")
     k_rows, v_rows = _rows_on(k, "k", dtype, device), _rows_on(v, "v", dtype, device)
-    tokens, columns = k.shape
-    if v.shape != k.shape:
+    shape = tokens, columns = k.shape
+    if v.shape != shape:
         raise KernelError(f"{what}: k and v must share a shape")
     k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, columns, None, device)
     item_at, pos_at, tables_at, width = _token_index(tok_item, tok_pos, tables, tokens, device)
-    return (k_rows, v_rows, k_at, v_at, item_at, pos_at, tables_at, width, tokens, kv_heads, head_dim, page_size, pages,
+    return (*k_rows, *v_rows, k_at, v_at, item_at, pos_at, tables_at, width, tokens, kv_heads, head_dim, page_size, pages,
             dtype_code(dtype))
 
 
@@ -1391,16 +1411,16 @@ def kv_write_int4(k, v, k_pool, v_pool, tok_item, tok_pos, tables):
     ``clamp(rint(x / d), -8, 7) + 8``.  ``(code - 8) d`` is a bfloat16 number exactly.  A group with an infinity or a NaN in it is
     held as NaN.  Tokens without a page (a table entry outside the pool) are not stored, as in ``kv_write``; no two
     tokens of a call may have one place."""
-    (k_from, k_stride), (v_from, v_stride), k_at, v_at, *index = _int4_rows("kv_write_int4", k, v, k_pool, v_pool, tok_item,
-                                                                            tok_pos, tables)
+    k_from, k_stride, v_from, v_stride, k_at, v_at, *index = _int4_rows("kv_write_int4", k, v, k_pool, v_pool, tok_item,
+                                                                        tok_pos, tables)
     _call("ps_kv_write_int4", k_from, v_from, k_stride, v_stride, k_at, v_at, *index, _stream())
 
 
 def kv_read_int4(k_pool, v_pool, k, v, tok_item, tok_pos, tables):
     """The values that a cache in 4 bits holds for tokens, into rows of k and v ([tokens, kv_heads*head_dim]); rows of
     tokens without a page are left as they were."""
-    (k_to, k_stride), (v_to, v_stride), k_at, v_at, *index = _int4_rows("kv_read_int4", k, v, k_pool, v_pool, tok_item,
-                                                                        tok_pos, tables)
+    k_to, k_stride, v_to, v_stride, k_at, v_at, *index = _int4_rows("kv_read_int4", k, v, k_pool, v_pool, tok_item, tok_pos,
+                                                                    tables)
     _call("ps_kv_read_int4", k_at, v_at, k_to, v_to, k_stride, v_stride, *index, _stream())
 
 
@@ -1431,9 +1451,7 @@ def attention_decode_int4(q, k_pool, v_pool, out, tok_item, tok_pos, tables, hea
     """``attention_decode`` over a cache in 4 bits, any head size up to 256, float or bfloat16 queries: the same attention over
     the values that the cache stands for.  ``partial``: float scratch of ``count * heads * splits * (head_dim + 2)``
     values when ``splits > 1``.  A token that sees no key gets zeros."""
-    _check(q, "q", ndim=2)
-    device = _one_device("attention_decode_int4", q)
-    dtype = q.dtype
+    dtype, device = _first("attention_decode_int4", q, "q")
     q_at, q_stride = _rows_on(q, "q", dtype, device)
     out_at, out_stride = _rows_on(out, "out", dtype, device)
     tokens, columns = q.shape
@@ -1446,8 +1464,7 @@ def attention_decode_int4(q, k_pool, v_pool, out, tok_item, tok_pos, tables, hea
         list_at, count = _dense(tok_list, "tok_list", torch.int32, 1, device), tok_list.size(0)
     partial_at = floats = 0
     if splits > 1:
-        _check(partial, "partial", torch.float32)
-        partial_at, floats = _dense(partial, "partial", torch.float32, partial.dim(), device), partial.numel()
+        partial_at, floats = _dense(partial, "partial", torch.float32, None, device), partial.numel()
     sink_at = 0
     if sink is not None:
         sink_at = _check_sink(sink, heads)
@@ -1478,15 +1495,14 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
                            window=0, max_kv_len=0, query_tile=PREFILL_TILE, sink=None, softcap=0.0):
     """``attention_prefill`` over a cache in 4 bits (bfloat16 queries, head sizes in multiples of 16)."""
     _check_prefill_constants()
-    _check(q, "q", torch.bfloat16, 2)
-    device = _one_device("attention_prefill_int4", q)
+    _, device = _first("attention_prefill_int4", q, "q")
     q_at, q_stride = _rows_on(q, "q", torch.bfloat16, device)
     out_at, out_stride = _rows_on(out, "out", torch.bfloat16, device)
     k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, q.size(1), heads, device)
     if out.shape != q.shape:
         raise KernelError("attention_prefill_int4: q and out rows must hold heads x head_dim values")
-    index = [_dense(tensor, name, torch.int32, 1, device)
-             for name, tensor in (("tile_item", tile_item), ("tile_q0", tile_q0), ("cu_tokens", cu_tokens), ("kv_lens", kv_lens))]
+    index = (_dense(tile_item, "tile_item", torch.int32, 1, device), _dense(tile_q0, "tile_q0", torch.int32, 1, device),
+             _dense(cu_tokens, "cu_tokens", torch.int32, 1, device), _dense(kv_lens, "kv_lens", torch.int32, 1, device))
     tables_at = _dense(tables, "tables", torch.int32, 2, device)
     tiles, items = tile_item.size(0), kv_lens.size(0)
     if tile_q0.size(0) != tiles or cu_tokens.size(0) != items + 1 or tables.size(0) != items:
@@ -2636,9 +2652,7 @@ def token_logprobs(logits, tokens, out, entropy=None, ranks=None, top_ids=None, 
     A row whose token is -1 has none: log probability 0, rank -1.  Any other token outside the vocabulary gives NaN and -1.
     Logits of minus infinity are tokens that cannot come; a row of nothing else, or with a NaN or an infinity above, has NaN
     for its log probabilities and its entropy."""
-    _check(logits, "logits", ndim=2)
-    device = _one_device("token_logprobs", logits)
-    dtype = logits.dtype
+    dtype, device = _first("token_logprobs", logits, "logits")
     logits_at, ld = _rows_on(logits, "logits", dtype, device)
     rows, vocab = logits.shape
 
@@ -2665,8 +2679,7 @@ def token_logprobs(logits, tokens, out, entropy=None, ranks=None, top_ids=None, 
             raise KernelError(f"token_logprobs: {top} alternatives out of {vocab} tokens; at most {MAX_TOP}")
     partial_at = floats = 0
     if partial is not None:
-        _check(partial, "partial", torch.float32)
-        partial_at, floats = _dense(partial, "partial", torch.float32, partial.dim(), device), partial.numel()
+        partial_at, floats = _dense(partial, "partial", torch.float32, None, device), partial.numel()
     _call("ps_token_logprobs", logits_at, ld, rows, vocab, tokens_at, out_at, entropy_at, ranks_at,
           ids_at if top else 0, best_at if top else 0, top, partial_at, floats, dtype_code(dtype), _stream())
     return out

@@ -13,13 +13,15 @@ from pagedserve_amd.ops import kernels, library
 BF16, F32 = torch.bfloat16, torch.float32
 
 
-@pytest.fixture
-def on_gpu():
+# (twice: where the current device is unknown, and where the tensors' is the current one)
+@pytest.fixture(params=[None, -1])
+def on_gpu(request):
     """CPU tensors pass the question where they live; whatever gets past the checks is caught."""
     launched = []
     with mock.patch.object(torch.Tensor, "is_cuda", property(lambda tensor: True)), \
             mock.patch.object(kernels, "_call", lambda name, *args: launched.append(name)), \
             mock.patch.object(kernels, "_stream", lambda: 0), \
+            mock.patch.object(torch._C, "_cuda_getDevice", lambda: request.param, create=True), \
             mock.patch.object(kernels, "_check_prefill_constants", lambda: None):
         yield launched
 
