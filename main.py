@@ -5,10 +5,10 @@ Options keep the reference's names and meanings where it has them (``--strategy`
 ``--kv-cache-memory-utilization``, ``--kv-cache-safety-mb``, ``--dtype``); ``--model`` is a
 model folder (or ``reference`` for a small random model) instead of a fixed list of names,
 and ``--disable-hip-graphs`` takes the place of ``--disable-cuda-graphs`` (also accepted).
-There is one attention implementation and no quantized cache: ``--decode-attention-backend``
-takes ``hip`` only (the reference's ``torch`` and ``triton`` do not exist here and are refused
-with a message that says so), and ``--kv-cache-dtype`` takes ``model`` only and refuses
-``int8``.
+There is one attention implementation: ``--decode-attention-backend`` takes ``hip`` only (the
+reference's ``torch`` and ``triton`` do not exist here and are refused with a message that says
+so).  ``--kv-cache-dtype`` takes ``model`` or ``int4`` and refuses the reference's ``int8``.
+``--score`` prints how likely the model finds the given prompts instead of continuing them.
 """
 
 import argparse
@@ -21,7 +21,7 @@ from pagedserve_amd.sampling.params import SamplingParams
 
 SUPPORTED_DTYPES = ("float32", "bfloat16")
 SUPPORTED_DECODE_ATTENTION_BACKENDS = ("hip",)    # the reference's option (main.py:27) with the one value built here
-SUPPORTED_KV_CACHE_DTYPES = ("model", "int8")                      # main.py:28
+SUPPORTED_KV_CACHE_DTYPES = ("model", "int4", "int8")              # main.py:28 ("int8" is refused, with a message)
 
 
 def parse_args(argv=None):
@@ -48,7 +48,7 @@ def parse_args(argv=None):
     parser.add_argument("--decode-attention-backend", default="hip",
                         help="attention implementation: 'hip', the only one built")
     parser.add_argument("--kv-cache-dtype", choices=SUPPORTED_KV_CACHE_DTYPES, default="model",
-                        help="KV storage dtype: the model's (quantized caches are not built)")
+                        help="KV storage dtype: the model's, or codes of 4 bits ('int4'); 'int8' is not built")
     parser.add_argument("--disable-hip-graphs", "--disable-cuda-graphs", dest="disable_hip_graphs",
                         action="store_true", help="disable HIP-graph replay of decode steps")
     parser.add_argument("--random-weights", action="store_true",
@@ -64,13 +64,42 @@ def parse_args(argv=None):
     parser.add_argument("--temperature", type=float, default=0.0, help="0 = greedy")
     parser.add_argument("--sample-seed", type=int, help="seed of temperature sampling")
     parser.add_argument("--ignore-eos", action="store_true")
+    parser.add_argument("--score", type=int, nargs="?", const=0, metavar="N",
+                        help="print the prompts' log probabilities, token by token, with N alternatives each, "
+                             "instead of continuing them")
     args = parser.parse_args(argv)
-    if args.kv_cache_dtype != "model":
-        parser.error("--kv-cache-dtype int8: quantized caches are not built; the cache has the model's dtype")
+    if args.kv_cache_dtype == "int8":
+        parser.error("--kv-cache-dtype int8: such quantized caches are not built; the cache has the model's dtype or, "
+                     "with 'int4', codes of 4 bits")
+    if args.score is not None and not 0 <= args.score <= 32:
+        parser.error("--score takes 0 to 32 alternatives")
+    if args.score is not None and not (args.prompt or args.prompt_ids):
+        parser.error("--score needs a --prompt or --prompt-ids")
     if args.decode_attention_backend not in SUPPORTED_DECODE_ATTENTION_BACKENDS:
         parser.error(f"--decode-attention-backend {args.decode_attention_backend}: this engine has one "
                      "attention implementation, 'hip' (hand-written kernels); leave the option out")
     return args
+
+
+def print_scores(scheduler, args):
+    from pagedserve_amd.engine.scoring import score_tokens
+
+    texts = [[int(piece) for piece in text.replace(",", " ").split()] for text in args.prompt_ids or []]
+    if args.prompt and scheduler.tokenizer is None:
+        raise SystemExit("--score --prompt needs a tokenizer; give --prompt-ids")
+    texts += [list(scheduler.tokenizer.encode(prompt)) for prompt in args.prompt or []]
+    for number, scores in enumerate(score_tokens(scheduler.engine, texts, args.score)):
+        count = max(1, len(scores.token_ids) - 1)
+        print(f"text {number}: {len(scores.token_ids)} tokens, log probability {scores.total:.4f}, "
+              f"per token {scores.total / count:.4f}")
+        for place, token in enumerate(scores.token_ids):
+            if scores.logprobs[place] is None:
+                print(f"  {place}: {token}")
+                continue
+            best = "" if not args.score else "  " + " ".join(f"{i}:{p:.3f}" for i, p in scores.alternatives[place])
+            print(f"  {place}: {token}  logprob {scores.logprobs[place]:.4f}  rank {scores.ranks[place]}  "
+                  f"entropy {scores.entropies[place]:.4f}{best}")
+    return 0
 
 
 def main(argv=None):
@@ -82,7 +111,10 @@ def main(argv=None):
         kv_cache_safety_mb=args.kv_cache_safety_mb, execution_dtype=args.dtype,
         enable_hip_graphs=not args.disable_hip_graphs, block_size=args.block_size,
         num_kv_pages=args.num_kv_pages, max_num_batched_tokens=args.max_num_batched_tokens,
-        random_weights=args.random_weights, seed=args.seed, max_model_len=args.max_model_len)
+        random_weights=args.random_weights, seed=args.seed, max_model_len=args.max_model_len,
+        kv_cache_dtype=args.kv_cache_dtype)
+    if args.score is not None:
+        return print_scores(scheduler, args)
     sampling = SamplingParams(temperature=args.temperature, seed=args.sample_seed,
                               max_new_tokens=args.max_new_tokens, ignore_eos=args.ignore_eos)
     request_ids = []

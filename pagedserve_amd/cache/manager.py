@@ -32,6 +32,10 @@ class CacheFull(RuntimeError):
     """No free page (or slot) is left (src/model/kv_manager.py:116-117)."""
 
 
+# How pages hold keys and values: in the model's type, or in codes of 4 bits (csrc/cache_int4.h)
+CACHE_FORMATS = ("model", "int4")
+
+
 @dataclass(frozen=True)
 class CacheGroupSpec:
     """Cache entries that share page geometry and visibility."""
@@ -67,6 +71,14 @@ class CacheGroupSpec:
     @property
     def value_head_dim(self) -> int:
         return self.value_dim or self.head_dim
+
+    def bytes_per_key(self, dtype: torch.dtype, cache_format: str = "model") -> int:
+        """Bytes that one position of one key/value head takes, key and value together."""
+        if cache_format == "int4":
+            # (a step of 2 bytes to 16 of codes, for every 32 dimensions)
+            return 2 * 18 * -(-self.head_dim // 32)
+        per_key = self.head_dim + (0 if self.values_in_keys else self.value_head_dim)
+        return per_key * torch.empty(0, dtype=dtype).element_size()
 
     def geometry(self):
         return (self.kv_heads, self.head_dim, self.window, self.value_head_dim, self.values_in_keys,
@@ -150,9 +162,17 @@ RELEASED = -1
 class CacheManager:
     def __init__(self, groups: Sequence[CacheGroupSpec], num_pages, page_size: int,
                  max_slots: int, dtype: torch.dtype, device, states: Sequence[StateSpec] = (),
-                 max_positions: Optional[int] = None, allocate_pools: bool = True):
+                 max_positions: Optional[int] = None, allocate_pools: bool = True, cache_format: str = "model"):
         if page_size <= 0:
             raise ValueError("page_size must be positive")
+        if cache_format not in CACHE_FORMATS:
+            raise ValueError(f"cache format {cache_format!r}; known: {', '.join(CACHE_FORMATS)}")
+        if cache_format == "int4":
+            if page_size % 8:
+                raise ValueError(f"pages of a cache in 4 bits hold a multiple of 8 keys, not {page_size}")
+            if any(group.values_in_keys or group.value_head_dim != group.head_dim for group in groups):
+                raise ValueError("a cache in 4 bits holds values of their own, of the keys' head size")
+        self.cache_format = cache_format
         if max_slots <= 0:
             raise ValueError("max_slots must be positive")
         self.groups = tuple(groups)
@@ -183,6 +203,12 @@ class CacheManager:
         for group, pool in zip(self.groups, self.pools):
             if allocate_pools:
                 shape = (len(group.entries), pool.num_pages, group.kv_heads, page_size)
+                if cache_format == "int4":
+                    # (bytes: a page's codes, then its steps)
+                    shape += (group.bytes_per_key(dtype, cache_format) // 2,)
+                    self.key_pools.append(torch.empty(shape, dtype=torch.uint8, device=self.device))
+                    self.value_pools.append(torch.empty(shape, dtype=torch.uint8, device=self.device))
+                    continue
                 self.key_pools.append(torch.empty(shape + (group.head_dim,), dtype=dtype, device=self.device))
                 if group.values_in_keys:
                     self.value_pools.append(self.key_pools[-1])
@@ -212,10 +238,9 @@ class CacheManager:
     # ------------------------------------------------------------------ sizes
     def bytes_per_page(self, group_index: int) -> int:
         group = self.groups[group_index]
-        element = torch.empty(0, dtype=self.dtype).element_size()
         # src/model/kv_manager.py:55-58
-        per_key = group.head_dim + (0 if group.values_in_keys else group.value_head_dim)
-        return len(group.entries) * group.kv_heads * self.page_size * per_key * element
+        return (len(group.entries) * group.kv_heads * self.page_size
+                * group.bytes_per_key(self.dtype, self.cache_format))
 
     def pages_for_length(self, group_index: int, length: int, longest_step: Optional[int] = None) -> int:
         """Most pages that one request of ``length`` tokens holds in a group at any
@@ -348,7 +373,7 @@ class CacheManager:
     # ------------------------------------------------------------------ views
     def entry_pools(self, entry: int):
         """(keys, values) of one cache entry: ``[pages, kv_heads, page, head_dim]`` (the values
-        with their own head size where the group names one)."""
+        with their own head size where the group names one; in 4 bits bytes, ``[pages, kv_heads, page, bytes a key]``)."""
         group_index, local = self.entry_location[entry]
         return self.key_pools[group_index][local], self.value_pools[group_index][local]
 

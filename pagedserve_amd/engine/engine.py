@@ -75,7 +75,8 @@ class StepError(ValueError):
 
 class Engine:
     def __init__(self, model, num_pages: int, page_size: int = 16, max_requests: int = 64,
-                 max_step_tokens: int = 2048, use_graphs: bool = True, max_context: int = None):
+                 max_step_tokens: int = 2048, use_graphs: bool = True, max_context: int = None,
+                 kv_cache_dtype: str = "model"):
         if not torch.cuda.is_available():
             raise RuntimeError("pagedserve_amd runs on a GPU only; no CPU path exists")
         self.model = model
@@ -85,6 +86,7 @@ class Engine:
         self.page_size = page_size
         self.max_requests = max_requests
         self.max_step_tokens = max_step_tokens
+        model.check_cache_format(kv_cache_dtype)
         groups, states = model.cache_requirements()
         # A request cannot grow beyond the model's positions, nor (where no group gives pages
         # back behind a window) beyond what the pool holds: block tables are that wide.  A model
@@ -99,7 +101,8 @@ class Engine:
             smallest = num_pages if isinstance(num_pages, int) else min(num_pages)
             self.max_positions = min(self.max_positions, smallest * page_size)
         self.cache = CacheManager(groups, num_pages, page_size, max_requests, self.dtype,
-                                  self.device, states, max_positions=self.max_positions)
+                                  self.device, states, max_positions=self.max_positions,
+                                  cache_format=kv_cache_dtype)
         self.views = model.cache_views(self.cache)
         self.workspace = Workspace(max_step_tokens, self.device)
         self.table_width = -(-self.max_positions // page_size)

@@ -11,7 +11,7 @@ from typing import List, Optional, Sequence, Union
 
 import torch
 
-from ..cache.manager import kv_cache_budget
+from ..cache.manager import CACHE_FORMATS, kv_cache_budget
 from ..config.base import read_config_json
 from ..config.registry import find_preset
 from ..model.loading import load_model, random_model, resolve_dtype
@@ -19,6 +19,7 @@ from ..sampling.params import SamplingParams
 from . import hostgc
 from .engine import Engine
 from .scheduler import ORCA_STRATEGY, ContinuousBatchScheduler
+from .scoring import TokenScores, score_tokens
 from .tokenizer import load_tokenizer
 
 MIB = 1024 * 1024
@@ -27,11 +28,9 @@ DEFAULT_KV_SAFETY_MB = 3072            # main.py:31
 REFERENCE_MODEL = "reference"   # a preset that the architecture's registry entry names
 
 
-def _bytes_per_page(model, page_size, dtype):
+def _bytes_per_page(model, page_size, dtype, kv_cache_dtype="model"):
     groups, _ = model.cache_requirements()
-    element = torch.empty(0, dtype=dtype).element_size()
-    return sum(len(g.entries) * g.kv_heads * page_size
-               * (g.head_dim + (0 if g.values_in_keys else g.value_head_dim)) * element for g in groups)
+    return sum(len(g.entries) * g.kv_heads * page_size * g.bytes_per_key(dtype, kv_cache_dtype) for g in groups)
 
 
 def build_scheduler(model=REFERENCE_MODEL, scheduling_strategy=ORCA_STRATEGY, prefill_chunk_size=16,
@@ -49,8 +48,10 @@ def build_scheduler(model=REFERENCE_MODEL, scheduling_strategy=ORCA_STRATEGY, pr
 
     The reference's names for the same things are taken as well (main.py:136-150):
     ``model_name`` for ``model``, ``enable_cuda_graphs`` for ``enable_hip_graphs``.  Of its
-    ``decode_attention_backend`` only ``"hip"`` exists here and of ``kv_cache_dtype`` only
-    ``"model"`` (quantized caches are not built); other values are errors."""
+    ``decode_attention_backend`` only ``"hip"`` exists here.  ``kv_cache_dtype``: ``"model"``, or
+    ``"int4"`` for codes of 4 bits with a step for every 32 dimensions (4.5 bits a value, csrc/cache_int4.h), which
+    architectures whose attention caches keys and values as projected take (pages of a multiple of 8
+    tokens); other values are errors."""
     if model_name is not None:
         model = model_name
     if enable_cuda_graphs is not None:
@@ -58,9 +59,9 @@ def build_scheduler(model=REFERENCE_MODEL, scheduling_strategy=ORCA_STRATEGY, pr
     if decode_attention_backend != "hip":
         raise ValueError(f"Unknown decode attention backend '{decode_attention_backend}': "
                          "the one implementation here is 'hip'")
-    if kv_cache_dtype != "model":
-        raise ValueError(f"KV cache dtype '{kv_cache_dtype}': quantized caches are not built; "
-                         "the cache has the model's dtype ('model')")
+    if kv_cache_dtype not in CACHE_FORMATS:
+        raise ValueError(f"KV cache dtype '{kv_cache_dtype}': such quantized caches are not built; "
+                         "the cache has the model's dtype ('model') or codes of 4 bits ('int4')")
     if not torch.cuda.is_available():
         raise RuntimeError("pagedserve_amd needs a GPU (MI355X); there is no CPU path")
     dtype = resolve_dtype(execution_dtype)
@@ -78,7 +79,8 @@ def build_scheduler(model=REFERENCE_MODEL, scheduling_strategy=ORCA_STRATEGY, pr
         max_batch_size = 32          # main.py:180-181 (its GPU default)
     if max_batch_size <= 0:
         raise ValueError("max_batch_size must be positive")
-    per_page = _bytes_per_page(loaded, block_size, dtype)
+    loaded.check_cache_format(kv_cache_dtype)
+    per_page = _bytes_per_page(loaded, block_size, dtype, kv_cache_dtype)
     source = "explicit"
     if per_page == 0:
         pages = 1        # a model without cached keys (recurrent mixers only): slots are all it holds
@@ -102,7 +104,8 @@ def build_scheduler(model=REFERENCE_MODEL, scheduling_strategy=ORCA_STRATEGY, pr
         raise ValueError(f"Memory budget is too small; one block requires {per_page} bytes")
     step_tokens = max_num_batched_tokens or max(2048, max_batch_size)
     engine = Engine(loaded, num_pages=pages, page_size=block_size, max_requests=max_batch_size,
-                    max_step_tokens=step_tokens, use_graphs=enable_hip_graphs, max_context=max_model_len)
+                    max_step_tokens=step_tokens, use_graphs=enable_hip_graphs, max_context=max_model_len,
+                    kv_cache_dtype=kv_cache_dtype)
     engine.memory_budget_source = source
     from ..sampling.sampler import Sampler
 
@@ -130,7 +133,7 @@ class GenerationOutput:
 
 
 class LLM:
-    """``LLM(model=folder, dtype=...).generate(prompts, sampling_params)``."""
+    """``LLM(model=folder, dtype=...).generate(prompts, sampling_params)``, ``.score(texts)``."""
 
     def __init__(self, model, dtype="float32", **engine_args):
         self.scheduler = build_scheduler(model, execution_dtype=dtype, **engine_args)
@@ -165,3 +168,16 @@ class LLM:
                                             list(state.generated_token_ids), text,
                                             state.finish_reason))
         return outputs
+
+    def score(self, texts: Sequence[Union[str, Sequence[int]]], top: int = 0) -> List[TokenScores]:
+        """How likely the model finds given texts (or token ids), token by token: log probabilities, ranks, the
+        entropy in front of every token and, with ``top``, the most likely alternatives
+        (``engine/scoring.py``)."""
+        listed = []
+        for text in texts:
+            if isinstance(text, str):
+                if self.scheduler.tokenizer is None:
+                    raise ValueError("scoring a text needs a tokenizer; give token ids")
+                text = self.scheduler.tokenizer.encode(text)
+            listed.append([int(token) for token in text])
+        return score_tokens(self.engine, listed, top)

@@ -158,6 +158,19 @@ class DecoderModel:
         groups = [CacheGroupSpec(tuple(entries), *geometry) for geometry, entries in by_geometry.items()]
         return groups, states
 
+    def check_cache_format(self, cache_format: str):
+        """Refuse a form of cache that a mixer with keys and values of its own does not take."""
+        if cache_format != "int4":
+            return
+        for call in self.spec.schedule:
+            mixer = self.blocks[call.block].mixer
+            spec = self._entry_spec[call.cache]
+            specs = spec if isinstance(spec, tuple) else (spec,)
+            if any(isinstance(one, PagedKVSpec) for one in specs) and not mixer.takes_int4_cache:
+                raise ValueError(
+                    f"KV cache dtype 'int4': block {call.block} ({type(mixer).__name__}) does not take a cache in 4 bits "
+                    "(attention over keys and values as projected does; layers that norm, rotate or gate them do not)")
+
     def cache_views(self, cache) -> List[CacheView]:
         """One view per call of the run list, in order."""
         def view_of(entry, spec, writes):

@@ -62,6 +62,10 @@ class Attention(Mixer):
     * ``pad_heads``: heads are cached with their size rounded up to a multiple of this (zeros
       behind), so that a head size which the tiled kernels do not take still runs on them.
 
+    Layers without a launch of their own for queries and keys also take a cache in 4 bits
+    (``takes_int4_cache``): the packed product then leaves keys and values as rows, a launch stores them as
+    codes, and attention runs over these.
+
     ``rotary_layout="halves"``, ``rotary_scaling``, ``rotary_bands``, ``head_norm``, ``values_from_keys`` and ``logistic`` go
     through the launch that treats every head on its own (``kernels.attention_prepare_heads``);
     that one does not norm over the whole projection or mix values.
@@ -80,6 +84,10 @@ class Attention(Mixer):
     query_tile = (kernels.PREFILL_TILE, kernels.PREFILL_SMALL_TILE, kernels.PREFILL_LARGE_TILE)
 
     VALUE_MIXES = ("none", "source", "mix")
+
+    @property
+    def takes_int4_cache(self) -> bool:
+        return type(self) is Attention and not self.prepared
 
     chunk = 0      # (mixers that are built on this one and set no chunk of their own)
     logistic = None
@@ -333,6 +341,8 @@ class Attention(Mixer):
         tokens = ctx.tokens
         tables = ctx.tables[cache.group]
         gates = None
+        if cache.k_pool.dtype == torch.uint8:
+            return self._forward_int4(x, residual, ctx, cache, tables)
         if self.prepared:
             q, gates = self._project_prepared(x, ctx, cache, tables)
         else:
@@ -364,6 +374,52 @@ class Attention(Mixer):
                 kernels.kv_write(k, v, cache.k_pool, cache.v_pool, ctx.tok_item, ctx.positions,
                                  tables)
         return q
+
+    def _forward_int4(self, x, residual, ctx, cache, tables):
+        """The same layer over a cache in 4 bits: one launch more, which stores the step's keys and values as codes."""
+        if self.prepared:
+            raise NotImplementedError("attention with prepared queries and keys takes no cache in 4 bits")
+        tokens = ctx.tokens
+        _, q, k, v = rows = ctx.workspace.column_views("qkv", self.q_cols + 2 * self.kv_cols, self.dtype, tokens,
+                                                       (self.q_cols, self.kv_cols, self.kv_cols))
+        kernels.linear(x, self.qkv_weight, self.qkv_bias, rows[0], packed=self.qkv_packed,
+                       memo=site_memo(self._memo_qkv, ctx.workspace), shared=ctx.shared_calls)
+        if self.position is not None and self.position.transforms_qk:
+            self.position.apply_to_qk(q, k, ctx)
+        if cache.writes:
+            kernels.kv_write_int4(k, v, cache.k_pool, cache.v_pool, ctx.tok_item, ctx.positions, tables)
+        context = ctx.workspace.first_rows("attn", self.q_cols, self.dtype, tokens)
+        singles = ctx.single_tokens.numel() if ctx.single_tokens is not None else 0
+        if singles:
+            splits = kernels.int4_decode_splits(self.dtype, singles, self.heads, self.kv_heads, self.head_dim,
+                                                self._visible(ctx.max_kv_len))
+            kernels.attention_decode_int4(q, cache.k_pool, cache.v_pool, context, None if singles == tokens else ctx.tok_item,
+                                          ctx.positions, tables, self.heads, self.scale, splits,
+                                          partial=self._int4_records(ctx) if splits > 1 else None, window=self.span,
+                                          tok_list=None if singles == tokens else ctx.single_tokens, sink=self.sink,
+                                          softcap=self.score_cap)
+        if singles < tokens and kernels.prefill_int4_supported(self.dtype, self.head_dim, tables.shape[1]):
+            size = kernels.prefill_int4_tile(self.heads, self.head_dim,
+                                             {size: lists[0].numel() for size, lists in ctx.query_tiles.items()},
+                                             ctx.max_kv_len)
+            kernels.attention_prefill_int4(q, cache.k_pool, cache.v_pool, context, *ctx.query_tiles[size], ctx.cu_tokens,
+                                           ctx.kv_lens, tables, self.heads, self.scale, window=self.span,
+                                           max_kv_len=ctx.max_kv_len, query_tile=size, sink=self.sink,
+                                           softcap=self.score_cap)
+            # (the tiles hold the items of several tokens)
+        elif singles < tokens:
+            kernels.attention_decode_int4(q, cache.k_pool, cache.v_pool, context, ctx.tok_item, ctx.positions, tables,
+                                          self.heads, self.scale, 1, window=self.span, tok_list=ctx.portion_tokens,
+                                          sink=self.sink, softcap=self.score_cap)
+        self._project_out(context, residual, ctx)
+
+    def _int4_records(self, ctx):
+        """Scratch for the ranges' records of a decode step over a cache in 4 bits, at its largest: the rule asks for
+        ranges until three blocks of up to 16 heads come to a unit, or six beside one per token and key/value head."""
+        group = min(16, self.heads // self.kv_heads)
+        worst = 6 * kernels.compute_units() * group + ctx.workspace.max_rows * self.heads
+        return ctx.workspace.flat(f"attn_partial_int4_{self.heads}x{self.head_dim}", worst * (self.head_dim + 2),
+                                  torch.float32)
 
     def _attend(self, q, context, gates, residual, ctx, cache, tables):
         tokens = ctx.tokens

@@ -65,7 +65,7 @@ class CacheView:
     entry: int
     writes: bool
     group: Optional[int] = None                # index of the cache group (paged entries)
-    k_pool: Optional[torch.Tensor] = None      # [pages, kv_heads, page, head_dim]
+    k_pool: Optional[torch.Tensor] = None      # [pages, kv_heads, page, head_dim] (bytes: a cache in 4 bits)
     v_pool: Optional[torch.Tensor] = None      # [pages, kv_heads, page, value head size]
     state: Optional[torch.Tensor] = None       # [max_slots, ...]
     # a mixer made of several mixers (its ``cache_spec`` is a tuple): one view per child
@@ -137,6 +137,9 @@ class Head(Part):
 
 class Mixer(Part):
     accepts_pending_norm = False
+    # True when ``forward`` also takes pools of bytes that hold keys and values in 4 bits
+    # (``CacheManager(cache_format="int4")``).
+    takes_int4_cache = False
 
     def cache_spec(self):
         """``PagedKVSpec``, ``SlotStateSpec`` or ``None``; a mixer made of several mixers returns
