@@ -49,6 +49,14 @@ struct Int4Pages {
   static constexpr bool INT4 = true;
 };
 
+// A block may take one of several ranges of its keys and leave records instead of the result: of every query the
+// unnormalised sums [tile][head][range][query][head_dim], and maximum (in units of log 2) and sum [tile][..][query][2].
+struct PrefillRange {
+  int range, ranges;
+  float* sums;
+  float* states;
+};
+
 // The work of one block: one head of one tile of queries.  The caller provides the block's LDS
 // (the kernel below its own; a kernel that runs blocks of several kinds in one launch a share
 // of what all of them need).
@@ -61,7 +69,8 @@ __device__ __forceinline__ void attention_prefill_block(
     const int* __restrict__ tile_item, const int* __restrict__ tile_q0,
     const int* __restrict__ cu_tokens, const int* __restrict__ kv_lens,
     const int* __restrict__ tables, int table_width, int heads, int kv_heads, int page_size,
-    int page_shift, int num_pages, float scale, int window, const AttnExtras extra) {
+    int page_shift, int num_pages, float scale, int window, const AttnExtras extra,
+    const PrefillRange part = PrefillRange{0, 1, nullptr, nullptr}) {
   constexpr int HD = NDB * 16;
   constexpr int ROW = HD * 2;                    // bytes of one key in a tile
   constexpr int CH = HD / 8;                     // 16-byte pieces per row
@@ -173,11 +182,10 @@ __device__ __forceinline__ void attention_prefill_block(
     load_piece[j] = (slot + CH - (key_local / SPREAD) % CH) % CH;
   }
   const int page_mask = page_size - 1;                // where the page size is a power of two
-  // the page's first row and the key's place in the page, for a lane's piece j of the tile at k0
-  auto place_of = [&](int j, int k0, uint32_t& page_row, int& within) {
+  // the page's first row and a key's place in the page
+  auto place_of = [&](int key, uint32_t& page_row, int& within) {
     // keys outside the tile's visible range are fetched from a visible key instead: they
     // are masked below, and whatever lies in pages that were given back is never read
-    int key = k0 + load_key[j];
     key = key < key_begin ? key_begin : (key >= key_end ? key_end - 1 : key);
     int logical;
     if (page_shift >= 0) {
@@ -198,7 +206,7 @@ __device__ __forceinline__ void attention_prefill_block(
       for (int j = 0; j < PER_OPERAND; ++j) {
         uint32_t page_row;
         int within;
-        place_of(j, k0, page_row, within);
+        place_of(k0 + load_key[j], page_row, within);
         row[j] = page_row + (uint32_t)within;
       }
 #pragma unroll
@@ -213,57 +221,89 @@ __device__ __forceinline__ void attention_prefill_block(
       }
     }
   };
-  // Codes: a lane's pieces of a tile are asked for two tiles ahead, and one tile ahead they become values in LDS.
+  // Codes are asked for two tiles ahead of the one being multiplied, and one tile ahead they become values in LDS.  A
+  // thread takes a quarter of a key's row, or of a value's: 8 dimensions of each group, whose codes lie side by side,
+  // and the row's steps.  The first half of the items are keys'.
   constexpr int GROUPS = (HD + PS_INT4_GROUP - 1) / PS_INT4_GROUP;
-  uint32_t k_codes[PER_OPERAND], v_codes[PER_OPERAND][4];
-  uint16_t k_steps[PER_OPERAND], v_steps[PER_OPERAND];
+  constexpr int THREADS = 64 * AP_WAVES, ROW_ITEMS = 4 * AP_KEYS, ITEMS = 2 * ROW_ITEMS / THREADS;
+  constexpr int STEP_WORDS = (GROUPS + 1) / 2;
+  static_assert(!Pages::INT4 || (ITEMS >= 1 && 2 * ROW_ITEMS % THREADS == 0 && ROW_ITEMS % 64 == 0), "whole waves of one kind");
+  uint32_t codes[Pages::INT4 ? ITEMS : 1][GROUPS], steps[Pages::INT4 ? ITEMS : 1][STEP_WORDS],
+      value_steps[Pages::INT4 ? ITEMS : 1][STEP_WORDS];
+  // Which key an item is of: of every 16 in an order that spreads the stores of 16 lanes over the banks, whose rows are
+  // turned by the key's number (rows of 64 dimensions: keys 0, 1, 8, 9, .., of 128: 0, 4, 8, 12, ..).
+  auto key_of = [&](int item) {
+    const int key = (item % ROW_ITEMS) / 4;
+    if constexpr (CH == 8) return (key & ~15) | (key & 1) | (key & 2) << 2 | (key & 12) >> 1;
+    else if constexpr (CH == 16) return (key & ~15) | (key & 3) << 2 | (key & 12) >> 2;
+    else return key;
+  };
+  auto load_steps = [&](const uint8_t* from, uint32_t* words) {
+    if constexpr (GROUPS % 8 == 0) {
+      const uint4 v = *reinterpret_cast<const uint4*>(from);
+      words[0] = v.x;
+      words[1] = v.y;
+      words[2] = v.z;
+      words[3] = v.w;
+    } else if constexpr (GROUPS % 4 == 0) {
+      const uint2 v = *reinterpret_cast<const uint2*>(from);
+      words[0] = v.x;
+      words[1] = v.y;
+    } else if constexpr (GROUPS % 2 == 0) {
+#pragma unroll
+      for (int i = 0; i < STEP_WORDS; ++i) words[i] = reinterpret_cast<const uint32_t*>(from)[i];
+    } else {
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        const uint32_t bits = reinterpret_cast<const uint16_t*>(from)[g];
+        words[g / 2] = g % 2 ? words[g / 2] | bits << 16 : bits;
+      }
+    }
+  };
   auto fetch = [&](int k0) {
     if constexpr (Pages::INT4) {
-      const uint8_t* k_at[PER_OPERAND];
-      const uint8_t* v_at[PER_OPERAND];
-      int rows[PER_OPERAND];
 #pragma unroll
-      for (int j = 0; j < PER_OPERAND; ++j) {
+      for (int j = 0; j < ITEMS; ++j) {
+        const int item = j * THREADS + tid;
+        const bool is_value = j * THREADS + wave * 64 >= ROW_ITEMS;      // (the same in a wave)
+        const int key_local = key_of(item), c = item & 3;
         uint32_t page_row;
         int within;
-        place_of(j, k0, page_row, within);
+        place_of(k0 + key_local, page_row, within);
         const uint64_t at = (uint64_t)page_row * (18 * GROUPS);
-        k_at[j] = k_pool + at;
-        v_at[j] = v_pool + at;
-        rows[j] = within;
-      }
+        const uint8_t* from = (is_value ? v_pool : k_pool) + at + within * (16 * GROUPS) + c * (4 * GROUPS);
+        if constexpr (GROUPS % 4 == 0) {
 #pragma unroll
-      for (int j = 0; j < PER_OPERAND; ++j) {
-        const int g = load_piece[j] >> 2, c = load_piece[j] & 3;
-        const int row = rows[j] * (16 * GROUPS);
-        const int steps = page_size * (16 * GROUPS) + 2 * (rows[j] * GROUPS + g);
-        k_codes[j] = *reinterpret_cast<const uint32_t*>(k_at[j] + row + 4 * (c * GROUPS + g));
-        k_steps[j] = *reinterpret_cast<const uint16_t*>(k_at[j] + steps);
-        const uint8_t* from = v_at[j] + row + 4 * c * GROUPS;
-        if constexpr (GROUPS == 1) {
-          v_codes[j][0] = *reinterpret_cast<const uint32_t*>(from);
-        } else if constexpr (GROUPS == 2) {
-          const uint2 both = *reinterpret_cast<const uint2*>(from);
-          v_codes[j][0] = both.x;
-          v_codes[j][1] = both.y;
-        } else if constexpr (GROUPS == 4) {
-          const uint4 all = *reinterpret_cast<const uint4*>(from);
-          v_codes[j][0] = all.x;
-          v_codes[j][1] = all.y;
-          v_codes[j][2] = all.z;
-          v_codes[j][3] = all.w;
+          for (int i = 0; i < GROUPS / 4; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(from + 16 * i);
+            codes[j][4 * i] = v.x;
+            codes[j][4 * i + 1] = v.y;
+            codes[j][4 * i + 2] = v.z;
+            codes[j][4 * i + 3] = v.w;
+          }
+        } else if constexpr (GROUPS % 2 == 0) {
+#pragma unroll
+          for (int i = 0; i < GROUPS / 2; ++i) {
+            const uint2 v = *reinterpret_cast<const uint2*>(from + 8 * i);
+            codes[j][2 * i] = v.x;
+            codes[j][2 * i + 1] = v.y;
+          }
         } else {
 #pragma unroll
-          for (int b = 0; b < 4; ++b) v_codes[j][b] = from[b * GROUPS + g];
+          for (int i = 0; i < GROUPS; ++i) codes[j][i] = reinterpret_cast<const uint32_t*>(from)[i];
         }
-        v_steps[j] = *reinterpret_cast<const uint16_t*>(v_at[j] + steps);
+        const int step_at = page_size * (16 * GROUPS) + within * (2 * GROUPS);
+        load_steps(v_pool + at + step_at, value_steps[j]);
+        if (!is_value) load_steps(k_pool + at + step_at, steps[j]);
       }
     }
   };
   // eight codes as the bfloat16 values that they stand for, exactly
-  auto values_of = [&](uint32_t codes, float step) {
+  auto values_of = [&](uint32_t word, float step) {
     const float base = -8.f * step;
-    const uint32_t even = codes & 0x0f0f0f0fu, odd = codes >> 4 & 0x0f0f0f0fu;
+    uint32_t even = word & 0x0f0f0f0fu, odd = word >> 4 & 0x0f0f0f0fu;
+    // (kept as they are: a byte of them is a float by one instruction, four bits of the word by two)
+    asm("" : "+v"(even), "+v"(odd));
     u32x4 words;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -275,27 +315,47 @@ __device__ __forceinline__ void attention_prefill_block(
     if constexpr (Pages::INT4) {
       unsigned char* stage = stages + (tile_number % STAGES) * STAGE_BYTES;
 #pragma unroll
-      for (int j = 0; j < PER_OPERAND; ++j) {
-        const int number = wave * PER_OPERAND + j < INSTRUCTIONS ? wave * PER_OPERAND + j : INSTRUCTIONS - 1;
-        const int g = load_piece[j] >> 2;
-        uint32_t v_word;
-        if constexpr (GROUPS == 1) v_word = v_codes[j][0];
-        else if constexpr (GROUPS == 2) v_word = __builtin_amdgcn_perm(v_codes[j][1], v_codes[j][0], g ? 0x07050301u : 0x06040200u);
-        else if constexpr (GROUPS == 4) {
-          const uint32_t pick = 0x0c0c0400u + 0x0101u * g;
-          v_word = __builtin_amdgcn_perm(v_codes[j][1], v_codes[j][0], pick) |
-                   __builtin_amdgcn_perm(v_codes[j][3], v_codes[j][2], pick) << 16;
-        } else {
-          v_word = v_codes[j][0] | v_codes[j][1] << 8 | v_codes[j][2] << 16 | v_codes[j][3] << 24;
+      for (int j = 0; j < ITEMS; ++j) {
+        const int item = j * THREADS + tid;
+        const bool is_value = j * THREADS + wave * 64 >= ROW_ITEMS;
+        const int key_local = key_of(item), c = item & 3;
+        const int turn = (key_local / SPREAD) % CH;
+        unsigned char* row = stage + (is_value ? TILE_BYTES : 0) + key_local * ROW;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const int piece = 4 * g + c;
+          if (CH % 4 != 0 && piece >= CH) continue;           // (behind the last dimension)
+          // A value that is no number must not reach the queries that do not see its key, whose weight of 0 would
+          // still make it one: it is 0 here, and the key takes its place, whose scores are masked.
+          const float v_step = __uint_as_float(value_steps[j][g / 2] >> (16 * (g % 2)) << 16);
+          uint32_t word;
+          float step;
+          if (is_value) {
+            // byte b of the word for this group is byte b GROUPS + g of the row's quarter
+            if constexpr (GROUPS == 1) word = codes[j][0];
+            else if constexpr (GROUPS == 2)
+              word = __builtin_amdgcn_perm(codes[j][1], codes[j][0], g ? 0x07050301u : 0x06040200u);
+            else if constexpr (GROUPS == 4)
+              word = __builtin_amdgcn_perm(codes[j][1], codes[j][0], 0x0c0c0400u + 0x0101u * g) |
+                     __builtin_amdgcn_perm(codes[j][3], codes[j][2], 0x04000c0cu + 0x01010000u * g);
+            else {
+              word = 0;
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                const int byte = b * GROUPS + g;
+                word |= (codes[j][byte / 4] >> (8 * (byte % 4)) & 0xffu) << (8 * b);
+              }
+            }
+            step = v_step == v_step ? v_step : 0.f;
+          } else {
+            word = codes[j][g];
+            // (0 times a step, which is finite or no number)
+            step = fmaf(v_step, 0.f, __uint_as_float(steps[j][g / 2] >> (16 * (g % 2)) << 16));
+          }
+          int slot = piece + turn;
+          slot = slot >= CH ? slot - CH : slot;
+          *reinterpret_cast<u32x4*>(row + slot * 16) = values_of(word, step);
         }
-        // A value that is no number must not reach the queries that do not see its key, whose weight of 0 would
-        // still make it one: it is 0 here, and the key takes its place, whose scores are masked.
-        const uint32_t k_bits = k_steps[j], v_bits = v_steps[j];
-        const bool number_held = (v_bits & 0x7fffu) <= 0x7f80u;
-        const float k_step = __uint_as_float((number_held ? k_bits : v_bits) << 16);
-        const float v_step = __uint_as_float(number_held ? v_bits << 16 : 0u);
-        *reinterpret_cast<u32x4*>(stage + number * 1024 + lane * 16) = values_of(k_codes[j], k_step);
-        *reinterpret_cast<u32x4*>(stage + TILE_BYTES + number * 1024 + lane * 16) = values_of(v_word, v_step);
       }
     }
   };
@@ -304,7 +364,7 @@ __device__ __forceinline__ void attention_prefill_block(
   // every exponential is one v_exp_f32; probabilities are rounded to bfloat16 right after.
   const float scale_log2 = scale * 1.4426950408889634f;
   float m = -INFINITY, l = 0.f;
-  if (extra.sink != nullptr && wave_k == 0) {
+  if (extra.sink != nullptr && wave_k == 0 && part.range == 0) {
     // a score without key or value: it starts the denominator of the wave with the first keys
     m = extra.sink[head] * 1.4426950408889634f;
     l = 1.f;
@@ -357,16 +417,24 @@ __device__ __forceinline__ void attention_prefill_block(
       }
   }
 
-  const int k_first = key_begin / AP_KEYS * AP_KEYS;
-  const int tiles = (key_end - k_first + AP_KEYS - 1) / AP_KEYS;
+  int k_first = key_begin / AP_KEYS * AP_KEYS;
+  int tiles = (key_end - k_first + AP_KEYS - 1) / AP_KEYS;
+  if (Pages::INT4 && part.ranges > 1) {
+    const int per = (tiles + part.ranges - 1) / part.ranges;
+    k_first += part.range * per * AP_KEYS;
+    tiles -= part.range * per;
+    tiles = tiles < per ? tiles : per;      // (none or fewer: a range without keys)
+  }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the table is in LDS
   // the queries have arrived with that; a use here keeps the compiler from waiting for them
   // (and with them for every tile in flight) inside the loop
 #pragma unroll
   for (int step = 0; step < NDB; ++step) asm volatile("" : "+v"(qf[step]));
   if constexpr (Pages::INT4) {
-    fetch(k_first);
-    store(0);
+    if (tiles > 0) {
+      fetch(k_first);
+      store(0);
+    }
     if (tiles > 1) fetch(k_first + AP_KEYS);
   } else {
 #pragma unroll
@@ -614,6 +682,23 @@ __device__ __forceinline__ void attention_prefill_block(
     }
   }
 
+  if (Pages::INT4 && part.ranges > 1) {
+    if (!q_valid) return;
+    const int64_t record =
+        (((int64_t)tile_index * heads + head) * part.ranges + part.range) * QUERIES + wave_q * 32 + sub;
+    float* sums = part.sums + record * HD;
+#pragma unroll
+    for (int db = 0; db < NDB32; ++db)
+#pragma unroll
+      for (int quad = 0; quad < 4; ++quad) {
+        const int dim = db * 32 + quad * 8 + half * 4;
+        if (dim >= HD) continue;
+        *reinterpret_cast<float4*>(sums + dim) = make_float4(acc[db][quad * 4], acc[db][quad * 4 + 1],
+                                                             acc[db][quad * 4 + 2], acc[db][quad * 4 + 3]);
+      }
+    if (half == 0) *reinterpret_cast<float2*>(part.states + record * 2) = make_float2(m, l);
+    return;
+  }
   // element e of an accumulator: head dimension db*32 + (e/4)*8 + half*4 + e%4 of query `sub`
   if (q_valid && l != 0.f) {
     const float inv = gate_factor(extra, tok0 + qi, head) / l;

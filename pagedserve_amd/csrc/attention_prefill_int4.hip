@@ -1,8 +1,15 @@
 // Tiled attention of prompt portions over a cache in 4 bits: the blocks of attention_prefill.hip (see there for the
-// method) with another way of getting a tile of keys and values into LDS.  A lane asks for its pieces of eight codes two
-// tiles ahead of the one being multiplied, 4 bytes of codes and a step of 2 where the other cache has 16, and turns
-// them into bfloat16 values one tile ahead, exactly (cache_int4.h says why that is no rounding); what follows is the same
-// code, so that this attention is that one over a cache of these values.
+// method) with another way of getting a tile of keys and values into LDS.  A thread asks for a quarter of a key's (or a
+// value's) row of codes, 4 bytes of each group, two tiles ahead of the one being multiplied, and turns them into bfloat16
+// values one tile ahead, exactly (cache_int4.h says why that is no rounding); what follows is the same code, so that this
+// attention is that one over a cache of these values.
+//
+// Bound: the vector instructions of the conversion (3.6 to a value: four bits to a float, one product, half a packing;
+// every block converts what it reads) come on top of those of the softmax, which bound the other cache's kernel.  2 x
+// 4,096 tokens of 12 heads of 64: 108 us, 478 TFLOP/s (the other cache 87); 16 heads of 128 behind 5,000 keys, 962
+// tokens: 116 to 122 us, 340 TFLOP/s (the other cache 94).  Where the tiles are fewer than the compute units, keys are cut into
+// ranges, whose records a second launch joins: 512 tokens of 12 heads behind 3,500 keys 29.5 us (the other cache, without
+// ranges, 41), 64 of 8 heads of 128 behind 8,000 24.4 (121).
 #include <math.h>
 
 #include "common.h"
@@ -10,27 +17,63 @@
 
 #include "attention_prefill_block.h"
 
-template <int NDB, int KS, int QW = 2, int KR = 1>
+template <int NDB, int KS, int QW, int KR>
 __global__ __launch_bounds__(64 * QW * KS) void attention_prefill_int4_kernel(
     const bf16_t* __restrict__ q, int64_t q_stride, const uint8_t* __restrict__ k_pool,
     const uint8_t* __restrict__ v_pool, bf16_t* __restrict__ out, int64_t out_stride,
     const int* __restrict__ tile_item, const int* __restrict__ tile_q0,
     const int* __restrict__ cu_tokens, const int* __restrict__ kv_lens,
     const int* __restrict__ tables, int table_width, int heads, int kv_heads, int page_size,
-    int page_shift, int num_pages, float scale, int window, const AttnExtras extra) {
+    int page_shift, int num_pages, float scale, int window, const AttnExtras extra, int ranges, float* sums,
+    float* states) {
   __shared__ PrefillLds<NDB, KS, QW, KR> lds;
   attention_prefill_block<NDB, KS, QW, KR, Int4Pages>(lds, blockIdx.x, blockIdx.y, q, q_stride, k_pool, v_pool, out,
-                                                      out_stride, tile_item, tile_q0, cu_tokens, kv_lens, tables,
-                                                      table_width, heads, kv_heads, page_size, page_shift,
-                                                      num_pages, scale, window, extra);
+                                                     out_stride, tile_item, tile_q0, cu_tokens, kv_lens, tables,
+                                                     table_width, heads, kv_heads, page_size, page_shift,
+                                                     num_pages, scale, window, extra,
+                                                     PrefillRange{(int)blockIdx.z, ranges, sums, states});
+}
+
+// The records of a tile's queries joined: four dimensions of a query to a thread.
+__global__ __launch_bounds__(256) void attention_prefill_int4_join_kernel(
+    const float* __restrict__ sums, const float* __restrict__ states, bf16_t* __restrict__ out, int64_t out_stride,
+    const int* __restrict__ tile_item, const int* __restrict__ tile_q0, const int* __restrict__ cu_tokens, int heads,
+    int head_dim, int query_tile, int ranges) {
+  const int head = blockIdx.x, item = tile_item[blockIdx.y], q0 = tile_q0[blockIdx.y];
+  const int tok0 = cu_tokens[item] + q0, left = cu_tokens[item + 1] - tok0;
+  const int rows = left < query_tile ? left : query_tile;
+  const int quads = head_dim / 4, i = blockIdx.z * 256 + threadIdx.x;
+  if (i >= rows * quads) return;
+  const int row = i / quads, d = (i - row * quads) * 4;
+  const int64_t first = ((int64_t)blockIdx.y * heads + head) * ranges * query_tile + row;
+  float m = -INFINITY;
+  for (int r = 0; r < ranges; ++r) m = fmaxf(m, states[(first + (int64_t)r * query_tile) * 2]);
+  float total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < ranges; ++r) {
+    const int64_t record = first + (int64_t)r * query_tile;
+    const float2 state = *reinterpret_cast<const float2*>(states + record * 2);
+    const float4 v = *reinterpret_cast<const float4*>(sums + record * head_dim + d);
+    // (a range without keys: a maximum of -inf, sums of 0; a maximum that is no number stays one in its sums)
+    const float c = state.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state.x - m);
+    total = fmaf(state.y, c, total);
+    x[0] = fmaf(v.x, c, x[0]);
+    x[1] = fmaf(v.y, c, x[1]);
+    x[2] = fmaf(v.z, c, x[2]);
+    x[3] = fmaf(v.w, c, x[3]);
+  }
+  if (total == 0.f) return;                // (a query that sees nothing: its row stays, as without ranges)
+  const float inv = 1.f / total;
+  *reinterpret_cast<uint2*>(out + (tok0 + row) * out_stride + (int64_t)head * head_dim + d) =
+      make_uint2(pack2_bf16(x[0] * inv, x[1] * inv), pack2_bf16(x[2] * inv, x[3] * inv));
 }
 
 extern "C" int ps_attention_prefill_int4(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool,
                                          void* out, int64_t out_stride, const int* tile_item, const int* tile_q0,
                                          int tiles, const int* cu_tokens, const int* kv_lens, const int* tables,
-                                         int table_width, int heads, int kv_heads, int head_dim, int page_size,
-                                         int num_pages, float scale, int window, int max_kv_len, int query_tile,
-                                         const float* sink, float softcap, void* stream) {
+                                         int table_width, int heads, int kv_heads, int head_dim,
+                                         int page_size, int num_pages, float scale, int window, int max_kv_len,
+                                         int query_tile, const float* sink, float softcap, int ranges,
+                                         float* partial, int64_t partial_floats, void* stream) {
   const char* who = "ps_attention_prefill_int4";
   PS_REQUIRE(tiles >= 0 && heads > 0 && kv_heads > 0 && page_size > 0 && num_pages > 0 && table_width > 0,
              "%s: bad sizes", who);
@@ -40,10 +83,9 @@ extern "C" int ps_attention_prefill_int4(const void* q, int64_t q_stride, const 
   PS_REQUIRE(page_size % 8 == 0 && page_size <= (1 << 20),
              "%s: pages of a cache in 4 bits hold a multiple of 8 keys, not %d", who, page_size);
   PS_REQUIRE(tiles <= 65535, "%s: too many tiles (%d)", who, tiles);
-  PS_REQUIRE(query_tile == AP_QUERIES || (query_tile == AP_QUERIES / 2 && head_dim <= 128) ||
-                 (query_tile == AP_QUERIES * 2 && head_dim <= AP_LARGE_HEAD_DIM),
-             "%s: tiles of %d, (head sizes up to 128) %d or (head sizes up to %d) %d queries, not %d", who,
-             AP_QUERIES, AP_QUERIES / 2, AP_LARGE_HEAD_DIM, AP_QUERIES * 2, query_tile);
+  PS_REQUIRE(query_tile == AP_QUERIES || (query_tile == AP_QUERIES * 2 && head_dim <= AP_LARGE_HEAD_DIM),
+             "%s: tiles of %d or, head sizes up to %d, %d queries, not %d", who, AP_QUERIES, AP_LARGE_HEAD_DIM,
+             AP_QUERIES * 2, query_tile);
   PS_REQUIRE((int64_t)num_pages * kv_heads * page_size < ((int64_t)1 << 32),
              "%s: a pool of %d pages x %d heads x %d keys has 2^32 key rows or more", who, num_pages, kv_heads, page_size);
   PS_REQUIRE(scale > 0.f, "%s: the score scale must be positive, got %g", who, scale);
@@ -51,6 +93,12 @@ extern "C" int ps_attention_prefill_int4(const void* q, int64_t q_stride, const 
              table_width, AP_TABLE_MAX);
   PS_REQUIRE((q_stride % 8) == 0 && ((uintptr_t)q % 16) == 0 && (out_stride % 4) == 0 && ((uintptr_t)out % 8) == 0,
              "%s: q and out rows must allow 16- and 8-byte accesses", who);
+  PS_REQUIRE(ranges >= 1 && ranges <= 64, "%s: 1 to 64 ranges of keys, not %d", who, ranges);
+  const int64_t records = (int64_t)tiles * heads * ranges * query_tile;
+  PS_REQUIRE(ranges == 1 || tiles == 0 ||
+                 (partial != nullptr && (uintptr_t)partial % 16 == 0 && partial_floats >= records * (head_dim + 2)),
+             "%s: %d ranges need %lld floats of scratch from a multiple of 16 bytes on, not %lld", who, ranges,
+             (long long)(records * (head_dim + 2)), (long long)partial_floats);
   if (tiles == 0) return 0;
   int page_shift = -1;
   if ((page_size & (page_size - 1)) == 0) {
@@ -59,24 +107,23 @@ extern "C" int ps_attention_prefill_int4(const void* q, int64_t q_stride, const 
   }
   hipStream_t s = (hipStream_t)stream;
   const AttnExtras extra = {sink, nullptr, 0, softcap, nullptr, 1.f};
-  dim3 grid(heads, tiles);
+  dim3 grid(heads, tiles, ranges);
+  float* states = ranges > 1 ? partial + records * head_dim : nullptr;
   // four waves along the keys where few blocks see many keys, as for the other cache
-  const bool wide = (int64_t)tiles * heads <= ps_compute_units() * 2 && (max_kv_len <= 0 || max_kv_len >= 512);
-#define PS_LAUNCH_P4(THREADS, ...)                                                                              \
-  hipLaunchKernelGGL((attention_prefill_int4_kernel<__VA_ARGS__>), grid, dim3(THREADS), 0, s, (const bf16_t*)q, \
+  const bool wide = (int64_t)tiles * heads * ranges <= ps_compute_units() * 2 && (max_kv_len <= 0 || max_kv_len >= 512);
+#define PS_LAUNCH_P4(NDB, KS, QW, KR)                                                                            \
+  hipLaunchKernelGGL((attention_prefill_int4_kernel<NDB, KS, QW, KR>), grid, dim3(64 * KS * QW), 0, s, (const bf16_t*)q, \
                      q_stride, (const uint8_t*)k_pool, (const uint8_t*)v_pool, (bf16_t*)out, out_stride,        \
                      tile_item, tile_q0, cu_tokens, kv_lens, tables, table_width, heads, kv_heads, page_size,   \
-                     page_shift, num_pages, scale, window, extra)
+                     page_shift, num_pages, scale, window, extra, ranges, partial, states)
 #define PS_TILES_P4(NDB)                                      \
   case NDB:                                                   \
     if (query_tile == AP_QUERIES * 2) {                       \
-      if constexpr (NDB <= AP_LARGE_HEAD_DIM / 16) PS_LAUNCH_P4(256, NDB, 1, 4, 2); \
-    } else if (query_tile != AP_QUERIES) {                    \
-      if constexpr (NDB <= 8) PS_LAUNCH_P4(256, NDB, 4, 1);   \
+      if constexpr (NDB <= 4) PS_LAUNCH_P4(NDB, 1, 4, 2);        \
     } else if (NDB <= 8 && wide) {                            \
-      if constexpr (NDB <= 8) PS_LAUNCH_P4(512, NDB, 4);      \
+      if constexpr (NDB <= 8) PS_LAUNCH_P4(NDB, 4, 2, 1);        \
     } else {                                                  \
-      PS_LAUNCH_P4(256, NDB, 2);                              \
+      PS_LAUNCH_P4(NDB, 2, 2, 1);                                \
     }                                                         \
     break
   switch (head_dim / 16) {
@@ -95,10 +142,15 @@ extern "C" int ps_attention_prefill_int4(const void* q, int64_t q_stride, const 
     PS_TILES_P4(13);
     PS_TILES_P4(14);
     PS_TILES_P4(15);
-    default: PS_LAUNCH_P4(256, 16, 2);
+    default: PS_LAUNCH_P4(16, 2, 2, 1);
   }
 #undef PS_TILES_P4
 #undef PS_LAUNCH_P4
   PS_CHECK_LAUNCH("ps_attention_prefill_int4");
+  if (ranges > 1) {
+    hipLaunchKernelGGL(attention_prefill_int4_join_kernel, dim3(heads, tiles, (query_tile * (head_dim / 4) + 255) / 256), dim3(256), 0, s,
+                       partial, states, (bf16_t*)out, out_stride, tile_item, tile_q0, cu_tokens, heads, head_dim, query_tile, ranges);
+    PS_CHECK_LAUNCH("ps_attention_prefill_int4(join)");
+  }
   return 0;
 }

@@ -2,11 +2,13 @@
 faces (on CPU tensors that claim to be on the device) and those at the C entries, which return before any launch."""
 
 import ctypes
+import os
 from unittest import mock
 
 import pytest
 import torch
 
+import kernel_code
 import plain_int4 as plain
 from pagedserve_amd.ops import kernels, library
 
@@ -101,7 +103,7 @@ def test_tensors_on_two_devices(on_gpu):
     for function, args in ((kernels.kv_write_int4, _write()), (kernels.kv_read_int4, _write()),
                            (kernels.attention_decode_int4, _decode(tok_list=_ints(2), sink=torch.zeros(4), splits=2,
                                                                    partial=torch.zeros(4000))),
-                           (kernels.attention_prefill_int4, _prompt(sink=torch.zeros(4))),
+                           (kernels.attention_prefill_int4, _prompt(sink=torch.zeros(4), ranges=2, partial=torch.zeros(9))),
                            (kernels.token_logprobs, _logprobs(entropy=torch.zeros(3), ranks=_ints(3), top_ids=_ints(3, 2),
                                                               top_logprobs=torch.zeros(3, 2), partial=torch.zeros(9)))):
         names = [name for name, value in args.items() if isinstance(value, torch.Tensor)]
@@ -140,7 +142,8 @@ def test_decode_refused(on_gpu, changed, message):
     ({"q": torch.zeros(3, 256), "out": torch.zeros(3, 256)}, "bfloat16"), ({"heads": 3}, "do not fit"),
     ({"tile_q0": _ints(2)}, "inconsistent"), ({"cu_tokens": _ints(3)}, "inconsistent"), ({"tables": _ints(2, 5)}, "inconsistent"),
     ({"kv_lens": _ints(2)[::2]}, None), ({"kv_lens": _ints(4)[::2], "cu_tokens": _ints(3), "tables": _ints(2, 5)}, "contiguous"),
-    ({"tile_item": _ints(1).long()}, "int32"), ({"sink": torch.zeros(5)}, "one float per head")])
+    ({"tile_item": _ints(1).long()}, "int32"), ({"sink": torch.zeros(5)}, "one float per head"),
+    ({"ranges": 2, "partial": torch.zeros(9, dtype=BF16)}, "partial"), ({"ranges": 2, "partial": torch.zeros(9, 2)[:, 0]}, "contiguous")])
 def test_prompt_refused(on_gpu, changed, message):
     if message is None:
         kernels.attention_prefill_int4(**_prompt(**changed))
@@ -199,19 +202,19 @@ def test_decode_refused_by_the_library(changed, message):
 
 
 PORTIONS = dict(table_width=5, heads=4, kv_heads=2, head_dim=64, page_size=16, num_pages=4, scale=0.125, window=0, max_kv_len=0,
-                query_tile=64)
+                query_tile=64, sink=0, softcap=0.0, ranges=1)
 
 
 @pytest.mark.parametrize("changed,message", [
     ({"heads": 5}, "multiple of kv_heads"), ({"head_dim": 72}, "multiple of 16"), ({"head_dim": 272}, "up to 256"),
     ({"page_size": 20}, "multiple of 8"), ({"query_tile": 96}, "queries"), ({"query_tile": 128, "head_dim": 128}, "queries"),
-    ({"query_tile": 32, "head_dim": 160}, "queries"), ({"scale": 0.0}, "positive"), ({"table_width": 2049}, "exceed"),
+    ({"query_tile": 32}, "queries"), ({"ranges": 0}, "ranges"), ({"ranges": 65}, "ranges"), ({"ranges": 2}, "floats of scratch"), ({"scale": 0.0}, "positive"), ({"table_width": 2049}, "exceed"),
     ({"num_pages": 1 << 28}, "key rows")])
 def test_prompt_refused_by_the_library(changed, message):
     sizes = dict(PORTIONS, **changed)
-    status, error = _c("ps_attention_prefill_int4", 0, 256, 0, 0, 0, 256, 0, 0, 1, 0, 0, 0, *sizes.values(), 0, 0.0, 0)
+    status, error = _c("ps_attention_prefill_int4", 0, 256, 0, 0, 0, 256, 0, 0, 1, 0, 0, 0, *sizes.values(), 0, 0, 0)
     assert status == 1 and message in error
-    status, error = _c("ps_attention_prefill_int4", 0, 252, 0, 0, 0, 256, 0, 0, 1, 0, 0, 0, *PORTIONS.values(), 0, 0.0, 0)
+    status, error = _c("ps_attention_prefill_int4", 0, 252, 0, 0, 0, 256, 0, 0, 1, 0, 0, 0, *PORTIONS.values(), 0, 0, 0)
     assert status == 1 and "accesses" in error
 
 
@@ -231,7 +234,7 @@ def test_nothing_to_do_is_no_launch():
     assert _c("ps_token_logprobs", 0, 50, 0, 50, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)[0] == 0
     sizes = dict(ATTEND, count=0)
     assert _c("ps_attention_decode_int4", 0, 256, 0, 0, 0, 256, 0, 0, 0, 0, 0, 0, *sizes.values(), 0, 0.0, 1, 0)[0] == 0
-    assert _c("ps_attention_prefill_int4", 0, 256, 0, 0, 0, 256, 0, 0, 0, 0, 0, 0, *PORTIONS.values(), 0, 0.0, 0)[0] == 0
+    assert _c("ps_attention_prefill_int4", 0, 256, 0, 0, 0, 256, 0, 0, 0, 0, 0, 0, *PORTIONS.values(), 0, 0, 0)[0] == 0
 
 
 @pytest.mark.parametrize("dim", [1, 7, 32, 33, 64, 250])
@@ -249,3 +252,22 @@ def test_the_form_itself(dim):
     assert bool((off <= 1.26 * per).all()) and groups == -(-dim // 32)
     assert float((off <= 0.51 * per).double().mean()) > 0.9
     assert kernels.int4_row_bytes(dim) == 18 * groups
+
+
+@pytest.mark.skipif(kernel_code.disassembler() is None, reason="no disassembler")
+@pytest.mark.parametrize("kernel", ["attention_prefill_int4_kernel", "attention_decode_int4_heads_kernel"])
+def test_no_register_is_used_before_its_load(kernel, tmp_path):
+    """Every instance of the kernels that read their operands from LDS by assembly, as built."""
+    path = os.path.join(library.in_tree_dir(), library.LIB_NAME)
+    if not os.path.isfile(path):
+        pytest.skip("the library is not built in the tree")
+    images = [image for image in kernel_code.code_objects(path, library.ARCH) if kernel.encode() in image]
+    assert images, "no source file holds this kernel"
+    seen = 0
+    for image in images:
+        for name, code in kernel_code.kernels(kernel_code.disassemble(image, library.ARCH, tmp_path)):
+            if kernel in name:
+                seen += 1
+                assert any(operation.startswith("ds_read") for _, operation, _, _ in code), name
+                assert not kernel_code.early_uses(code), (name, kernel_code.early_uses(code)[:4])
+    assert seen > 3

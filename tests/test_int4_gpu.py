@@ -250,21 +250,65 @@ def test_prompt_portions(kv_heads, group, dim, page, counts, starts, window, sin
                                   softcap)) for i in range(len(counts))]
     expected = [torch.cat([part[which] for part in parts]) for which in range(3)]
     limit = plain.allowed(*expected, BF16, True)
-    for size in (32, 64, 128):
-        if size == 32 and dim > 128 or size == 128 and dim > 64:
+    for size in (64, 128):
+        if size == 128 and dim > 64:
             continue
         tiles = [(item, q0) for item, count in enumerate(counts) for q0 in range(0, count, size)]
-        for max_kv_len in (100, 0):                          # (steers the launch)
+        for max_kv_len, ranges in ((100, None), (0, 1), (600, 1), (0, 2), (600, 5)):      # (they steer the launch)
             out = torch.full((tokens + 1, heads * dim), -9.0, dtype=BF16).cuda()
             kernels.attention_prefill_int4(q.cuda(), *pools, out[:tokens], _ints([t[0] for t in tiles]),
                                            _ints([t[1] for t in tiles]), _ints(cu), _ints(lengths), tables.cuda(), heads,
-                                           scale, window, max_kv_len, size, sinks, softcap)
-            assert bool(((out[:tokens].double().cpu() - expected[0]).abs() <= limit).all()), (size, max_kv_len)
+                                           scale, window, max_kv_len, size, sinks, softcap, ranges)
+            assert bool(((out[:tokens].double().cpu() - expected[0]).abs() <= limit).all()), (size, max_kv_len, ranges)
             assert bool((out[tokens] == -9.0).all())
     out = torch.zeros((tokens, heads * dim), dtype=BF16).cuda()
     kernels.attention_decode_int4(q.cuda(), *pools, out, _ints(items), _ints(positions), tables.cuda(), heads, scale, 1,
                                   None, window, sink=sinks, softcap=softcap)
     assert bool(((out.double().cpu() - expected[0]).abs() <= limit).all())
+
+
+LONG = [
+    # kv_heads, group, dim, page, counts, starts, window, sink, softcap, query_tile
+    (2, 2, 64, 16, (70, 3), (1500, 40), 0, True, 0.0, 64), (1, 4, 64, 24, (130,), (900,), 300, False, 0.0, 128),
+    (1, 2, 128, 8, (20, 64), (1100, 700), 0, False, 20.0, 64), (1, 1, 256, 16, (66,), (800,), -256, True, 0.0, 64)]
+
+
+@pytest.mark.parametrize("kv_heads,group,dim,page,counts,starts,window,sink,softcap,size", LONG)
+def test_prompt_portions_in_ranges(kv_heads, group, dim, page, counts, starts, window, sink, softcap, size):
+    """Ranges of keys of long contexts, as the rule cuts them and in numbers that leave some without keys; the scratch holds
+    what is no number before, and what lies behind its records stays."""
+    from pagedserve_amd.ops import kernels
+
+    heads = kv_heads * group
+    tables, pages, _, positions = _requests(counts, starts, page, 44)
+    lengths = [a + b for a, b in zip(counts, starts)]
+    pools, kept = _cache(tables, pages, lengths, kv_heads, dim, page, 45)
+    tokens = sum(counts)
+    g = torch.Generator().manual_seed(46)
+    q = (torch.randn((tokens, heads * dim), generator=g) * 1.5).to(BF16)
+    sinks = torch.randn(heads, generator=g).cuda() if sink else None
+    scale = dim ** -0.5
+    cu = [sum(counts[:i]) for i in range(len(counts) + 1)]
+    parts = [list(plain.attention(q[cu[i]:cu[i + 1]], *kept[i], positions[cu[i]:cu[i + 1]], heads, scale, window, sinks,
+                                  softcap)) for i in range(len(counts))]
+    expected = [torch.cat([part[which] for part in parts]) for which in range(3)]
+    limit = plain.allowed(*expected, BF16, True)
+    tiles = [(item, q0) for item, count in enumerate(counts) for q0 in range(0, count, size)]
+    rule = kernels.prefill_int4_ranges(len(tiles), heads, max(lengths))
+    assert rule > 1
+    for ranges in (rule, 7, 64):
+        needed = len(tiles) * heads * ranges * size * (dim + 2)
+        partial = torch.full((needed + 8,), math.nan).cuda()
+        out = torch.full((tokens + 1, heads * dim), -9.0, dtype=BF16).cuda()
+        kernels.attention_prefill_int4(q.cuda(), *pools, out[:tokens], _ints([t[0] for t in tiles]),
+                                       _ints([t[1] for t in tiles]), _ints(cu), _ints(lengths), tables.cuda(), heads, scale,
+                                       window, max(lengths), size, sinks, softcap, ranges, partial)
+        assert bool(((out[:tokens].double().cpu() - expected[0]).abs() <= limit).all()), ranges
+        assert bool((out[tokens] == -9.0).all()) and bool(partial[needed:].isnan().all())
+    with pytest.raises(kernels.KernelError, match="floats of scratch"):
+        kernels.attention_prefill_int4(q.cuda(), *pools, out[:tokens], _ints([t[0] for t in tiles]),
+                                       _ints([t[1] for t in tiles]), _ints(cu), _ints(lengths), tables.cuda(), heads, scale,
+                                       window, max(lengths), size, sinks, softcap, 64, partial[:-9])
 
 
 @pytest.mark.parametrize("bad", ["key", "value"])
@@ -280,11 +324,11 @@ def test_a_later_nan_reaches_no_earlier_query(bad):
     kernels.kv_write_int4(rows[0].cuda(), rows[1].cuda(), k_pool, v_pool, *index)
     q = torch.randn((40, 64), generator=torch.Generator().manual_seed(53)).to(BF16)
     expected = list(plain.attention(q[:39], kept[0][0][:39], kept[0][1][:39], positions[:39], 1, 0.125))
-    for size in (32, 64, 128):
+    for size, ranges in ((64, 1), (128, 1), (64, 3), (128, 2)):
         tiles = list(range(0, 40, size))
         out = torch.zeros(40, 64, dtype=BF16).cuda()
         kernels.attention_prefill_int4(q.cuda(), k_pool, v_pool, out, _ints([0] * len(tiles)), _ints(tiles), _ints([0, 40]),
-                                       _ints([40]), tables.cuda(), 1, 0.125, query_tile=size)
+                                       _ints([40]), tables.cuda(), 1, 0.125, query_tile=size, ranges=ranges)
         assert bool(((out[:39].double().cpu() - expected[0]).abs() <= plain.allowed(*expected, BF16, True)).all())
         assert bool(out[39].isnan().any())
     out = torch.zeros(40, 64, dtype=BF16).cuda()
