@@ -46,15 +46,40 @@ __device__ inline float int4_step(float high, float low) {
   return fabsf(step) < 1.17549435e-38f ? 0.f : __uint_as_float(size | (bits & 0x80000000u));
 }
 
-// The code of x under a step other than 0.  The quotient is correctly rounded, so that only a quotient that is
-// exactly half way between two whole numbers leaves open on which side x / d lies: there the remainder, which is
-// exact, decides.
-__device__ inline int int4_code(float x, float step) {
-  const float ratio = x / step;
-  float whole = rintf(ratio);
-  if (fabsf(ratio - whole) == 0.5f) {
-    const float rest = fmaf(-ratio, step, x);
-    if (rest != 0.f) whole = (rest > 0.f) == (step > 0.f) ? ceilf(ratio) : floorf(ratio);
+// The codes of eight numbers, less 8, under a step other than 0; BF16: numbers of 8 significant bits.
+//
+// The product with the step's reciprocal, which may be off in its last place, is x / d but for some last places.  Of
+// numbers of 8 bits the quotient lies a 2^9th of itself or more from a half or on it: one correction by the remainder
+// makes it exact there, and rounding it gives the code.  (Not where the remainder is below the normal floats.)  Else the
+// whole number nearest to the product is taken, and the remainder of that, at most about half a step, is exact (a
+// multiple of the last place of x or of d, whichever is lower, and within 24 bits of it) and decides, ties to even.
+template <bool BF16>
+__device__ inline void int4_codes(const float* x, float step, float* codes) {
+  const float inverse = __builtin_amdgcn_rcpf(step), half = fabsf(step) * 0.5f;
+  if (BF16 && half >= 7.8886091e-31f) {       // 2^-100
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float ratio = x[i] * inverse;
+      codes[i] = rintf(fmaf(fmaf(-ratio, step, x[i]), inverse, ratio));
+    }
+  } else {
+    float rest[8], most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      codes[i] = rintf(x[i] * inverse);
+      rest[i] = fmaf(-codes[i], step, x[i]);
+      most = fmaxf(most, fabsf(rest[i]));
+    }
+    if (most >= half) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool odd = fabsf(fmaf(-2.f, rintf(codes[i] * 0.5f), codes[i])) == 1.f;
+        const bool off = (fabsf(rest[i]) > half) | ((fabsf(rest[i]) == half) & odd);
+        const float by = (rest[i] > 0.f) == (step > 0.f) ? 1.f : -1.f;
+        codes[i] += off ? by : 0.f;
+      }
+    }
   }
-  return (int)fminf(fmaxf(whole, -8.f), 7.f) + 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) codes[i] = fminf(fmaxf(codes[i], -8.f), 7.f);
 }

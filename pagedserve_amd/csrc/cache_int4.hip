@@ -1,8 +1,15 @@
 // The step's keys and values into their pages as 4-bit codes, and back (see cache_int4.h for the form).
 //
-// 16 lanes take one group of one head of one token: two neighbouring dimensions to a lane, which are one
-// byte of the page, and the extremes over the group are four exchanges within a row of lanes.  Keys and values are two
-// halves of one grid.  What bounds both is the trip: position -> block table -> page.
+// Four lanes share a row of a head: 8 dimensions of each of its G groups to a lane, which are 4 G bytes side by side in
+// the page for keys and for values alike, so that a row comes by loads of 16 bytes and leaves by stores of 4 G.  The
+// extremes over a group are two exchanges among the four lanes.  Keys and values are two halves of one grid.  Where there
+// are many tokens a block of one wave takes 16 of them of one head: neighbouring tokens lie side by side in the page, and the lines
+// of 128 bytes that they share are written by one compute unit.
+//
+// Of 2 x 1,024 tokens, 25 heads of 64, bfloat16: stored in 7.6 us (2.2 TB/s of all bytes), read back in 6.5 (2.6 TB/s); 8,192
+// tokens, 8 heads of 128: 16.9 and 16.8 us; 8 tokens of 12 heads: 2.9 and 2.9.  What bounds it is the trip position ->
+// block table -> page -> row, which all waves make at the same time.  (Blocks of two and four waves: the same within 3 %;
+// with 16 lanes to a group, a byte each, 20 and 13.9 us, 47 and 35.)
 #include <math.h>
 
 #include "cache_int4.h"
@@ -23,64 +30,218 @@ __device__ inline Int4Place int4_place(const int* __restrict__ tok_item, const i
   return {page >= 0 && page < num_pages ? page : -1, pos - logical * page_size};
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void kv_write_int4_kernel(
-    const T* __restrict__ k, const T* __restrict__ v, int64_t k_stride, int64_t v_stride,
-    uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool, const int* __restrict__ tok_item,
-    const int* __restrict__ tok_pos, const int* __restrict__ tables, int table_width, int kv_heads, int head_dim,
-    int groups, int page_size, int num_pages) {
-  const int t = blockIdx.x;
-  const bool values = blockIdx.z != 0;
-  const int unit = blockIdx.y * 16 + threadIdx.x / 16;      // which group of which head
-  const int n = threadIdx.x & 15;
-  if (unit >= kv_heads * groups) return;                     // (whole rows of lanes)
-  const int head = unit / groups, g = unit - head * groups;
-  const Int4Place place = int4_place(tok_item, tok_pos, tables, table_width, t, page_size, num_pages);
-  if (place.page < 0) return;
-  const T* row = (values ? v + t * v_stride : k + t * k_stride) + (int64_t)head * head_dim;
-  const int d0 = g * PS_INT4_GROUP + 2 * n;
-  const float a = d0 < head_dim ? to_float(row[d0]) : 0.f;
-  const float b = d0 + 1 < head_dim ? to_float(row[d0 + 1]) : 0.f;
-  const float high = lanes_max<16>(fmaxf(a, b));
-  const float low = -lanes_max<16>(fmaxf(-a, -b));
-  // (a maximum passes over a NaN: what is not finite is counted apart)
-  const bool finite = fabsf(a) < INFINITY && fabsf(b) < INFINITY;
-  const bool all_finite = lanes_max<16>(finite ? 0.f : 1.f) == 0.f;
-  const float step = all_finite ? int4_step(high, low) : __uint_as_float(0x7fc00000u);
-  int codes = 0x88;
-  if (all_finite && step != 0.f) codes = int4_code(a, step) | int4_code(b, step) << 4;
-  uint8_t* page = (values ? v_pool : k_pool) + int4_page_at(place.page, kv_heads, head, page_size, groups);
-  const int at = values ? int4_value_byte(16 * g + n, groups) : int4_key_word(4 * g + (n >> 2), groups) + (n & 3);
-  page[place.within * 16 * groups + at] = (uint8_t)codes;
-  if (n == 0)
-    reinterpret_cast<uint16_t*>(page + page_size * 16 * groups)[place.within * groups + g] =
-        (uint16_t)(__float_as_uint(step) >> 16);
+// A row's 8 dimensions from d0 on as numbers, zeros behind the last; WIDE: by loads of 16 bytes.
+template <bool WIDE, typename T>
+__device__ inline void int4_load8(const T* __restrict__ row, int d0, int head_dim, float* x) {
+  // (every load is made, from the row's last dimensions where there are none: one in a branch is waited for in it)
+  const bool inside = d0 < head_dim;
+  if constexpr (WIDE && sizeof(T) == 2) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(row + (inside ? d0 : head_dim - 8));
+    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(inside ? words[i] << 16 : 0u);
+      x[2 * i + 1] = __uint_as_float(inside ? words[i] & 0xffff0000u : 0u);
+    }
+  } else if constexpr (WIDE) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 part = *reinterpret_cast<const float4*>(row + (inside ? d0 : head_dim - 8) + 4 * i);
+      x[4 * i] = inside ? part.x : 0.f;
+      x[4 * i + 1] = inside ? part.y : 0.f;
+      x[4 * i + 2] = inside ? part.z : 0.f;
+      x[4 * i + 3] = inside ? part.w : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float value = to_float(row[d0 + i < head_dim ? d0 + i : head_dim - 1]);
+      x[i] = d0 + i < head_dim ? value : 0.f;
+    }
+  }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void kv_read_int4_kernel(
-    const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool, T* __restrict__ k, T* __restrict__ v,
-    int64_t k_stride, int64_t v_stride, const int* __restrict__ tok_item, const int* __restrict__ tok_pos,
-    const int* __restrict__ tables, int table_width, int kv_heads, int head_dim, int groups, int page_size,
-    int num_pages) {
-  const int t = blockIdx.x;
+template <bool WIDE, typename T>
+__device__ inline void int4_store8(T* __restrict__ row, int d0, int head_dim, const float* x) {
+  if constexpr (WIDE) {
+    if (d0 >= head_dim) return;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(row + d0) =
+          make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+    } else {
+      *reinterpret_cast<float4*>(row + d0) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(row + d0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (d0 + i < head_dim) row[d0 + i] = from_float<T>(x[i]);
+  }
+}
+
+// N words from or to an address that is a multiple of the largest power of two in 4 N bytes, 16 at most.
+template <int N>
+__device__ inline void int4_load_words(const uint8_t* from, uint32_t* words) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(from)[i];
+      words[4 * i] = v.x;
+      words[4 * i + 1] = v.y;
+      words[4 * i + 2] = v.z;
+      words[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 v = reinterpret_cast<const uint2*>(from)[i];
+      words[2 * i] = v.x;
+      words[2 * i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) words[i] = reinterpret_cast<const uint32_t*>(from)[i];
+  }
+}
+template <int N>
+__device__ inline void int4_store_words(uint8_t* to, const uint32_t* words) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      reinterpret_cast<uint4*>(to)[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) reinterpret_cast<uint2*>(to)[i] = make_uint2(words[2 * i], words[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) reinterpret_cast<uint32_t*>(to)[i] = words[i];
+  }
+}
+
+// The quarter of a value's row holds byte i of group g's word as its byte i G + g: from the words of the groups, and back.
+template <int G, bool BACK>
+__device__ inline void int4_turn_bytes(uint32_t* words) {
+  uint32_t turned[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) turned[g] = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int at = i * G + g;
+      if (BACK) turned[g] |= (words[at / 4] >> (8 * (at % 4)) & 0xffu) << (8 * i);
+      else turned[at / 4] |= (words[g] >> (8 * i) & 0xffu) << (8 * (at % 4));
+    }
+#pragma unroll
+  for (int g = 0; g < G; ++g) words[g] = turned[g];
+}
+
+// The token and head of four lanes: 2^token_shift tokens by 16 >> token_shift heads to a block.
+__device__ inline void int4_row_of(int token_shift, int& t, int& head) {
+  const int local = threadIdx.x >> 2;
+  t = (blockIdx.x << token_shift) + (local & ((1 << token_shift) - 1));
+  head = blockIdx.y * (16 >> token_shift) + (local >> token_shift);
+}
+
+template <typename T, int G, bool WIDE>
+__global__ __launch_bounds__(64) void kv_write_int4_kernel(
+    const T* __restrict__ k, const T* __restrict__ v, int64_t k_stride, int64_t v_stride,
+    uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool, const int* __restrict__ tok_item,
+    const int* __restrict__ tok_pos, const int* __restrict__ tables, int table_width, int tokens, int kv_heads,
+    int head_dim, int page_size, int num_pages, int token_shift) {
   const bool values = blockIdx.z != 0;
-  const int unit = blockIdx.y * 16 + threadIdx.x / 16;
-  const int n = threadIdx.x & 15;
-  if (unit >= kv_heads * groups) return;
-  const int head = unit / groups, g = unit - head * groups;
+  const int c = threadIdx.x & 3;
+  int t, head;
+  int4_row_of(token_shift, t, head);
+  if (t >= tokens || head >= kv_heads) return;               // (whole groups of four lanes)
+  const T* row = (values ? v + t * v_stride : k + t * k_stride) + (int64_t)head * head_dim;
+  float x[G][8];
+#pragma unroll
+  for (int g = 0; g < G; ++g) int4_load8<WIDE>(row, g * PS_INT4_GROUP + 8 * c, head_dim, x[g]);
   const Int4Place place = int4_place(tok_item, tok_pos, tables, table_width, t, page_size, num_pages);
   if (place.page < 0) return;
-  const uint8_t* page = (values ? v_pool : k_pool) + int4_page_at(place.page, kv_heads, head, page_size, groups);
-  const int at = values ? int4_value_byte(16 * g + n, groups) : int4_key_word(4 * g + (n >> 2), groups) + (n & 3);
-  const int codes = page[place.within * 16 * groups + at];
-  const uint32_t bits =
-      reinterpret_cast<const uint16_t*>(page + page_size * 16 * groups)[place.within * groups + g];
-  const float step = __uint_as_float(bits << 16);
+  uint32_t words[G], steps[(G + 1) / 2];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    float high = x[g][0], low = x[g][0], finite = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      high = fmaxf(high, x[g][i]);
+      low = fminf(low, x[g][i]);
+      finite = fmaf(x[g][i], 0.f, finite);                   // (NaN by an infinity or a NaN, which an extreme passes over)
+    }
+    high = lanes_max<4>(high);
+    low = -lanes_max<4>(-low);
+    const bool all_finite = lanes_max<4>(finite == 0.f ? 0.f : 1.f) == 0.f;
+    const float step = all_finite ? int4_step(high, low) : __uint_as_float(0x7fc00000u);
+    words[g] = 0x88888888u;
+    if (all_finite && step != 0.f) {
+      float codes[8];
+      int4_codes<sizeof(T) == 2>(x[g], step, codes);
+      uint32_t halves[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // four codes less 8 as the digits of a number to the base of 16, and 8 to each
+        float digits = 0.f;
+#pragma unroll
+        for (int i = 3; i >= 0; --i) digits = fmaf(digits, 16.f, codes[4 * h + i]);
+        halves[h] = (uint32_t)(digits + 34952.f);
+      }
+      words[g] = halves[0] | halves[1] << 16;
+    }
+    const uint32_t bits = __float_as_uint(step) >> 16;
+    steps[g / 2] = g % 2 ? steps[g / 2] | bits << 16 : bits;
+  }
+  if (values) int4_turn_bytes<G, false>(words);
+  uint8_t* page = (values ? v_pool : k_pool) + int4_page_at(place.page, kv_heads, head, page_size, G);
+  int4_store_words<G>(page + place.within * (16 * G) + c * (4 * G), words);
+  if (c == 0) {
+    uint8_t* to = page + page_size * (16 * G) + place.within * (2 * G);
+    if constexpr (G % 2 == 0) {
+      int4_store_words<G / 2>(to, steps);
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g) reinterpret_cast<uint16_t*>(to)[g] = (uint16_t)(steps[g / 2] >> (16 * (g % 2)));
+    }
+  }
+}
+
+template <typename T, int G, bool WIDE>
+__global__ __launch_bounds__(64) void kv_read_int4_kernel(
+    const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool, T* __restrict__ k, T* __restrict__ v,
+    int64_t k_stride, int64_t v_stride, const int* __restrict__ tok_item, const int* __restrict__ tok_pos,
+    const int* __restrict__ tables, int table_width, int tokens, int kv_heads, int head_dim, int page_size,
+    int num_pages, int token_shift) {
+  const bool values = blockIdx.z != 0;
+  const int c = threadIdx.x & 3;
+  int t, head;
+  int4_row_of(token_shift, t, head);
+  if (t >= tokens || head >= kv_heads) return;
+  const Int4Place place = int4_place(tok_item, tok_pos, tables, table_width, t, page_size, num_pages);
+  if (place.page < 0) return;
+  const uint8_t* page = (values ? v_pool : k_pool) + int4_page_at(place.page, kv_heads, head, page_size, G);
+  uint32_t words[G], steps[(G + 1) / 2];
+  int4_load_words<G>(page + place.within * (16 * G) + c * (4 * G), words);
+  const uint8_t* from = page + page_size * (16 * G) + place.within * (2 * G);
+  if constexpr (G % 2 == 0) {
+    int4_load_words<G / 2>(from, steps);
+  } else {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint32_t bits = reinterpret_cast<const uint16_t*>(from)[g];
+      steps[g / 2] = g % 2 ? steps[g / 2] | bits << 16 : bits;
+    }
+  }
+  if (values) int4_turn_bytes<G, true>(words);
   T* row = (values ? v + t * v_stride : k + t * k_stride) + (int64_t)head * head_dim;
-  const int d0 = g * PS_INT4_GROUP + 2 * n;
-  if (d0 < head_dim) row[d0] = from_float<T>((float)((codes & 15) - 8) * step);
-  if (d0 + 1 < head_dim) row[d0 + 1] = from_float<T>((float)((codes >> 4) - 8) * step);
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const float step = __uint_as_float(steps[g / 2] >> (16 * (g % 2)) << 16);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)((int)(words[g] >> (4 * i) & 15u) - 8) * step;
+    int4_store8<WIDE>(row, g * PS_INT4_GROUP + 8 * c, head_dim, x);
+  }
 }
 
 static int check_int4_rows(const char* who, int64_t k_stride, int64_t v_stride, int table_width, int tokens,
@@ -96,6 +257,30 @@ static int check_int4_rows(const char* who, int64_t k_stride, int64_t v_stride, 
   return 0;
 }
 
+// Whether rows allow accesses of 16 bytes.
+static bool int4_wide(const void* k, const void* v, int64_t k_stride, int64_t v_stride, int head_dim, int dtype) {
+  const int64_t lane = dtype == PS_F32 ? 4 : 8;
+  return head_dim % 8 == 0 && k_stride % lane == 0 && v_stride % lane == 0 && ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
+}
+// Tokens of a block, as a power of two.
+static int int4_token_shift(int tokens) { return tokens >= 64 ? 4 : 0; }
+
+#define PS_OF_WIDTH(LAUNCH, T, G)  \
+  if (wide) LAUNCH(T, G, true);    \
+  else LAUNCH(T, G, false);        \
+  break
+#define PS_OF_GROUPS(LAUNCH, T)               \
+  switch (int4_groups(head_dim)) {            \
+    case 1: PS_OF_WIDTH(LAUNCH, T, 1);        \
+    case 2: PS_OF_WIDTH(LAUNCH, T, 2);        \
+    case 3: PS_OF_WIDTH(LAUNCH, T, 3);        \
+    case 4: PS_OF_WIDTH(LAUNCH, T, 4);        \
+    case 5: PS_OF_WIDTH(LAUNCH, T, 5);        \
+    case 6: PS_OF_WIDTH(LAUNCH, T, 6);        \
+    case 7: PS_OF_WIDTH(LAUNCH, T, 7);        \
+    default: PS_OF_WIDTH(LAUNCH, T, 8);       \
+  }
+
 extern "C" int ps_kv_write_int4(const void* k, const void* v, int64_t k_stride, int64_t v_stride, void* k_pool,
                                 void* v_pool, const int* tok_item, const int* tok_pos, const int* tables,
                                 int table_width, int tokens, int kv_heads, int head_dim, int page_size,
@@ -103,16 +288,21 @@ extern "C" int ps_kv_write_int4(const void* k, const void* v, int64_t k_stride, 
   if (check_int4_rows("ps_kv_write_int4", k_stride, v_stride, table_width, tokens, kv_heads, head_dim, page_size,
                       num_pages, dtype))
     return 1;
+  PS_REQUIRE(((uintptr_t)k_pool | (uintptr_t)v_pool) % 16 == 0, "%s: pools must begin at multiples of 16 bytes", "ps_kv_write_int4");
   if (tokens == 0) return 0;
-  const int groups = int4_groups(head_dim);
-  const dim3 grid(tokens, (kv_heads * groups + 15) / 16, 2);
+  const bool wide = int4_wide(k, v, k_stride, v_stride, head_dim, dtype);
+  const int shift = int4_token_shift(tokens), per_block = 16 >> shift;
+  const dim3 grid((tokens + (1 << shift) - 1) >> shift, (kv_heads + per_block - 1) / per_block, 2);
   hipStream_t s = (hipStream_t)stream;
-#define PS_LAUNCH_W4(T)                                                                                         \
-  hipLaunchKernelGGL(kv_write_int4_kernel<T>, grid, dim3(256), 0, s, (const T*)k, (const T*)v, k_stride, v_stride, \
-                     (uint8_t*)k_pool, (uint8_t*)v_pool, tok_item, tok_pos, tables, table_width, kv_heads, head_dim, \
-                     groups, page_size, num_pages)
-  if (dtype == PS_F32) PS_LAUNCH_W4(float);
-  else PS_LAUNCH_W4(bf16_t);
+#define PS_LAUNCH_W4(T, G, WIDE)                                                                                          \
+  hipLaunchKernelGGL((kv_write_int4_kernel<T, G, WIDE>), grid, dim3(64), 0, s, (const T*)k, (const T*)v, k_stride, v_stride, \
+                     (uint8_t*)k_pool, (uint8_t*)v_pool, tok_item, tok_pos, tables, table_width, tokens, kv_heads, \
+                     head_dim, page_size, num_pages, shift)
+  if (dtype == PS_F32) {
+    PS_OF_GROUPS(PS_LAUNCH_W4, float)
+  } else {
+    PS_OF_GROUPS(PS_LAUNCH_W4, bf16_t)
+  }
 #undef PS_LAUNCH_W4
   PS_CHECK_LAUNCH("ps_kv_write_int4");
   return 0;
@@ -125,16 +315,21 @@ extern "C" int ps_kv_read_int4(const void* k_pool, const void* v_pool, void* k, 
   if (check_int4_rows("ps_kv_read_int4", k_stride, v_stride, table_width, tokens, kv_heads, head_dim, page_size,
                       num_pages, dtype))
     return 1;
+  PS_REQUIRE(((uintptr_t)k_pool | (uintptr_t)v_pool) % 16 == 0, "%s: pools must begin at multiples of 16 bytes", "ps_kv_read_int4");
   if (tokens == 0) return 0;
-  const int groups = int4_groups(head_dim);
-  const dim3 grid(tokens, (kv_heads * groups + 15) / 16, 2);
+  const bool wide = int4_wide(k, v, k_stride, v_stride, head_dim, dtype);
+  const int shift = int4_token_shift(tokens), per_block = 16 >> shift;
+  const dim3 grid((tokens + (1 << shift) - 1) >> shift, (kv_heads + per_block - 1) / per_block, 2);
   hipStream_t s = (hipStream_t)stream;
-#define PS_LAUNCH_R4(T)                                                                                     \
-  hipLaunchKernelGGL(kv_read_int4_kernel<T>, grid, dim3(256), 0, s, (const uint8_t*)k_pool, (const uint8_t*)v_pool, \
-                     (T*)k, (T*)v, k_stride, v_stride, tok_item, tok_pos, tables, table_width, kv_heads, head_dim, \
-                     groups, page_size, num_pages)
-  if (dtype == PS_F32) PS_LAUNCH_R4(float);
-  else PS_LAUNCH_R4(bf16_t);
+#define PS_LAUNCH_R4(T, G, WIDE)                                                                                        \
+  hipLaunchKernelGGL((kv_read_int4_kernel<T, G, WIDE>), grid, dim3(64), 0, s, (const uint8_t*)k_pool, (const uint8_t*)v_pool, \
+                     (T*)k, (T*)v, k_stride, v_stride, tok_item, tok_pos, tables, table_width, tokens, kv_heads,   \
+                     head_dim, page_size, num_pages, shift)
+  if (dtype == PS_F32) {
+    PS_OF_GROUPS(PS_LAUNCH_R4, float)
+  } else {
+    PS_OF_GROUPS(PS_LAUNCH_R4, bf16_t)
+  }
 #undef PS_LAUNCH_R4
   PS_CHECK_LAUNCH("ps_kv_read_int4");
   return 0;

@@ -113,6 +113,30 @@ def test_values_between_codes():
     assert torch.equal(back[0].double().cpu(), values) and torch.equal(back[1].double().cpu(), values)
 
 
+@pytest.mark.parametrize("kind", [BF16, F32])
+def test_values_of_every_magnitude(kind):
+    """Numbers of 8 bits, whose quotients by a step of 5 often are half way between two codes, from the smallest steps
+    to the largest: the very codes of the definition."""
+    from pagedserve_amd.ops import kernels
+
+    g = torch.Generator().manual_seed(10)
+    rows = torch.randint(-255, 256, (256, 128), generator=g).double()
+    rows[::3] = torch.randint(-16, 17, (86, 128), generator=g).double() * 8 + 0.0
+    for t in range(256):
+        rows[t, 32 * (t % 4):32 * (t % 4) + 32] *= 0.125 ** (t % 3)
+        rows[t] *= 2.0 ** (t - 136)                          # (the steps' exponents: -126 and below to 124)
+    rows = rows.to(torch.float32).to(kind)
+    tables, pages, items, positions = _requests((256,), (0,), 16, 11)
+    pools = [torch.zeros(pages, 2, 16, 36, dtype=torch.uint8).cuda() for _ in range(2)]
+    index = (_ints(items), _ints(positions), tables.cuda())
+    kernels.kv_write_int4(rows.cuda(), rows.cuda(), *pools, *index)
+    back = [torch.zeros(256, 128).cuda() for _ in range(2)]
+    kernels.kv_read_int4(*pools, *back, *index)
+    _, _, values = plain.held(rows, 2)
+    for got in back:
+        torch.testing.assert_close(got.double().cpu(), values, rtol=0, atol=0, equal_nan=True)
+
+
 def test_values_that_are_no_numbers():
     """A group with a NaN or an infinity in it is NaN, its neighbours are not; tiny groups are zeros; tokens without a page
     are neither stored nor read."""
