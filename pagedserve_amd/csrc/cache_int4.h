@@ -7,7 +7,7 @@
 // rounded to five significant bits, ties to even: e itself is code 0 up to that rounding, all sixteen codes are
 // used, and (code - 8) d, three bits times five, is a bfloat16 number without rounding, so that
 // attention over this cache is attention over a bfloat16 cache which holds these values.  (Root mean
-// square error of normal values 8.62 % of theirs, 8.60 % with the step unrounded; codes -7 .. 7 of the magnitude 9.7 %.)  A step
+// square error of normal values 8.62 % of theirs, 8.60 % with the step unrounded; codes -7 .. 7 of the magnitude 9.7 %.)  A step that is still
 // below the normal floats becomes 0, and the group zeros; a group that holds an infinity or a NaN
 // gets a NaN for its step and is NaN as a whole, as a cache in the model's type would show it.
 //
@@ -38,12 +38,14 @@ __device__ inline int int4_value_byte(int b, int groups) { return (b & 15) * gro
 
 // The step of a group from its largest and its smallest element.
 __device__ inline float int4_step(float high, float low) {
-  const float step = (high >= -low ? high : low) * -0.125f;
-  const uint32_t bits = __float_as_uint(step);
+  const float e = high >= -low ? high : low;
+  const uint32_t bits = __float_as_uint(e * -0.125f);
   uint32_t size = bits & 0x7fffffffu;
   size = (size + 0x3ffffu + ((size >> 19) & 1u)) & ~0x7ffffu;       // five significant bits, ties to even
   if (size > 0x7df80000u) size = 0x7df80000u;                       // 31/16 2^124, eight times which is a finite float
-  return fabsf(step) < 1.17549435e-38f ? 0.f : __uint_as_float(size | (bits & 0x80000000u));
+  if (size < 0x00800000u) size = 0x00800000u;
+  // (from 2^-123 (1 - 2^-6) on, five bits make an eighth of it the smallest normal float)
+  return fabsf(e) < __uint_as_float(0x01fc0000u) ? 0.f : __uint_as_float(size | (bits & 0x80000000u));
 }
 
 // The codes of eight numbers, less 8, under a step other than 0; BF16: numbers of 8 significant bits.
