@@ -227,7 +227,7 @@ __device__ __forceinline__ void attention_prefill_block(
   constexpr int GROUPS = (HD + PS_INT4_GROUP - 1) / PS_INT4_GROUP;
   constexpr int THREADS = 64 * AP_WAVES, ROW_ITEMS = 4 * AP_KEYS, ITEMS = 2 * ROW_ITEMS / THREADS;
   constexpr int STEP_WORDS = (GROUPS + 1) / 2;
-  static_assert(!Pages::INT4 || (ITEMS >= 1 && 2 * ROW_ITEMS % THREADS == 0 && ROW_ITEMS % 64 == 0), "whole waves of one kind");
+  static_assert(!Pages::INT4 || ROW_ITEMS % THREADS == 0, "an item of every thread is of one kind");
   uint32_t codes[Pages::INT4 ? ITEMS : 1][GROUPS], steps[Pages::INT4 ? ITEMS : 1][STEP_WORDS],
       value_steps[Pages::INT4 ? ITEMS : 1][STEP_WORDS];
   // Which key an item is of: of every 16 in an order that spreads the stores of 16 lanes over the banks, whose rows are
@@ -265,7 +265,7 @@ __device__ __forceinline__ void attention_prefill_block(
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j) {
         const int item = j * THREADS + tid;
-        const bool is_value = j * THREADS + wave * 64 >= ROW_ITEMS;      // (the same in a wave)
+        const bool is_value = j * THREADS >= ROW_ITEMS;
         const int key_local = key_of(item), c = item & 3;
         uint32_t page_row;
         int within;
@@ -317,7 +317,7 @@ __device__ __forceinline__ void attention_prefill_block(
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j) {
         const int item = j * THREADS + tid;
-        const bool is_value = j * THREADS + wave * 64 >= ROW_ITEMS;
+        const bool is_value = j * THREADS >= ROW_ITEMS;
         const int key_local = key_of(item), c = item & 3;
         const int turn = (key_local / SPREAD) % CH;
         unsigned char* row = stage + (is_value ? TILE_BYTES : 0) + key_local * ROW;
