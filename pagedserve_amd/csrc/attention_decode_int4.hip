@@ -180,7 +180,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
 
   const int first = pos < 0 ? 0 : first_visible_key(pos, a.window);
   const int64_t room = (int64_t)a.table_width * a.page_size;
-  const int end_key = pos + 1 < room ? pos + 1 : (int)room;
+  const int end_key = pos < 0 ? 0 : pos < room ? pos + 1 : (int)room;
   int begin = first & ~(I4_TILE - 1), end = end_key;
   if (a.splits > 1) {
     int chunk = (end - begin + a.splits - 1) / a.splits;
@@ -559,8 +559,7 @@ __global__ __launch_bounds__(256) void attention_decode_int4_kernel(
 
   // (a token in front of its context sees nothing, and reads no entry of the table)
   const int first = pos < 0 ? 0 : first_visible_key(pos, window);
-  int end = pos + 1;
-  if (end > (int64_t)table_width * page_size) end = table_width * page_size;
+  int end = pos < 0 ? 0 : pos < (int64_t)table_width * page_size ? pos + 1 : table_width * page_size;
   int begin = first;
   if (splits > 1) {
     const int chunk = ((end - first + splits - 1) / splits + TURN - 1) / TURN * TURN;

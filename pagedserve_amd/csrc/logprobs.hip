@@ -385,7 +385,7 @@ __global__ __launch_bounds__(512) void logprobs_join_kernel(const T* __restrict_
 // one, with 5 alternatives 10.7 and 14.6 us, without 5.8 and 11.3; 64 rows in 4 parts 13.2 and 16.3; 256 rows in 2
 // parts 22.4 and 20.7.)
 static int lp_parts(int rows, int vocab) {
-  const int least = (vocab + LP_PART - 1) / LP_PART;
+  const int least = (vocab - 1) / LP_PART + 1;
   int wanted = ps_compute_units() / (rows > 0 ? rows : 1);
   if (wanted > vocab / 4096 + 1) wanted = vocab / 4096 + 1;
   if (wanted > 16) wanted = 16;

@@ -1535,6 +1535,8 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
     ranges = prefill_int4_ranges(tiles, heads, max_kv_len) if ranges is None else int(ranges)
     partial_at = floats = 0
     if ranges > 1:
+        if query_tile not in (PREFILL_TILE, PREFILL_LARGE_TILE):
+            raise KernelError(f"attention_prefill_int4: tiles of {PREFILL_TILE} or {PREFILL_LARGE_TILE} queries, not {query_tile}")
         if partial is None:
             partial = torch.empty(tiles * heads * ranges * query_tile * (head_dim + 2), dtype=torch.float32, device=q.device)
         partial_at, floats = _dense(partial, "partial", torch.float32, None, device), partial.numel()

@@ -143,7 +143,7 @@ def test_decode_refused(on_gpu, changed, message):
     ({"tile_q0": _ints(2)}, "inconsistent"), ({"cu_tokens": _ints(3)}, "inconsistent"), ({"tables": _ints(2, 5)}, "inconsistent"),
     ({"kv_lens": _ints(2)[::2]}, None), ({"kv_lens": _ints(4)[::2], "cu_tokens": _ints(3), "tables": _ints(2, 5)}, "contiguous"),
     ({"tile_item": _ints(1).long()}, "int32"), ({"sink": torch.zeros(5)}, "one float per head"),
-    ({"ranges": 2, "partial": torch.zeros(9, dtype=BF16)}, "partial"), ({"ranges": 2, "partial": torch.zeros(9, 2)[:, 0]}, "contiguous")])
+    ({"ranges": 2, "query_tile": -64}, "queries"), ({"ranges": 2, "partial": torch.zeros(9, dtype=BF16)}, "partial"), ({"ranges": 2, "partial": torch.zeros(9, 2)[:, 0]}, "contiguous")])
 def test_prompt_refused(on_gpu, changed, message):
     if message is None:
         kernels.attention_prefill_int4(**_prompt(**changed))

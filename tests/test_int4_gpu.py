@@ -114,6 +114,24 @@ def test_values_between_codes():
 
 
 @pytest.mark.parametrize("kind", [BF16, F32])
+@pytest.mark.parametrize("splits", [1, 64])
+def test_positions_outside_the_table(kind, splits):
+    """Positions far in front of the context are in front of it; one behind the table sees all that the table has."""
+    from pagedserve_amd.ops import kernels
+
+    tables, pages, _, _ = _requests((1, 1, 1), (49, 49, 49), 16, 12)
+    tables = tables[:, :4].contiguous()
+    pools, kept = _cache(tables, pages, (64, 64, 64), 2, 64, 16, 13)
+    q = torch.randn((3, 128), generator=torch.Generator().manual_seed(14)).to(kind)
+    out = torch.full((3, 128), 5.0, dtype=kind).cuda()
+    kernels.attention_decode_int4(q.cuda(), *pools, out, None, _ints([-(1 << 31), (1 << 31) - 1, -64]), tables.cuda(), 2,
+                                  0.125, splits, torch.zeros(3 * 2 * splits * 66).cuda())
+    assert bool((out[0] == 0).all()) and bool((out[2] == 0).all())
+    expected = list(plain.attention(q[1:2], *kept[1], [63], 2, 0.125))
+    assert bool(((out[1:2].double().cpu() - expected[0]).abs() <= plain.allowed(*expected, kind, kind == BF16)).all())
+
+
+@pytest.mark.parametrize("kind", [BF16, F32])
 def test_values_of_every_magnitude(kind):
     """Numbers of 8 bits, whose quotients by a step of 5 often are half way between two codes, from the smallest steps
     to the largest: the very codes of the definition."""
