@@ -57,13 +57,14 @@ struct PrefillRange {
   float* states;
 };
 
-// The work of one block: one head of one tile of queries.  The caller provides the block's LDS
+// The work of one block: one head (HP: two neighbouring heads of one key/value head, half of the waves along the queries
+// each) of one tile of queries.  The caller provides the block's LDS
 // (the kernel below its own; a kernel that runs blocks of several kinds in one launch a share
 // of what all of them need).
 // head_dim / 16; waves along the keys; waves along the queries; runs of 32 keys per wave and tile
-template <int NDB, int KS, int QW = 2, int KR = 1, typename Pages = Bf16Pages>
+template <int NDB, int KS, int QW = 2, int KR = 1, typename Pages = Bf16Pages, int HP = 1>
 __device__ __forceinline__ void attention_prefill_block(
-    PrefillLds<NDB, KS, QW, KR>& lds, const int head, const int tile_index,
+    PrefillLds<NDB, KS, QW, KR>& lds, const int block_head, const int tile_index,
     const bf16_t* __restrict__ q, int64_t q_stride, const typename Pages::Element* __restrict__ k_pool,
     const typename Pages::Element* __restrict__ v_pool, bf16_t* __restrict__ out, int64_t out_stride,
     const int* __restrict__ tile_item, const int* __restrict__ tile_q0,
@@ -78,7 +79,8 @@ __device__ __forceinline__ void attention_prefill_block(
   constexpr int WAVE_KEYS = 32 * KR;             // keys of a wave per tile
   constexpr int AP_KEYS = WAVE_KEYS * KS;        // keys per tile
   constexpr int AP_WAVES = QW * KS;
-  constexpr int QUERIES = 32 * QW;               // queries per block
+  constexpr int QUERIES = 32 * QW / HP;          // queries per block
+  static_assert(QW % HP == 0, "whole waves to a head");
   static_assert(QW == 1 || QW == 2 || QW == 4, "one, two or four waves along the queries");
   static_assert(KR == 1 || KR == 2, "one or two runs of keys per wave");
   constexpr int TILE_BYTES = AP_KEYS * ROW;
@@ -112,11 +114,13 @@ __device__ __forceinline__ void attention_prefill_block(
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // the same in every lane: scalar
-  const int wave_q = wave % QW;  // which 32 queries
+  const int wave_row = wave % QW;
+  const int wave_q = wave_row % (QW / HP);  // which 32 queries
+  const int head = block_head * HP + wave_row / (QW / HP);
   const int wave_k = wave / QW;  // which run of 32 keys of every tile
   const int sub = lane & 31;     // query of this lane within the wave; key or dimension row
   const int half = lane >> 5;    // which half of a step's reduction dimension
-  const int kv_head = head / (heads / kv_heads);
+  const int kv_head = block_head * HP / (heads / kv_heads);
 
   // blocks start in the order of their numbers, heads fastest: the caller lists the tiles that
   // see the most keys first, so the longest blocks start first and the shortest fill the gaps
@@ -227,7 +231,12 @@ __device__ __forceinline__ void attention_prefill_block(
   constexpr int GROUPS = (HD + PS_INT4_GROUP - 1) / PS_INT4_GROUP;
   constexpr int THREADS = 64 * AP_WAVES, ROW_ITEMS = 4 * AP_KEYS, ITEMS = 2 * ROW_ITEMS / THREADS;
   constexpr int STEP_WORDS = (GROUPS + 1) / 2;
-  static_assert(!Pages::INT4 || ROW_ITEMS % THREADS == 0, "an item of every thread is of one kind");
+  static_assert(!Pages::INT4 || (2 * ROW_ITEMS % THREADS == 0 && ROW_ITEMS % 64 == 0), "whole waves of one kind");
+  // (known at compile time where a turn of all threads is of one kind: no branch)
+  auto of_values = [&](int j) {
+    if constexpr (ROW_ITEMS % THREADS == 0) return j * THREADS >= ROW_ITEMS;
+    else return j * THREADS + wave * 64 >= ROW_ITEMS;
+  };
   uint32_t codes[Pages::INT4 ? ITEMS : 1][GROUPS], steps[Pages::INT4 ? ITEMS : 1][STEP_WORDS],
       value_steps[Pages::INT4 ? ITEMS : 1][STEP_WORDS];
   // Which key an item is of: of every 16 in an order that spreads the stores of 16 lanes over the banks, whose rows are
@@ -265,7 +274,7 @@ __device__ __forceinline__ void attention_prefill_block(
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j) {
         const int item = j * THREADS + tid;
-        const bool is_value = j * THREADS >= ROW_ITEMS;
+        const bool is_value = of_values(j);
         const int key_local = key_of(item), c = item & 3;
         uint32_t page_row;
         int within;
@@ -317,7 +326,7 @@ __device__ __forceinline__ void attention_prefill_block(
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j) {
         const int item = j * THREADS + tid;
-        const bool is_value = j * THREADS >= ROW_ITEMS;
+        const bool is_value = of_values(j);
         const int key_local = key_of(item), c = item & 3;
         const int turn = (key_local / SPREAD) % CH;
         unsigned char* row = stage + (is_value ? TILE_BYTES : 0) + key_local * ROW;
@@ -654,7 +663,7 @@ __device__ __forceinline__ void attention_prefill_block(
     ap_wait_loads_and_sync<0>();               // every wave is past its last operand reads
     float* states = reinterpret_cast<float*>(stages);
     if (wave_k > 0) {
-      float* mine = states + ((wave_k - 1) * QW + wave_q) * 64 * STATE + lane;
+      float* mine = states + ((wave_k - 1) * QW + wave_row) * 64 * STATE + lane;
       mine[0] = m;
       mine[64] = l;
 #pragma unroll
@@ -666,7 +675,7 @@ __device__ __forceinline__ void attention_prefill_block(
     if (wave_k > 0) return;
 #pragma unroll 1
     for (int other = 1; other < KS; ++other) {
-      const float* theirs = states + ((other - 1) * QW + wave_q) * 64 * STATE + lane;
+      const float* theirs = states + ((other - 1) * QW + wave_row) * 64 * STATE + lane;
       const float m_o = theirs[0];
       const float l_o = theirs[64];
       const float m_n = fmaxf(m, m_o);

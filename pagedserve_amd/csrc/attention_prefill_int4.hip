@@ -4,12 +4,20 @@
 // values one tile ahead, exactly (cache_int4.h says why that is no rounding); what follows is the same code, so that this
 // attention is that one over a cache of these values.
 //
-// Bound: the vector instructions of the conversion (3.6 to a value: four bits to a float, one product, half a packing;
-// every block converts what it reads) come on top of those of the softmax, which bound the other cache's kernel.  2 x
-// 4,096 tokens of 12 heads of 64: 108 us, 478 TFLOP/s (the other cache 87); 16 heads of 128 behind 5,000 keys, 962
-// tokens: 116 to 122 us, 340 TFLOP/s (the other cache 94).  Where the tiles are fewer than the compute units, keys are cut into
-// ranges, whose records a second launch joins: 512 tokens of 12 heads behind 3,500 keys 29.5 us (the other cache, without
-// ranges, 41), 64 of 8 heads of 128 behind 8,000 24.4 (121).
+// Bound: the vector instructions of the conversion (3.5 to a value: four bits to a float, one product, half a packing;
+// every block converts what it reads) come on top of those of the softmax, which bound the other cache's kernel.  So a
+// block multiplies what it has converted with as many queries as its registers allow: 128 rows, of one head, or of two
+// that share a key/value head, where the blocks fill the units.  2 x 4,096 tokens of 12 heads of 64: 110 us, 470 TFLOP/s
+// (the other cache 87); 4,096 of 16 heads of 128 142 us, 484 TFLOP/s (64 rows: 181); 16 heads of 128 behind 5,000 keys,
+// 962 tokens, 99 us, 410 TFLOP/s, by pairs of heads and 112 by one (the other cache 94).
+//
+// Where the blocks are fewer than the compute units, keys are cut into ranges, whose records a second launch joins: 512
+// tokens of 12 heads behind 3,500 keys 29 us (the other cache, without ranges, 41), 64 of 8 heads of 128 behind 8,000
+// 24.4 (121).
+//
+// Blocks of 64 rows: 8 waves, four along the keys, for heads of up to 128 (16 heads of 128: 4,096 tokens 180 us, of four
+// waves, two along the keys, 258), but many blocks of smaller heads, whose four waves fit a unit more often (2 x 4,096 tokens of 12
+// heads of 64 130 us), and heads beyond 128, whose accumulators take the registers of eight.
 #include <math.h>
 
 #include "common.h"
@@ -17,7 +25,7 @@
 
 #include "attention_prefill_block.h"
 
-template <int NDB, int KS, int QW, int KR>
+template <int NDB, int KS, int QW, int KR, int HP>
 __global__ __launch_bounds__(64 * QW * KS) void attention_prefill_int4_kernel(
     const bf16_t* __restrict__ q, int64_t q_stride, const uint8_t* __restrict__ k_pool,
     const uint8_t* __restrict__ v_pool, bf16_t* __restrict__ out, int64_t out_stride,
@@ -27,7 +35,7 @@ __global__ __launch_bounds__(64 * QW * KS) void attention_prefill_int4_kernel(
     int page_shift, int num_pages, float scale, int window, const AttnExtras extra, int ranges, float* sums,
     float* states) {
   __shared__ PrefillLds<NDB, KS, QW, KR> lds;
-  attention_prefill_block<NDB, KS, QW, KR, Int4Pages>(lds, blockIdx.x, blockIdx.y, q, q_stride, k_pool, v_pool, out,
+  attention_prefill_block<NDB, KS, QW, KR, Int4Pages, HP>(lds, blockIdx.x, blockIdx.y, q, q_stride, k_pool, v_pool, out,
                                                      out_stride, tile_item, tile_q0, cu_tokens, kv_lens, tables,
                                                      table_width, heads, kv_heads, page_size, page_shift,
                                                      num_pages, scale, window, extra,
@@ -72,8 +80,8 @@ extern "C" int ps_attention_prefill_int4(const void* q, int64_t q_stride, const 
                                          int tiles, const int* cu_tokens, const int* kv_lens, const int* tables,
                                          int table_width, int heads, int kv_heads, int head_dim,
                                          int page_size, int num_pages, float scale, int window, int max_kv_len,
-                                         int query_tile, const float* sink, float softcap, int ranges,
-                                         float* partial, int64_t partial_floats, void* stream) {
+                                         int query_tile, const float* sink, float softcap, int block_heads,
+                                         int ranges, float* partial, int64_t partial_floats, void* stream) {
   const char* who = "ps_attention_prefill_int4";
   PS_REQUIRE(tiles >= 0 && heads > 0 && kv_heads > 0 && page_size > 0 && num_pages > 0 && table_width > 0,
              "%s: bad sizes", who);
@@ -83,9 +91,12 @@ extern "C" int ps_attention_prefill_int4(const void* q, int64_t q_stride, const 
   PS_REQUIRE(page_size % 8 == 0 && page_size <= (1 << 20),
              "%s: pages of a cache in 4 bits hold a multiple of 8 keys, not %d", who, page_size);
   PS_REQUIRE(tiles <= 65535, "%s: too many tiles (%d)", who, tiles);
-  PS_REQUIRE(query_tile == AP_QUERIES || (query_tile == AP_QUERIES * 2 && head_dim <= AP_LARGE_HEAD_DIM),
-             "%s: tiles of %d or, head sizes up to %d, %d queries, not %d", who, AP_QUERIES, AP_LARGE_HEAD_DIM,
-             AP_QUERIES * 2, query_tile);
+  PS_REQUIRE(query_tile == AP_QUERIES || (query_tile == AP_QUERIES * 2 && head_dim <= 128),
+             "%s: tiles of %d or, head sizes up to 128, %d queries, not %d", who, AP_QUERIES, AP_QUERIES * 2, query_tile);
+  PS_REQUIRE(block_heads == 1 || (block_heads == 2 && heads / kv_heads % 2 == 0 && query_tile == AP_QUERIES &&
+                                  head_dim > 64 && head_dim <= 128),
+             "%s: %d heads to a block (two of one key/value head, head sizes from 65 to 128, tiles of %d queries)", who,
+             block_heads, AP_QUERIES);
   PS_REQUIRE((int64_t)num_pages * kv_heads * page_size < ((int64_t)1 << 32),
              "%s: a pool of %d pages x %d heads x %d keys has 2^32 key rows or more", who, num_pages, kv_heads, page_size);
   PS_REQUIRE(scale > 0.f, "%s: the score scale must be positive, got %g", who, scale);
@@ -107,24 +118,28 @@ extern "C" int ps_attention_prefill_int4(const void* q, int64_t q_stride, const 
   }
   hipStream_t s = (hipStream_t)stream;
   const AttnExtras extra = {sink, nullptr, 0, softcap, nullptr, 1.f};
-  dim3 grid(heads, tiles, ranges);
+  const dim3 grid(heads / block_heads, tiles, ranges);
   float* states = ranges > 1 ? partial + records * head_dim : nullptr;
-  // four waves along the keys where few blocks see many keys, as for the other cache
+  // head sizes up to 64: four waves along the keys where few blocks see many keys, as for the other cache
   const bool wide = (int64_t)tiles * heads * ranges <= ps_compute_units() * 2 && (max_kv_len <= 0 || max_kv_len >= 512);
-#define PS_LAUNCH_P4(NDB, KS, QW, KR)                                                                            \
-  hipLaunchKernelGGL((attention_prefill_int4_kernel<NDB, KS, QW, KR>), grid, dim3(64 * KS * QW), 0, s, (const bf16_t*)q, \
+#define PS_LAUNCH_P4(NDB, KS, QW, KR, HP)                                                                            \
+  hipLaunchKernelGGL((attention_prefill_int4_kernel<NDB, KS, QW, KR, HP>), grid, dim3(64 * KS * QW), 0, s, (const bf16_t*)q, \
                      q_stride, (const uint8_t*)k_pool, (const uint8_t*)v_pool, (bf16_t*)out, out_stride,        \
                      tile_item, tile_q0, cu_tokens, kv_lens, tables, table_width, heads, kv_heads, page_size,   \
                      page_shift, num_pages, scale, window, extra, ranges, partial, states)
-#define PS_TILES_P4(NDB)                                      \
-  case NDB:                                                   \
-    if (query_tile == AP_QUERIES * 2) {                       \
-      if constexpr (NDB <= 4) PS_LAUNCH_P4(NDB, 1, 4, 2);        \
-    } else if (NDB <= 8 && wide) {                            \
-      if constexpr (NDB <= 8) PS_LAUNCH_P4(NDB, 4, 2, 1);        \
-    } else {                                                  \
-      PS_LAUNCH_P4(NDB, 2, 2, 1);                                \
-    }                                                         \
+#define PS_TILES_P4(NDB)                                                   \
+  case NDB:                                                                \
+    if constexpr (NDB <= 4) {                                              \
+      if (query_tile == AP_QUERIES * 2) PS_LAUNCH_P4(NDB, 1, 4, 2, 1);     \
+      else if (wide) PS_LAUNCH_P4(NDB, 4, 2, 1, 1);                        \
+      else PS_LAUNCH_P4(NDB, 2, 2, 1, 1);                                  \
+    } else if constexpr (NDB <= 8) {                                       \
+      if (query_tile == AP_QUERIES * 2) PS_LAUNCH_P4(NDB, 2, 4, 1, 1);     \
+      else if (block_heads == 2) PS_LAUNCH_P4(NDB, 2, 4, 1, 2);            \
+      else PS_LAUNCH_P4(NDB, 4, 2, 1, 1);                                  \
+    } else {                                                               \
+      PS_LAUNCH_P4(NDB, 2, 2, 1, 1);                                       \
+    }                                                                      \
     break
   switch (head_dim / 16) {
     PS_TILES_P4(1);
@@ -142,7 +157,7 @@ extern "C" int ps_attention_prefill_int4(const void* q, int64_t q_stride, const 
     PS_TILES_P4(13);
     PS_TILES_P4(14);
     PS_TILES_P4(15);
-    default: PS_LAUNCH_P4(16, 2, 2, 1);
+    default: PS_LAUNCH_P4(16, 2, 2, 1, 1);
   }
 #undef PS_TILES_P4
 #undef PS_LAUNCH_P4

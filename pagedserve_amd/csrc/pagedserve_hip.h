@@ -308,7 +308,7 @@ int ps_attention_decode_int4(const void* q, int64_t q_stride, const void* k_pool
                              const int* tables, int table_width, int count, int heads, int kv_heads,
                              int head_dim, int page_size, int num_pages, float scale, int window,
                              int splits, const float* sink, float softcap, int dtype, void* stream);
-// ps_attention_prefill over such a cache (bfloat16 q and out), the keys of every tile cut into `ranges` where units would
+// ps_attention_prefill over such a cache (bfloat16 q and out), block_heads (1 or 2) heads of a key/value head to a block, the keys of every tile cut into `ranges` where units would
 // stay idle over long contexts.  With more than one, partial (from a multiple of 16 bytes on) is scratch of
 // tiles x heads x ranges x query_tile x (head_dim + 2) floats.
 int ps_attention_prefill_int4(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool,
@@ -316,8 +316,8 @@ int ps_attention_prefill_int4(const void* q, int64_t q_stride, const void* k_poo
                               int tiles, const int* cu_tokens, const int* kv_lens, const int* tables,
                               int table_width, int heads, int kv_heads, int head_dim, int page_size,
                               int num_pages, float scale, int window, int max_kv_len, int query_tile,
-                              const float* sink, float softcap, int ranges, float* partial, int64_t partial_floats,
-                              void* stream);
+                              const float* sink, float softcap, int block_heads, int ranges, float* partial,
+                              int64_t partial_floats, void* stream);
 
 // logprobs[r] = log softmax(logits[r])[tokens[r]] of rows `ld` apart, of `dtype`.  entropy, ranks, top_ids, top_logprobs: null, or what
 // is wanted of them (the two last [rows, top], top up to 32).  A token of -1: none (0, rank -1); others outside the vocabulary: NaN, -1.

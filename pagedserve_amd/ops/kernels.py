@@ -156,7 +156,7 @@ _SIGNATURES = {
                                  c_float, c_int, c_int, c_void_p, c_float, c_int, c_void_p],
     "ps_attention_prefill_int4": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int,
                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
-                                  c_int, c_int, c_int, c_void_p, c_float, c_int, c_void_p, c_int64, c_void_p],
+                                  c_int, c_int, c_int, c_void_p, c_float, c_int, c_int, c_void_p, c_int64, c_void_p],
     "ps_token_logprobs": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                           c_int, c_void_p, c_int64, c_int, c_void_p],
     "ps_sample": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
@@ -1484,35 +1484,51 @@ def prefill_int4_supported(dtype, head_dim, table_width=0) -> bool:
 def prefill_int4_tile(heads, head_dim, tiles, max_kv_len=0) -> int:
     """Queries per tile for ``attention_prefill_int4``, 64 or 128: ``tiles`` maps each size to the number of tiles that a
     step's portions make of it.  Larger tiles turn fewer codes into values; where a size leaves units idle the ranges of
-    the keys fill them, so that tiles of 32 queries do not pay.  Tiles of 128 are taken where those of the other cache
-    are, and where their ranges fill more units (512 tokens of 12 heads of 64 behind 3,500: 240 blocks and 29.5 us against
-    192 and 34.0; 256 behind 1,800: 192 and 16.4 against 240 and 15.3; even, as 1,024 of 16 heads behind 3,000: 57.5
-    against 56.4)."""
+    the keys fill them, so that tiles of 32 queries do not pay.  Tiles of 128 are taken
+
+    * for heads of up to 64 dimensions where those of the other cache are, and where their ranges fill more units (512
+      tokens of 12 heads behind 3,500: 240 blocks and 29.5 us against 192 and 34.0; 256 behind 1,800: 192 and 16.4
+      against 240 and 15.3; even, as 1,024 of 16 heads behind 3,000: 57.5 against 56.4),
+    * for heads of up to 128 from two blocks per unit on (4,096 tokens of 16 heads of 128, 512 blocks: 142 against 179 us;
+      2 x 1,024, 256 blocks: 38.5 against 37.5)."""
     large = tiles[PREFILL_LARGE_TILE]
-    if head_dim <= PREFILL_LARGE_TILE_HEAD_DIM and large and (
-            prefill_large_tile_pays(heads, head_dim, large, max_kv_len) or
-            large * prefill_int4_ranges(large, heads, max_kv_len)
-            > tiles[PREFILL_TILE] * prefill_int4_ranges(tiles[PREFILL_TILE], heads, max_kv_len)):
-        return PREFILL_LARGE_TILE
-    return PREFILL_TILE
+    if head_dim > 128 or not large:
+        return PREFILL_TILE
+    if head_dim > PREFILL_LARGE_TILE_HEAD_DIM:
+        pays = large * heads >= 2 * compute_units()
+    else:
+        small = tiles[PREFILL_TILE]
+        pays = (prefill_large_tile_pays(heads, head_dim, large, max_kv_len)
+                or large * prefill_int4_ranges(large, heads, max_kv_len) > small * prefill_int4_ranges(small, heads, max_kv_len))
+    return PREFILL_LARGE_TILE if pays else PREFILL_TILE
+
+
+def prefill_int4_block_heads(tiles, heads, kv_heads, head_dim, query_tile) -> int:
+    """Heads of a key/value head that a block of ``attention_prefill_int4`` takes, 1 or 2: two share the values that the
+    codes become.  Pays for heads of 65 to 128 dimensions where the pairs still make half a block per unit (16 heads of
+    128 that share 4: 962 tokens behind 5,000, 128 blocks, 101 against 112 us; 20 portions of 60 behind 300, 160 blocks,
+    21.2 against 30.8; but 512 tokens, 64 blocks, 22.4 against 17.3).  With smaller heads it is level."""
+    pairs = tiles * heads // 2
+    return 2 if (query_tile == PREFILL_TILE and 64 < head_dim <= 128 and heads // kv_heads % 2 == 0
+                 and 2 * pairs >= compute_units()) else 1
 
 
 def prefill_int4_ranges(tiles, heads, max_kv_len) -> int:
-    """Ranges that ``attention_prefill_int4`` cuts the keys of every tile into: as many as leave a block to each compute
-    unit, 16 at most, each of 128 keys or more (100 tokens of 12 heads behind 2,000 keys: 35 us in one range, 13.2 in
-    ten; 64 of 8 heads of 128 behind 8,000: 31.8 in eight, 24.4 in sixteen; ranges of 256 keys or more: 2 to 10 % slower
-    at 16 to 128 tokens; more blocks than units lose: 16 heads of 128 behind 5,000, 256 blocks, 123 us in one range and
-    140 in two)."""
+    """Ranges that ``attention_prefill_int4`` cuts the keys of every tile into (``heads``: blocks per tile): as many as
+    leave a block to each compute unit, 16 at most, each of 128 keys or more (100 tokens of 12 heads behind 2,000 keys: 35
+    us in one range, 13.2 in ten; 64 of 8 heads of 128 behind 8,000: 31.8 in eight, 24.4 in sixteen; ranges of 256 keys or
+    more: 2 to 10 % slower at 16 to 128 tokens; more blocks than units lose: 16 heads of 128 behind 5,000, 256 blocks,
+    124 us in one range and 129 in two)."""
     if max_kv_len < 256:
         return 1
     return max(1, min(compute_units() // max(1, tiles * heads), max_kv_len // 128, 16))
 
 
 def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_lens, tables, heads, scale,
-                           window=0, max_kv_len=0, query_tile=PREFILL_TILE, sink=None, softcap=0.0, ranges=None, partial=None):
+                           window=0, max_kv_len=0, query_tile=PREFILL_TILE, sink=None, softcap=0.0, block_heads=None, ranges=None, partial=None):
     """``attention_prefill`` over a cache in 4 bits (bfloat16 queries, head sizes in multiples of 16).
-    ``ranges``: parts of the keys of every tile, joined by a second launch (None: ``prefill_int4_ranges(...)``, one where
-    ``max_kv_len`` is not given); with more than one ``partial`` is float scratch of
+    ``block_heads``: 1 or 2 heads to a block (None: ``prefill_int4_block_heads(...)``).  ``ranges``: parts of the keys of
+    every tile, joined by a second launch (None: ``prefill_int4_ranges(...)``, one where ``max_kv_len`` is not given); with more than one ``partial`` is float scratch of
     ``tiles * heads * ranges * query_tile * (head_dim + 2)`` values, allocated for the call where it is None."""
     _check_prefill_constants()
     _, device = _first("attention_prefill_int4", q, "q")
@@ -1532,7 +1548,10 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
         sink_at = _check_sink(sink, heads)
         _dense(sink, "sink", torch.float32, 1, device)
     max_kv_len, query_tile = int(max_kv_len), int(query_tile)
-    ranges = prefill_int4_ranges(tiles, heads, max_kv_len) if ranges is None else int(ranges)
+    if block_heads is None:
+        block_heads = prefill_int4_block_heads(tiles, heads, kv_heads, head_dim, query_tile)
+    if ranges is None:
+        ranges = prefill_int4_ranges(tiles, heads // block_heads, max_kv_len)
     partial_at = floats = 0
     if ranges > 1:
         if query_tile not in (PREFILL_TILE, PREFILL_LARGE_TILE):
@@ -1542,7 +1561,8 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
         partial_at, floats = _dense(partial, "partial", torch.float32, None, device), partial.numel()
     _call("ps_attention_prefill_int4", q_at, q_stride, k_at, v_at, out_at, out_stride, index[0], index[1], tiles, index[2],
           index[3], tables_at, tables.size(1), heads, kv_heads, head_dim, page_size, pages, float(scale),
-          int(window), max_kv_len, query_tile, sink_at, _check_cap(softcap), ranges, partial_at, floats, _stream())
+          int(window), max_kv_len, query_tile, sink_at, _check_cap(softcap), int(block_heads), int(ranges),
+          partial_at, floats, _stream())
     return out
 
 

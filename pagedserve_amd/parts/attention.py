@@ -403,11 +403,12 @@ class Attention(Mixer):
                                              {size: lists[0].numel() for size, lists in ctx.query_tiles.items()},
                                              ctx.max_kv_len)
             tiles = ctx.query_tiles[size]
-            ranges = kernels.prefill_int4_ranges(tiles[0].numel(), self.heads, self._visible(ctx.max_kv_len))
+            pair = kernels.prefill_int4_block_heads(tiles[0].numel(), self.heads, self.kv_heads, self.head_dim, size)
+            ranges = kernels.prefill_int4_ranges(tiles[0].numel(), self.heads // pair, self._visible(ctx.max_kv_len))
             kernels.attention_prefill_int4(q, cache.k_pool, cache.v_pool, context, *tiles, ctx.cu_tokens, ctx.kv_lens, tables,
                                            self.heads, self.scale, window=self.span, max_kv_len=ctx.max_kv_len,
-                                           query_tile=size, sink=self.sink, softcap=self.score_cap, ranges=ranges,
-                                           partial=self._int4_tile_records(ctx) if ranges > 1 else None)
+                                           query_tile=size, sink=self.sink, softcap=self.score_cap, block_heads=pair,
+                                           ranges=ranges, partial=self._int4_tile_records(ctx) if ranges > 1 else None)
         elif singles < tokens:
             kernels.attention_decode_int4(q, cache.k_pool, cache.v_pool, context, ctx.tok_item, ctx.positions, tables,
                                           self.heads, self.scale, 1, window=self.span, tok_list=ctx.portion_tokens,
@@ -423,7 +424,7 @@ class Attention(Mixer):
                                   torch.float32)
 
     def _int4_tile_records(self, ctx):
-        """The same for prompt portions: their ranges make no more blocks of up to 128 queries than there are units."""
+        """The same for prompt portions: their ranges make no more blocks, of up to 128 rows, than there are units."""
         worst = kernels.compute_units() * kernels.PREFILL_LARGE_TILE
         return ctx.workspace.flat(f"tile_partial_int4_{self.head_dim}", worst * (self.head_dim + 2), torch.float32)
 

@@ -202,12 +202,14 @@ def test_decode_refused_by_the_library(changed, message):
 
 
 PORTIONS = dict(table_width=5, heads=4, kv_heads=2, head_dim=64, page_size=16, num_pages=4, scale=0.125, window=0, max_kv_len=0,
-                query_tile=64, sink=0, softcap=0.0, ranges=1)
+                query_tile=64, sink=0, softcap=0.0, block_heads=1, ranges=1)
 
 
 @pytest.mark.parametrize("changed,message", [
     ({"heads": 5}, "multiple of kv_heads"), ({"head_dim": 72}, "multiple of 16"), ({"head_dim": 272}, "up to 256"),
-    ({"page_size": 20}, "multiple of 8"), ({"query_tile": 96}, "queries"), ({"query_tile": 128, "head_dim": 128}, "queries"),
+    ({"page_size": 20}, "multiple of 8"), ({"query_tile": 96}, "queries"), ({"query_tile": 128, "head_dim": 144}, "queries"), ({"block_heads": 2, "head_dim": 64}, "heads to a block"),
+    ({"block_heads": 2, "head_dim": 144}, "heads to a block"), ({"block_heads": 2, "head_dim": 128, "query_tile": 128}, "heads to a block"),
+    ({"block_heads": 2, "head_dim": 128, "heads": 6}, "heads to a block"), ({"block_heads": 3}, "heads to a block"),
     ({"query_tile": 32}, "queries"), ({"ranges": 0}, "ranges"), ({"ranges": 65}, "ranges"), ({"ranges": 2}, "floats of scratch"), ({"scale": 0.0}, "positive"), ({"table_width": 2049}, "exceed"),
     ({"num_pages": 1 << 28}, "key rows")])
 def test_prompt_refused_by_the_library(changed, message):

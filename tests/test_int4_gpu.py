@@ -269,7 +269,8 @@ PROMPT = [
     (1, 1, 64, 8, (2,), (0,), 0, False, 0.0), (3, 1, 64, 16, (65, 130), (0, 0), 0, False, 0.0),
     (2, 4, 128, 16, (33, 70, 2), (100, 0, 31), 0, False, 0.0), (1, 2, 16, 8, (40,), (3,), 0, True, 0.0),
     (2, 1, 48, 24, (100, 20), (0, 50), 0, False, 30.0), (1, 3, 96, 16, (64,), (10,), 40, False, 0.0),
-    (1, 1, 256, 64, (70,), (20,), 0, True, 0.0), (1, 2, 80, 8, (35,), (5,), -16, False, 0.0),
+    (1, 1, 256, 64, (70,), (20,), 0, True, 0.0), (1, 2, 80, 8, (35,), (5,), -16, False, 0.0), (2, 6, 112, 16, (70, 9), (40, 0), 30, True, 20.0),
+    (1, 2, 128, 8, (64, 65, 1, 40), (0, 7, 130, 9), 0, True, 0.0),
     (1, 1, 160, 16, (50,), (0,), 0, False, 0.0), (2, 1, 32, 8, (129,), (200,), 0, False, 0.0), (1, 1, 112, 8, (60,), (8,), 0, False, 0.0)]
 
 
@@ -293,15 +294,17 @@ def test_prompt_portions(kv_heads, group, dim, page, counts, starts, window, sin
     expected = [torch.cat([part[which] for part in parts]) for which in range(3)]
     limit = plain.allowed(*expected, BF16, True)
     for size in (64, 128):
-        if size == 128 and dim > 64:
+        if size == 128 and dim > 128:
             continue
         tiles = [(item, q0) for item, count in enumerate(counts) for q0 in range(0, count, size)]
-        for max_kv_len, ranges in ((100, None), (0, 1), (600, 1), (0, 2), (600, 5)):      # (they steer the launch)
+        pairs = size == 64 < dim <= 128 and group % 2 == 0
+        for max_kv_len, ranges, pair in ((100, None, None), (0, 1, 1), (600, 1, 1), (0, 2, 1), (600, 5, 1),
+                                         *([(0, 1, 2), (600, 3, 2)] if pairs else [])):      # (they steer the launch)
             out = torch.full((tokens + 1, heads * dim), -9.0, dtype=BF16).cuda()
             kernels.attention_prefill_int4(q.cuda(), *pools, out[:tokens], _ints([t[0] for t in tiles]),
                                            _ints([t[1] for t in tiles]), _ints(cu), _ints(lengths), tables.cuda(), heads,
-                                           scale, window, max_kv_len, size, sinks, softcap, ranges)
-            assert bool(((out[:tokens].double().cpu() - expected[0]).abs() <= limit).all()), (size, max_kv_len, ranges)
+                                           scale, window, max_kv_len, size, sinks, softcap, pair, ranges)
+            assert bool(((out[:tokens].double().cpu() - expected[0]).abs() <= limit).all()), (size, max_kv_len, ranges, pair)
             assert bool((out[tokens] == -9.0).all())
     out = torch.zeros((tokens, heads * dim), dtype=BF16).cuda()
     kernels.attention_decode_int4(q.cuda(), *pools, out, _ints(items), _ints(positions), tables.cuda(), heads, scale, 1,
@@ -312,7 +315,7 @@ def test_prompt_portions(kv_heads, group, dim, page, counts, starts, window, sin
 LONG = [
     # kv_heads, group, dim, page, counts, starts, window, sink, softcap, query_tile
     (2, 2, 64, 16, (70, 3), (1500, 40), 0, True, 0.0, 64), (1, 4, 64, 24, (130,), (900,), 300, False, 0.0, 128),
-    (1, 2, 128, 8, (20, 64), (1100, 700), 0, False, 20.0, 64), (1, 1, 256, 16, (66,), (800,), -256, True, 0.0, 64)]
+    (1, 2, 128, 8, (20, 64), (1100, 700), 0, False, 20.0, 64), (1, 1, 128, 16, (140,), (1000,), 0, True, 0.0, 128), (1, 1, 256, 16, (66,), (800,), -256, True, 0.0, 64)]
 
 
 @pytest.mark.parametrize("kv_heads,group,dim,page,counts,starts,window,sink,softcap,size", LONG)
@@ -338,19 +341,19 @@ def test_prompt_portions_in_ranges(kv_heads, group, dim, page, counts, starts, w
     tiles = [(item, q0) for item, count in enumerate(counts) for q0 in range(0, count, size)]
     rule = kernels.prefill_int4_ranges(len(tiles), heads, max(lengths))
     assert rule > 1
-    for ranges in (rule, 7, 64):
+    for ranges, pair in ((rule, 1), (7, 1), (64, 1), *([(rule, 2), (5, 2)] if dim == 128 and group == 2 else [])):
         needed = len(tiles) * heads * ranges * size * (dim + 2)
         partial = torch.full((needed + 8,), math.nan).cuda()
         out = torch.full((tokens + 1, heads * dim), -9.0, dtype=BF16).cuda()
         kernels.attention_prefill_int4(q.cuda(), *pools, out[:tokens], _ints([t[0] for t in tiles]),
                                        _ints([t[1] for t in tiles]), _ints(cu), _ints(lengths), tables.cuda(), heads, scale,
-                                       window, max(lengths), size, sinks, softcap, ranges, partial)
-        assert bool(((out[:tokens].double().cpu() - expected[0]).abs() <= limit).all()), ranges
+                                       window, max(lengths), size, sinks, softcap, pair, ranges, partial)
+        assert bool(((out[:tokens].double().cpu() - expected[0]).abs() <= limit).all()), (ranges, pair)
         assert bool((out[tokens] == -9.0).all()) and bool(partial[needed:].isnan().all())
     with pytest.raises(kernels.KernelError, match="floats of scratch"):
         kernels.attention_prefill_int4(q.cuda(), *pools, out[:tokens], _ints([t[0] for t in tiles]),
                                        _ints([t[1] for t in tiles]), _ints(cu), _ints(lengths), tables.cuda(), heads, scale,
-                                       window, max(lengths), size, sinks, softcap, 64, partial[:-9])
+                                       window, max(lengths), size, sinks, softcap, pair, ranges, partial[:-9])
 
 
 @pytest.mark.parametrize("bad", ["key", "value"])
