@@ -17,7 +17,10 @@
 //            is to be taken off, 24 times, at the end.
 //
 // Bound by memory where there are blocks enough (4.5 bits a value), else by the trip block table -> codes: a tile's codes
-// are asked for a tile ahead, its table entries, which are the same for a wave and come through the scalar unit, two.
+// are asked for two or three tiles ahead (Int4Stage), its table entries, which are the same for a wave and come through the
+// scalar unit, one more.  32 requests over 8,192 keys, 12 heads of 64: 56 to 58 us, 4.0 TB/s, 82 % of a large copy's rate;
+// 64 over 768 to 1,024, 25 heads that share no keys: 33 to 35 us, 3.0 TB/s; 24 over up to 6,000, 16 heads of 128 over 2:
+// 17.7 us and 3.9 for the merge; 1 over 900: 5.0 and 2.0.
 //
 // float queries, and scales that are not positive, take the kernel on the vector unit: LPK lanes share a key, a lane holds
 // eight dimensions of the query and takes one word of the key's codes; a conversion of the code and a multiply-add to a

@@ -1300,7 +1300,7 @@ def _first(what, tensor, name):
     """(dtype, device) of a call's first rows, which lie on the current device: kernels are launched on its stream."""
     try:
         device = tensor.get_device()
-        if tensor.dim() == 2 and (device == torch._C._cuda_getDevice() if device >= 0 else tensor.is_cuda):
+        if device == torch._C._cuda_getDevice() if device >= 0 else tensor.is_cuda:
             return tensor.dtype, device
     except AttributeError:
         pass
@@ -1329,12 +1329,12 @@ def _dense(tensor, name, dtype, ndim, device):
 def _rows_on(tensor, name, dtype, device):
     """(address, row stride) of rows of this type on a call's device."""
     try:
-        if tensor.dtype is dtype and tensor.dim() == 2 and tensor.get_device() == device:
+        if tensor.dtype is dtype and tensor.get_device() == device:
             stride, step = tensor.stride()
-            if step == 1 and tensor.size(0) > 1:
+            if step == 1 and tensor.numel() > stride:         # (more than one row)
                 return tensor.data_ptr(), stride
             return tensor.data_ptr(), _rows(tensor, name)
-    except AttributeError:
+    except (AttributeError, ValueError):
         pass
     _check(tensor, name, dtype, 2)
     _elsewhere(tensor, name, device)
@@ -1374,13 +1374,13 @@ def _token_index(tok_item, tok_pos, tables, tokens, device, direct_items=False):
     """Addresses of a step's index arrays and the tables' width; as ``_check_step_index``."""
     try:
         items, width = tables.shape
-        if (tables.dtype is torch.int32 is tok_pos.dtype and tok_pos.dim() == 1 and tok_pos.size(0) >= tokens
+        if (tables.dtype is torch.int32 is tok_pos.dtype and tok_pos.dim() == 1 and tok_pos.numel() >= tokens
                 and tables.is_contiguous() and tok_pos.is_contiguous()
                 and tables.get_device() == device == tok_pos.get_device()):
             if tok_item is None:
                 if direct_items and items >= tokens:
                     return 0, tok_pos.data_ptr(), tables.data_ptr(), width
-            elif (tok_item.dtype is torch.int32 and tok_item.dim() == 1 and tok_item.size(0) >= tokens
+            elif (tok_item.dtype is torch.int32 and tok_item.dim() == 1 and tok_item.numel() >= tokens
                     and tok_item.is_contiguous() and tok_item.get_device() == device):
                 return tok_item.data_ptr(), tok_pos.data_ptr(), tables.data_ptr(), width
     except (AttributeError, ValueError):
@@ -1454,14 +1454,14 @@ def attention_decode_int4(q, k_pool, v_pool, out, tok_item, tok_pos, tables, hea
     dtype, device = _first("attention_decode_int4", q, "q")
     q_at, q_stride = _rows_on(q, "q", dtype, device)
     out_at, out_stride = _rows_on(out, "out", dtype, device)
-    tokens, columns = q.shape
+    shape = tokens, columns = q.shape
     k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, columns, heads, device)
-    if out.shape != q.shape:
+    if out.shape != shape:
         raise KernelError("attention_decode_int4: q and out rows must hold heads x head_dim values")
     item_at, pos_at, tables_at, width = _token_index(tok_item, tok_pos, tables, tokens, device, direct_items=True)
     list_at, count = 0, tokens
     if tok_list is not None:
-        list_at, count = _dense(tok_list, "tok_list", torch.int32, 1, device), tok_list.size(0)
+        list_at, count = _dense(tok_list, "tok_list", torch.int32, 1, device), tok_list.numel()
     partial_at = floats = 0
     if splits > 1:
         partial_at, floats = _dense(partial, "partial", torch.float32, None, device), partial.numel()
@@ -1534,14 +1534,16 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
     _, device = _first("attention_prefill_int4", q, "q")
     q_at, q_stride = _rows_on(q, "q", torch.bfloat16, device)
     out_at, out_stride = _rows_on(out, "out", torch.bfloat16, device)
-    k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, q.size(1), heads, device)
-    if out.shape != q.shape:
+    shape = _, columns = q.shape
+    k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, columns, heads, device)
+    if out.shape != shape:
         raise KernelError("attention_prefill_int4: q and out rows must hold heads x head_dim values")
     index = (_dense(tile_item, "tile_item", torch.int32, 1, device), _dense(tile_q0, "tile_q0", torch.int32, 1, device),
              _dense(cu_tokens, "cu_tokens", torch.int32, 1, device), _dense(kv_lens, "kv_lens", torch.int32, 1, device))
     tables_at = _dense(tables, "tables", torch.int32, 2, device)
-    tiles, items = tile_item.size(0), kv_lens.size(0)
-    if tile_q0.size(0) != tiles or cu_tokens.size(0) != items + 1 or tables.size(0) != items:
+    tiles, items = tile_item.numel(), kv_lens.numel()
+    table_rows, table_width = tables.shape
+    if tile_q0.numel() != tiles or cu_tokens.numel() != items + 1 or table_rows != items:
         raise KernelError("attention_prefill_int4: inconsistent tile or item arrays")
     sink_at = 0
     if sink is not None:
@@ -1560,7 +1562,7 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
             partial = torch.empty(tiles * heads * ranges * query_tile * (head_dim + 2), dtype=torch.float32, device=q.device)
         partial_at, floats = _dense(partial, "partial", torch.float32, None, device), partial.numel()
     _call("ps_attention_prefill_int4", q_at, q_stride, k_at, v_at, out_at, out_stride, index[0], index[1], tiles, index[2],
-          index[3], tables_at, tables.size(1), heads, kv_heads, head_dim, page_size, pages, float(scale),
+          index[3], tables_at, table_width, heads, kv_heads, head_dim, page_size, pages, float(scale),
           int(window), max_kv_len, query_tile, sink_at, _check_cap(softcap), int(block_heads), int(ranges),
           partial_at, floats, _stream())
     return out
@@ -2707,7 +2709,7 @@ def token_logprobs(logits, tokens, out, entropy=None, ranks=None, top_ids=None, 
 
     def per_row(tensor, name, kind):
         at = _dense(tensor, name, kind, 1, device)
-        if tensor.size(0) < rows:
+        if tensor.numel() < rows:
             raise KernelError(f"token_logprobs: {name} needs an entry per row ({rows})")
         return at
 
