@@ -451,7 +451,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
   block_m = fmaxf(block_m, sink);
   const float share = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - block_m);
   if (c == 0) {
-    s_l[wave * I4_HEADS + n] = l * share + (wave == 0 && sinks ? __builtin_amdgcn_exp2f(sink - block_m) : 0.f);
+    s_l[wave * I4_HEADS + n] = l * share + (wave == 0 && sink != -INFINITY ? __builtin_amdgcn_exp2f(sink - block_m) : 0.f);
     if (wave == 0) s_block[n] = block_m;
   }
   if (n < count) {
@@ -735,7 +735,7 @@ extern "C" int ps_attention_decode_int4(const void* q, int64_t q_stride, const v
   PS_REQUIRE(head_dim > 0 && head_dim <= 256, "ps_attention_decode_int4: head_dim %d must lie in 1..256", head_dim);
   PS_REQUIRE(page_size % 8 == 0 && page_size <= (1 << 20),
              "ps_attention_decode_int4: pages of a cache in 4 bits hold a multiple of 8 keys, not %d", page_size);
-  PS_REQUIRE((int64_t)table_width * page_size < ((int64_t)1 << 31),
+  PS_REQUIRE((int64_t)table_width * page_size < ((int64_t)1 << 30),
              "ps_attention_decode_int4: block tables of %d pages of %d keys", table_width, page_size);
   PS_REQUIRE(splits >= 1 && splits <= 64, "ps_attention_decode_int4: 1 to 64 ranges, not %d", splits);
   PS_REQUIRE(dtype == PS_F32 || dtype == PS_BF16, "ps_attention_decode_int4: unknown dtype %d", dtype);

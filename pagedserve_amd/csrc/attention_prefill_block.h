@@ -139,7 +139,11 @@ __device__ __forceinline__ void attention_prefill_block(
   const int wave_last = start + wave_last_q;
   const bool wave_active = q0 + wave_q * 32 < count;
   const int tile_last_q = q0 + QUERIES - 1 < count ? q0 + QUERIES - 1 : count - 1;
-  const int key_end = start + tile_last_q + 1;
+  // (over a cache in 4 bits positions behind the block table see what the table has)
+  const int64_t table_room = Pages::INT4 ? (int64_t)table_width * page_size : INT32_MAX;
+  const int room = table_room < INT32_MAX ? (int)table_room : INT32_MAX;
+  const int key_end = start + tile_last_q + 1 < room ? start + tile_last_q + 1 : room;
+  const int q_last = q_pos < room ? q_pos : room - 1;
   const int key_begin = first_visible_key(start + q0, window);
   // the first keys that the wave's first and last query see
   const int first_of_first = first_visible_key(wave_first, window);
@@ -520,7 +524,7 @@ __device__ __forceinline__ void attention_prefill_block(
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int key = kw + r * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
-            const bool visible = (key <= q_pos) & (key >= q_first);
+            const bool visible = (key <= q_last) & (key >= q_first);
             s[r][e] = visible ? s[r][e] : -INFINITY;
             tile_max = fmaxf(tile_max, s[r][e]);
           }

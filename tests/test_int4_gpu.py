@@ -131,6 +131,24 @@ def test_positions_outside_the_table(kind, splits):
     assert bool(((out[1:2].double().cpu() - expected[0]).abs() <= plain.allowed(*expected, kind, kind == BF16)).all())
 
 
+@pytest.mark.parametrize("dim,size,ranges", [(64, 64, 1), (64, 128, 2), (128, 128, 1), (128, 64, 3), (256, 64, 1)])
+def test_portions_that_pass_the_table(dim, size, ranges):
+    """A portion whose last queries lie behind the block table: they see all that the table has, those in front as ever."""
+    from pagedserve_amd.ops import kernels
+
+    tables, pages, _, _ = _requests((1,), (111,), 16, 15)
+    tables = tables[:, :7].contiguous()                        # 112 keys
+    pools, kept = _cache(tables, pages, (112,), 1, dim, 16, 16)
+    q = torch.randn((100, dim), generator=torch.Generator().manual_seed(17)).to(BF16)
+    positions = list(range(50, 150))
+    tiles = list(range(0, 100, size))
+    out = torch.zeros((100, dim), dtype=BF16).cuda()
+    kernels.attention_prefill_int4(q.cuda(), *pools, out, _ints([0] * len(tiles)), _ints(tiles), _ints([0, 100]),
+                                   _ints([150]), tables.cuda(), 1, dim ** -0.5, query_tile=size, ranges=ranges)
+    expected = list(plain.attention(q, *kept[0], [min(p, 111) for p in positions], 1, dim ** -0.5))
+    assert bool(((out.double().cpu() - expected[0]).abs() <= plain.allowed(*expected, BF16, True)).all())
+
+
 @pytest.mark.parametrize("kind", [BF16, F32])
 def test_values_of_every_magnitude(kind):
     """Numbers of 8 bits, whose quotients by a step of 5 often are half way between two codes, from the smallest steps
@@ -262,6 +280,24 @@ def test_tokens_that_see_nothing(kind):
             assert bool((out[:2] == 0).all())
             out_1, size, shift = plain.attention(q[2:], kept[2][0][:21], kept[2][1][:21], [20], 2, 0.125, window)
             assert bool(((out[2:].double().cpu() - out_1).abs() <= plain.allowed(out_1, size, shift, kind, kind == BF16)).all())
+
+
+@pytest.mark.parametrize("kind", [BF16, F32])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_sinks_of_minus_infinity(kind, splits):
+    """A sink that weighs nothing: attention without one, and zeros for a token that sees nothing."""
+    from pagedserve_amd.ops import kernels
+
+    tables, pages, _, _ = _requests((1, 1), (19, 299), 16, 34)
+    pools, kept = _cache(tables, pages, (20, 300), 2, 64, 16, 35)
+    q = torch.randn((2, 128), generator=torch.Generator().manual_seed(36)).to(kind)
+    sinks = torch.tensor([-math.inf, 0.5]).cuda()
+    out = torch.full((2, 128), 5.0, dtype=kind).cuda()
+    kernels.attention_decode_int4(q.cuda(), *pools, out, None, _ints([-1, 299]), tables.cuda(), 2, 0.125, splits,
+                                  torch.zeros(2 * 2 * splits * 66).cuda(), sink=sinks)
+    assert bool((out[0] == 0).all())
+    expected = list(plain.attention(q[1:], *kept[1], [299], 2, 0.125, 0, sinks))
+    assert bool(((out[1:].double().cpu() - expected[0]).abs() <= plain.allowed(*expected, kind, kind == BF16)).all())
 
 
 PROMPT = [
