@@ -17,10 +17,10 @@
 //            is to be taken off, 24 times, at the end.
 //
 // Bound by memory where there are blocks enough (4.5 bits a value), else by the trip block table -> codes: a tile's codes
-// are asked for two or three tiles ahead (Int4Stage), its table entries, which are the same for a wave and come through the
-// scalar unit, one more.  32 requests over 8,192 keys, 12 heads of 64: 56 to 58 us, 4.0 TB/s, 82 % of a large copy's rate;
-// 64 over 768 to 1,024, 25 heads that share no keys: 33 to 35 us, 3.0 TB/s; 24 over up to 6,000, 16 heads of 128 over 2:
-// 17.7 us and 3.9 for the merge; 1 over 900: 5.0 and 2.0.
+// are asked for one tile ahead (Int4Stage), its table entries, which are the same for a wave and come through the scalar
+// unit, two.  32 requests over 8,192 keys, 12 heads of 64: 51 us, 4.4 TB/s, 90 % of a large copy's rate (64: 92 us, 4.9 TB/s); 64 over
+// 768 to 1,024, 25 heads that share no keys: 29.4 us, 3.5 TB/s; 24 over up to 6,000, 16 heads of 128 over 2: 16.1 us; 1
+// over 900: 5.0 us and 2.0 for the merge.
 //
 // float queries, and scales that are not positive, take the kernel on the vector unit: LPK lanes share a key, a lane holds
 // eight dimensions of the query and takes one word of the key's codes; a conversion of the code and a multiply-add to a
@@ -134,9 +134,9 @@ struct Int4Decode {
 
 // EVEN: pages of a power of two, 16 or more: 16 keys from a multiple of 16 on lie in one page (else 8 from a multiple of 8), whose
 // place the scalar unit works out for the wave.
-// dynamic LDS: the waves' maxima and sums [WAVES][16] each, the block's maxima [16], then the waves' rings of DEPTH tiles, in
+// dynamic LDS: the waves' maxima and sums [WAVES][16] each, the block's maxima [16], then the waves' pairs of tiles, in
 // whose place the accumulators [WAVES][heads of the block][32 G] meet at the end
-template <int G, int WAVES, bool EVEN, int DEPTH>
+template <int G, int WAVES, bool EVEN>
 __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel(const Int4Decode a) {
   typedef Int4Stage<G> Stage;
   extern __shared__ __attribute__((aligned(1024))) float lds[];
@@ -237,10 +237,10 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
     for (int i = 1; i < UNITS; ++i) found += (at[i] - at[0]) & -(int64_t)(u == i);
     return found;
   };
-  unsigned char* ring = stages + wave * (DEPTH * Stage::BYTES);
+  unsigned char* pair = stages + wave * (2 * Stage::BYTES);
   auto issue = [&](int slot, const Entries& e, int base) __attribute__((always_inline)) {
     const Places at = places(e, base);
-    unsigned char* stage = ring + slot * Stage::BYTES;
+    unsigned char* stage = pair + slot * Stage::BYTES;
 #pragma unroll
     for (int j = 0; j < G; ++j) {
       const int piece = j * 64 + lane;
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
     }
   };
 
-  // DEPTH - 1 tiles are on their way while one is worked on; the table's entries are asked for one tile earlier still
+  // one tile is on its way while one is worked on; the table's entries are asked for one tile earlier still
   int base = begin + wave * I4_TILE, ahead = base;
   constexpr int STRIDE = I4_TILE * WAVES;
   Entries entries = {};
@@ -278,9 +278,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
   };
   if (base < end) {
     entries = ask(base);
-#pragma unroll
-    for (int i = 0; i < DEPTH - 1; ++i)
-      if (ahead < end) send(i);
+    send(0);
   }
 
   // the queries, column n of the products: dimensions 32 g + 8 c + (0, 4, 1, 5, ..), the order of a word's nibbles
@@ -312,7 +310,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
 
   // Lane (16 c + n) reads the words c G .. of keys n and 16 + n, and of keys 4 c .. + 3 and 16 + 4 c .. + 3 the bytes n G .. of
   // the values and all steps.
-  const uint32_t ring_at = (uint32_t)(uintptr_t)(int4_lds_ptr)ring;
+  const uint32_t pair_at = (uint32_t)(uintptr_t)(int4_lds_ptr)pair;
   const uint32_t key_lane = n * (16 * G) + c * (4 * G), value_lane = Stage::CODES + 4 * c * (16 * G) + n * G;
   const uint32_t step_lane = 2 * Stage::CODES + 4 * c * (2 * G);
   // scores of those 8 keys, head n; unscaled
@@ -403,15 +401,14 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
 
   int slot = 0;
   while (base < end) {
-    // the tile in the stage that was read last is on its way again
-    if (ahead < end) send(slot == 0 ? DEPTH - 1 : slot - 1);
+    // the stage that was read last is filled again
+    if (ahead < end) send(slot ^ 1);
     // the loads of this tile have landed; those behind it are on their way
-    if (on_way == DEPTH) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * Stage::LOADS) : "memory");
-    else if (DEPTH > 2 && on_way == DEPTH - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 2) * Stage::LOADS) : "memory");
+    if (on_way == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Stage::LOADS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const unsigned units = exist & 15u;
     const bool whole = base >= first && base + I4_TILE <= end && units == (1u << UNITS) - 1;
-    const uint32_t stage = ring_at + slot * Stage::BYTES;
+    const uint32_t stage = pair_at + slot * Stage::BYTES;
     float s[8];
     score(s, stage);
     if (a.softcap_log2 > 0.f) {
@@ -426,7 +423,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
       for (int i = 0; i < 8; ++i) s[i] = visible(16 * (i >> 2) + 4 * c + (i & 3)) ? s[i] : -INFINITY;
       // nobody knows what a masked key's steps are, and 0 times a NaN is none: the values' steps become 0 where they lie
       if (lane < I4_TILE && !visible(lane)) {
-        uint16_t* steps = reinterpret_cast<uint16_t*>(ring + slot * Stage::BYTES + 2 * Stage::CODES + Stage::STEPS) + lane * G;
+        uint16_t* steps = reinterpret_cast<uint16_t*>(pair + slot * Stage::BYTES + 2 * Stage::CODES + Stage::STEPS) + lane * G;
 #pragma unroll
         for (int g = 0; g < G; ++g) steps[g] = 0;
       }
@@ -436,7 +433,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
     base += STRIDE;
     exist >>= 4;
     --on_way;
-    slot = slot == DEPTH - 1 ? 0 : slot + 1;
+    slot ^= 1;
   }
 
   // the waves' states meet: maxima first, then sums and accumulators scaled to the block's
@@ -495,16 +492,17 @@ static void int4_allow_lds(const void* kernel, int bytes) {
 
 template <int G>
 static void launch_heads(const Int4Decode& a, int count, int waves, hipStream_t s) {
-  // tiles in a wave's ring: as many as leave room for the waves that the registers allow
-  constexpr int DEPTH = G <= 2 ? 4 : G <= 4 ? 3 : 2;
   const dim3 grid(count, a.kv_heads * a.parts, a.splits);
-  const int ring = waves * DEPTH * Int4Stage<G>::BYTES, meet = waves * a.block_heads * 32 * G * 4;
-  const int bytes = (I4_HEADS + waves * 2 * I4_HEADS) * 4 + (ring > meet ? ring : meet);
+  // A pair of tiles to a wave.  (Three or four leave room for fewer blocks on a unit, which weighs more: 64 requests of 25 heads over
+  // 1,024 keys 32.7 us with two, 34.0 with three and 36.4 with four, 128 of 12 over 1,000 29.7, 32.0 and 33.2; 64 of 32 heads
+  // of 128 over 8 and 1,500 keys 28.8 with two, 32 with three; 48 of 20 heads of 96 over 2,000 53 and 63.)
+  const int pairs = waves * 2 * Int4Stage<G>::BYTES, meet = waves * a.block_heads * 32 * G * 4;
+  const int bytes = (I4_HEADS + waves * 2 * I4_HEADS) * 4 + (pairs > meet ? pairs : meet);
   const bool even = a.page_size >= 16 && a.page_shift >= 0;
 #define PS_LAUNCH_H4E(WAVES, EVEN)                                                                              \
   do {                                                                                                          \
-    int4_allow_lds(reinterpret_cast<const void*>(attention_decode_int4_heads_kernel<G, WAVES, EVEN, DEPTH>), bytes); \
-    hipLaunchKernelGGL((attention_decode_int4_heads_kernel<G, WAVES, EVEN, DEPTH>), grid, dim3(64 * WAVES), bytes, s, a); \
+    int4_allow_lds(reinterpret_cast<const void*>(attention_decode_int4_heads_kernel<G, WAVES, EVEN>), bytes); \
+    hipLaunchKernelGGL((attention_decode_int4_heads_kernel<G, WAVES, EVEN>), grid, dim3(64 * WAVES), bytes, s, a); \
   } while (0)
 #define PS_LAUNCH_H4(WAVES)                \
   do {                                     \

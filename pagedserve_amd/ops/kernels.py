@@ -1431,19 +1431,24 @@ def int4_decode_splits(dtype, count, heads, kv_heads, head_dim, visible) -> int:
     * Up to 384 keys one range, whose block has eight waves where the blocks leave units idle (us in one range and in
       two or three: 1 and 8 requests of 12 heads over 144 and 300 keys 4.9 / 6.3 and 5.7 / 7.1).
     * Up to half a block per unit, ranges until three blocks come to a unit, of a turn or more, eight at most, sixteen where
-      even these leave units idle (1 request of 12 heads over 900 keys in 1, 4 and 8 ranges 8.4, 7.3 and 6.3, over 4,096 in 8,
-      16 and 32 9.4, 8.1 and 8.3; 8 over 1,000 in 1 and 8 9.3 and 8.5, over 4,000 in 8 and 16 14.1 and 15.0; 24 of 16 heads of 128 over 2, up
-      to 6,000 keys, in 4, 8 and 16 24.2, 19.2 and 21.4).
-    * More blocks: one range up to 2,048 keys (20 of 12 heads over 1,000 in 1 and 2 10.2 and 12.2), beyond ranges until six come
-      to a unit (32 of 12 over 8,192 keys in 1, 2 and 4 68, 59.7 and 57.3)."""
+      even these leave units idle, or are of two turns (us; 1 request of 12 heads over 900 keys in 1, 4 and 8 ranges 8.4, 7.3
+      and 6.3, over 4,096 in 8, 16 and 32 9.4, 8.1 and 8.3; 4 over 8,192 in 8 and 16 15.0 and 13.2; 8 over 1,000 in 1 and 8
+      9.3 and 8.1, over 4,000 in 8 and 16 12.9 and 13.9; 24 of 16 heads of 128 over 2 and 6,000 keys in 8 and 16 20.2
+      and 19.2, 16 of 16 over 4 and 2,000 11.7 and 14.5).
+    * More blocks: one range up to 2,048 keys (20 of 12 heads over 1,000 in 1 and 2 9.1 and 11.1), beyond of 512 keys or more,
+      eight at most, until nine blocks come to a unit, of bfloat16 heads beyond 64, fewer of whose blocks a unit holds, three (32 of 12 over 8,192
+      keys in 1, 4, 6 and 8 81, 53.6, 50.8 and 52.6, 64 in 2, 3 and 4 101, 91.7 and 92.6; 64 of 32 heads of 128 over 4 and 4,096
+      in 3 and 6 38.6 and 41.1)."""
     units = compute_units()
     group = 1 if dtype == torch.float32 else heads // kv_heads
     blocks = max(1, count * (heads // group) * -(-group // (16 if head_dim <= 128 else 8)))
     if visible <= 384:
         return 1
     if 2 * blocks > units:
-        return 1 if visible <= 2048 else max(1, min(-(-6 * units // blocks), 64))
-    return max(1, min(16 if 16 * blocks <= units else 8, 3 * units // blocks, -(-visible // 128)))
+        full = 3 if head_dim > 64 and dtype != torch.float32 else 9
+        return 1 if visible <= 2048 else max(1, min(-(-full * units // blocks), visible // 512, 8))
+    many = 16 * blocks <= units or (16 * blocks <= 3 * units and -(-visible // 256) >= 16)
+    return max(1, min(16 if many else 8, 3 * units // blocks, -(-visible // 128)))
 
 
 def attention_decode_int4(q, k_pool, v_pool, out, tok_item, tok_pos, tables, heads, scale, splits, partial=None,

@@ -417,9 +417,9 @@ class Attention(Mixer):
 
     def _int4_records(self, ctx):
         """Scratch for the ranges' records of a decode step over a cache in 4 bits, at its largest: the rule asks for
-        ranges until three blocks of up to 16 heads come to a unit, or six beside one per token and key/value head."""
+        ranges until three blocks of up to 16 heads come to a unit, or nine beside one per token and key/value head."""
         group = min(16, self.heads // self.kv_heads)
-        worst = 6 * kernels.compute_units() * group + ctx.workspace.max_rows * self.heads
+        worst = 9 * kernels.compute_units() * group + ctx.workspace.max_rows * self.heads
         return ctx.workspace.flat(f"attn_partial_int4_{self.heads}x{self.head_dim}", worst * (self.head_dim + 2),
                                   torch.float32)
 
