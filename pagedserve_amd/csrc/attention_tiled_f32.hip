@@ -25,10 +25,16 @@
 // item whose cached length after the step is L and which brings n tokens stands at position
 // L - n + i and sees keys first_visible_key(position, window) .. position.
 //
+// Over a cache in 4 bits (cache_int4.h) a lane reads its key's whole row of codes, 16 bytes a group, and of a value the
+// byte of its dimension in every group, with the keys' steps; they become floats, exactly, where they are multiplied:
+// 2 x 1,024 tokens of 12 heads of 64 66.5 us (floats 61.8), 512 behind 3,500 keys 161 (128), 512 of 16 heads of 128 over 4
+// behind 2,000 157 (139); token by token 366, 609 and 975.
+//
 // Head sizes that are multiples of 4 up to 128; others stay with the one-wave-per-token
 // kernel.
 #include <math.h>
 
+#include "cache_int4.h"
 #include "common.h"
 #include "pagedserve_hip.h"
 
@@ -40,12 +46,22 @@
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float af_f32x4;
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float af_f32x16;
 
+// What the pools hold: floats, or bytes of codes and steps.
+template <bool INT4>
+struct AfPool {
+  typedef float Element;
+};
+template <>
+struct AfPool<true> {
+  typedef uint8_t Element;
+};
+
 // DF: 32 head dimensions each; RAGGED: the head size is not 32 DF; PAIRS: one block takes the 64 queries of a tile,
-// two waves to 32 of them; `parts`: else, blocks to a listed tile (of 32 queries each)
-template <int DF, bool RAGGED, bool PAIRS>
+// two waves to 32 of them; `parts`: else, blocks to a listed tile (of 32 queries each); INT4: a cache in 4 bits
+template <int DF, bool RAGGED, bool PAIRS, bool INT4>
 __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
-    const float* __restrict__ q, int64_t q_stride, const float* __restrict__ k_pool,
-    const float* __restrict__ v_pool, float* __restrict__ out, int64_t out_stride,
+    const float* __restrict__ q, int64_t q_stride, const typename AfPool<INT4>::Element* __restrict__ k_pool,
+    const typename AfPool<INT4>::Element* __restrict__ v_pool, float* __restrict__ out, int64_t out_stride,
     const int* __restrict__ tile_item, const int* __restrict__ tile_q0,
     const int* __restrict__ cu_tokens, const int* __restrict__ kv_lens,
     const int* __restrict__ tables, int table_width, int heads, int kv_heads, int head_dim,
@@ -103,25 +119,76 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
     const int logical = (k0 + column) / page_size;
     return table[logical < table_width ? logical : table_width - 1];
   };
-  auto row_of = [&](int k0, int page) -> int64_t {
+  // (of codes: the first byte of the key's row of codes, and how far behind it the key's steps lie)
+  auto row_of = [&](int k0, int page, int& to_steps) -> int64_t {
     const int key = k0 + column;
-    const int logical = key / page_size;
+    const int logical = key / page_size, within = key - logical * page_size;
     const bool there = key < key_end && logical < table_width && page >= 0 && page < num_pages;
-    const int64_t row = (((int64_t)page * kv_heads + kv_head) * page_size + (key - logical * page_size)) * head_dim;
+    if constexpr (INT4) {
+      to_steps = there ? page_size * (16 * DF) - within * (14 * DF) : 0;
+      const int64_t row = int4_page_at(page, kv_heads, kv_head, page_size, DF) + within * (16 * DF);
+      return there ? row : -1;
+    }
+    const int64_t row = (((int64_t)page * kv_heads + kv_head) * page_size + within) * head_dim;
     return there ? row : -1;
   };
-  af_f32x4 key_values[STEPS];
+  af_f32x4 key_values[INT4 ? 1 : STEPS];
   float values[DF][16];
-  // (rows that are not there are read from the pool's first row and not used)
-  auto load_keys = [&](int64_t row) {
-    const float* source = k_pool + (row < 0 ? 0 : row);
+  // a key's words, its steps and those of its value; of 16 values a byte per group and the steps
+  constexpr int BYTES = DF == 3 ? 3 : 1, STEP_WORDS = DF == 4 ? 2 : DF == 3 ? 3 : 1;
+  uint4 key_codes[INT4 ? DF : 1];
+  uint32_t key_steps[INT4 ? STEP_WORDS : 1], poison[INT4 ? STEP_WORDS : 1];
+  uint32_t value_codes[INT4 ? 16 : 1][BYTES], value_steps[INT4 ? 16 : 1][STEP_WORDS];
+  auto load_steps = [&](const uint8_t* from, uint32_t (&words)[STEP_WORDS]) {
+    if constexpr (DF == 4) {
+      const uint2 both = *reinterpret_cast<const uint2*>(from);
+      words[0] = both.x;
+      words[1] = both.y;
+    } else if constexpr (DF == 2) {
+      words[0] = *reinterpret_cast<const uint32_t*>(from);
+    } else {
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const int dim = 8 * s + 4 * half;
-      key_values[s] = *reinterpret_cast<const af_f32x4*>(source + (!RAGGED || dim < head_dim ? dim : 0));
+      for (int g = 0; g < DF; ++g) words[g] = reinterpret_cast<const uint16_t*>(from)[g];
     }
   };
-  auto load_values = [&](int64_t row) {
+  auto step_of = [&](const uint32_t (&words)[STEP_WORDS], int g) {
+    if constexpr (DF % 2 == 1) return __uint_as_float(words[g] << 16);
+    else return __uint_as_float(g % 2 ? words[g / 2] & 0xffff0000u : words[g / 2] << 16);
+  };
+  // (rows that are not there are read from the pool's first row and not used)
+  auto load_keys = [&](int64_t row, int to_steps) {
+    const auto* source = k_pool + (row < 0 ? 0 : row);
+    if constexpr (INT4) {
+#pragma unroll
+      for (int g = 0; g < DF; ++g) key_codes[g] = reinterpret_cast<const uint4*>(source)[g];
+      load_steps(source + to_steps, key_steps);
+      load_steps(v_pool + (row < 0 ? 0 : row) + to_steps, poison);
+    } else {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const int dim = 8 * s + 4 * half;
+        key_values[s] = *reinterpret_cast<const af_f32x4*>(source + (!RAGGED || dim < head_dim ? dim : 0));
+      }
+    }
+  };
+  // the key's dimensions 8 s + 4 half .. + 3
+  auto key_piece = [&](int s) -> af_f32x4 {
+    if constexpr (INT4) {
+      const int g = s / 4, w = (s % 4) * DF + g;
+      const uint32_t words[4] = {key_codes[w / 4].x, key_codes[w / 4].y, key_codes[w / 4].z, key_codes[w / 4].w};
+      const uint32_t codes = words[w % 4] >> (16 * half);
+      // A value that is no number must not reach the queries that do not see its key, whose weight of 0 would still make
+      // it one: it is 0 below, and the key takes its place here, whose scores are masked.
+      const float step = fmaf(step_of(poison, g), 0.f, step_of(key_steps, g)), base = -8.f * step;
+      af_f32x4 piece;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) piece[i] = fmaf((float)(codes >> (4 * i) & 15u), step, base);
+      return piece;
+    } else {
+      return key_values[s];
+    }
+  };
+  auto load_values = [&](int64_t row, int to_steps) {
     const int64_t from = row < 0 ? 0 : row;
     const int low = (int)from, high = (int)(from >> 32);
 #pragma unroll
@@ -131,11 +198,34 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
       const int low_0 = __builtin_amdgcn_readlane(low, key), low_1 = __builtin_amdgcn_readlane(low, key + 4);
       const int high_0 = __builtin_amdgcn_readlane(high, key), high_1 = __builtin_amdgcn_readlane(high, key + 4);
       const int64_t base = ((int64_t)(half ? high_1 : high_0) << 32) | (unsigned int)(half ? low_1 : low_0);
+      if constexpr (INT4) {
+        const int steps_0 = __builtin_amdgcn_readlane(to_steps, key), steps_1 = __builtin_amdgcn_readlane(to_steps, key + 4);
+        const uint8_t* bytes = v_pool + base + (column >> 1) * DF;
+        if constexpr (DF == 4) value_codes[e][0] = *reinterpret_cast<const uint32_t*>(bytes);
+        else if constexpr (DF == 2) value_codes[e][0] = *reinterpret_cast<const uint16_t*>(bytes);
+        else
 #pragma unroll
-      for (int f = 0; f < DF; ++f) {
-        const int dim = 32 * f + column;
-        values[f][e] = v_pool[base + (!RAGGED || dim < head_dim ? dim : 0)];
+          for (int g = 0; g < DF; ++g) value_codes[e][g] = bytes[g];
+        load_steps(v_pool + base + (half ? steps_1 : steps_0), value_steps[e]);
+      } else {
+#pragma unroll
+        for (int f = 0; f < DF; ++f) {
+          const int dim = 32 * f + column;
+          values[f][e] = v_pool[base + (!RAGGED || dim < head_dim ? dim : 0)];
+        }
       }
+    }
+  };
+  auto convert_values = [&]() {
+    if constexpr (INT4) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+#pragma unroll
+        for (int f = 0; f < DF; ++f) {
+          const uint32_t code = value_codes[e][DF == 3 ? f : 0] >> ((DF == 3 ? 0 : 8 * f) + 4 * (column & 1)) & 15u;
+          const float step = step_of(value_steps[e], f);
+          values[f][e] = ((float)code - 8.f) * (step == step ? step : 0.f);
+        }
     }
   };
 
@@ -152,10 +242,11 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
   int k0 = key_begin + turn * AF_ROWS;
   if (k0 < key_end) {
     constexpr int TURN = TURNS * AF_ROWS;
-    int64_t row = row_of(k0, page_of(k0));
-    load_keys(row);
+    int to_steps = 0, next_to_steps = 0;
+    int64_t row = row_of(k0, page_of(k0), to_steps);
+    load_keys(row, to_steps);
     int next_page = page_of(k0 + TURN);
-    load_values(row);
+    load_values(row, to_steps);
     for (; k0 < key_end; k0 += TURN) {
       // two chains of half the length: no instruction waits for the one before, half the rounding
       af_f32x16 sums[2];
@@ -163,14 +254,14 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
       for (int e = 0; e < 16; ++e) sums[0][e] = sums[1][e] = 0.f;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        af_f32x4 piece = key_values[s];
+        af_f32x4 piece = key_piece(s);
         if (RAGGED && 8 * s + 4 * half >= head_dim) piece = af_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           sums[i & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(piece[i], query[s][i], sums[i & 1], 0, 0, 0);
       }
-      const int64_t next_row = row_of(k0 + TURN, next_page);
-      load_keys(next_row);
+      const int64_t next_row = row_of(k0 + TURN, next_page, next_to_steps);
+      load_keys(next_row, next_to_steps);
       next_page = page_of(k0 + 2 * TURN);
       __builtin_amdgcn_sched_barrier(0);   // (these loads stay in front of the softmax)
 
@@ -216,6 +307,7 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[f][e] *= correction;
       }
+      convert_values();
       if (there != ~0ull) {
         // (nothing of rows that are not there: a weight of zero would keep what is not a number)
 #pragma unroll
@@ -230,7 +322,7 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
 #pragma unroll
         for (int f = 0; f < DF; ++f)
           acc[f] = __builtin_amdgcn_mfma_f32_32x32x2f32(values[f][e], p[e], acc[f], 0, 0, 0);
-      load_values(next_row);
+      load_values(next_row, next_to_steps);
       row = next_row;
     }
   }
@@ -295,6 +387,27 @@ extern "C" int ps_attention_tiled_f32_supported(int head_dim) {
 
 extern "C" int ps_attention_tiled_f32_tile() { return AF_TILE; }
 
+#define PS_LAUNCH_AF_FORM(DF, RAGGED, PAIRS, INT4)                                                \
+  hipLaunchKernelGGL((attention_tiled_f32_kernel<DF, RAGGED, PAIRS, INT4>), dim3((unsigned)blocks), \
+                     dim3(64 * AF_WAVES), 0, s, (const float*)q, q_stride,                        \
+                     (const AfPool<INT4>::Element*)k_pool, (const AfPool<INT4>::Element*)v_pool,  \
+                     (float*)out, out_stride, tile_item, tile_q0, cu_tokens, kv_lens, tables,     \
+                     table_width, heads, kv_heads, head_dim, page_size, num_pages, scale, window, parts, extra)
+#define PS_LAUNCH_AF_DF(DF, INT4)                                                                 \
+  do {                                                                                            \
+    if (head_dim == 32 * DF && paired) PS_LAUNCH_AF_FORM(DF, false, true, INT4);                  \
+    else if (head_dim == 32 * DF) PS_LAUNCH_AF_FORM(DF, false, false, INT4);                      \
+    else if (paired) PS_LAUNCH_AF_FORM(DF, true, true, INT4);                                     \
+    else PS_LAUNCH_AF_FORM(DF, true, false, INT4);                                                \
+  } while (0)
+#define PS_LAUNCH_AF(INT4)                    \
+  switch ((head_dim + 31) / 32) {             \
+    case 1: PS_LAUNCH_AF_DF(1, INT4); break;  \
+    case 2: PS_LAUNCH_AF_DF(2, INT4); break;  \
+    case 3: PS_LAUNCH_AF_DF(3, INT4); break;  \
+    default: PS_LAUNCH_AF_DF(4, INT4); break; \
+  }
+
 extern "C" int ps_attention_tiled_f32(const void* q, int64_t q_stride, const void* k_pool,
                                       const void* v_pool, void* out, int64_t out_stride,
                                       const int* tile_item, const int* tile_q0, int tiles,
@@ -327,27 +440,38 @@ extern "C" int ps_attention_tiled_f32(const void* q, int64_t q_stride, const voi
   if (blocks == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
   const AttnExtras extra = {sink, gate, gate_ld, softcap, logistic, logistic_norm};
-#define PS_LAUNCH_AF(DF)                                                                          \
-  do {                                                                                            \
-    if (head_dim == 32 * DF && paired) PS_LAUNCH_AF_FORM(DF, false, true);                        \
-    else if (head_dim == 32 * DF) PS_LAUNCH_AF_FORM(DF, false, false);                            \
-    else if (paired) PS_LAUNCH_AF_FORM(DF, true, true);                                           \
-    else PS_LAUNCH_AF_FORM(DF, true, false);                                                      \
-  } while (0)
-#define PS_LAUNCH_AF_FORM(DF, RAGGED, PAIRS)                                                      \
-  hipLaunchKernelGGL((attention_tiled_f32_kernel<DF, RAGGED, PAIRS>), dim3((unsigned)blocks),     \
-                     dim3(64 * AF_WAVES), 0, s,                                                   \
-                     (const float*)q, q_stride, (const float*)k_pool, (const float*)v_pool,       \
-                     (float*)out, out_stride, tile_item, tile_q0, cu_tokens, kv_lens, tables,     \
-                     table_width, heads, kv_heads, head_dim, page_size, num_pages, scale, window, parts, extra)
-  switch ((head_dim + 31) / 32) {
-    case 1: PS_LAUNCH_AF(1); break;
-    case 2: PS_LAUNCH_AF(2); break;
-    case 3: PS_LAUNCH_AF(3); break;
-    default: PS_LAUNCH_AF(4); break;
-  }
-#undef PS_LAUNCH_AF_FORM
-#undef PS_LAUNCH_AF
+  PS_LAUNCH_AF(false);
   PS_CHECK_LAUNCH("ps_attention_tiled_f32");
+  return 0;
+}
+
+extern "C" int ps_attention_tiled_f32_int4(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool,
+                                           void* out, int64_t out_stride, const int* tile_item, const int* tile_q0,
+                                           int tiles, const int* cu_tokens, const int* kv_lens, const int* tables,
+                                           int table_width, int heads, int kv_heads, int head_dim, int page_size,
+                                           int num_pages, float scale, int window, const float* sink, float softcap,
+                                           int query_tile, int paired, void* stream) {
+  const char* who = "ps_attention_tiled_f32_int4";
+  PS_REQUIRE(tiles >= 0 && heads > 0 && kv_heads > 0 && page_size > 0 && num_pages > 0 && table_width > 0,
+             "%s: bad sizes", who);
+  PS_REQUIRE(ps_attention_tiled_f32_supported(head_dim), "%s: head_dim %d must be a multiple of 4 up to %d", who, head_dim,
+             AF_MAX_DIM);
+  PS_REQUIRE(heads % kv_heads == 0, "%s: heads (%d) must be a multiple of kv_heads (%d)", who, heads, kv_heads);
+  PS_REQUIRE(page_size % 8 == 0 && page_size <= (1 << 20),
+             "%s: pages of a cache in 4 bits hold a multiple of 8 keys, not %d", who, page_size);
+  PS_REQUIRE(scale > 0.f, "%s: the score scale must be positive, got %g", who, scale);
+  PS_REQUIRE(q_stride % 4 == 0 && out_stride % 4 == 0 &&
+                 ((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16 == 0,
+             "%s: rows of q, out and the pools must allow 16-byte accesses", who);
+  PS_REQUIRE(query_tile == AF_TILE || (query_tile == AF_ROWS && !paired),
+             "%s: tiles of %d (paired or not) or %d queries, not %d", who, AF_TILE, AF_ROWS, query_tile);
+  const int parts = paired ? 1 : query_tile / AF_ROWS;
+  const int64_t blocks = (int64_t)tiles * heads * parts;
+  PS_REQUIRE(blocks < ((int64_t)1 << 31), "%s: too many blocks", who);
+  if (blocks == 0) return 0;
+  hipStream_t s = (hipStream_t)stream;
+  const AttnExtras extra = {sink, nullptr, 0, softcap, nullptr, 1.f};
+  PS_LAUNCH_AF(true);
+  PS_CHECK_LAUNCH(who);
   return 0;
 }

@@ -319,6 +319,14 @@ int ps_attention_prefill_int4(const void* q, int64_t q_stride, const void* k_poo
                               const float* sink, float softcap, int block_heads, int ranges, float* partial,
                               int64_t partial_floats, void* stream);
 
+// ps_attention_tiled_f32 over such a cache.
+int ps_attention_tiled_f32_int4(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool,
+                                void* out, int64_t out_stride, const int* tile_item, const int* tile_q0,
+                                int tiles, const int* cu_tokens, const int* kv_lens, const int* tables,
+                                int table_width, int heads, int kv_heads, int head_dim, int page_size,
+                                int num_pages, float scale, int window, const float* sink, float softcap,
+                                int query_tile, int paired, void* stream);
+
 // logprobs[r] = log softmax(logits[r])[tokens[r]] of rows `ld` apart, of `dtype`.  entropy, ranks, top_ids, top_logprobs: null, or what
 // is wanted of them (the two last [rows, top], top up to 32).  A token of -1: none (0, rank -1); others outside the vocabulary: NaN, -1.
 // partial: scratch of ps_logprob_scratch(rows, vocab, top) floats.

@@ -157,6 +157,9 @@ _SIGNATURES = {
     "ps_attention_prefill_int4": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int,
                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
                                   c_int, c_int, c_int, c_void_p, c_float, c_int, c_int, c_void_p, c_int64, c_void_p],
+    "ps_attention_tiled_f32_int4": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int,
+                                    c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
+                                    c_int, c_void_p, c_float, c_int, c_int, c_void_p],
     "ps_token_logprobs": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                           c_int, c_void_p, c_int64, c_int, c_void_p],
     "ps_sample": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
@@ -1529,6 +1532,30 @@ def prefill_int4_ranges(tiles, heads, max_kv_len) -> int:
     return max(1, min(compute_units() // max(1, tiles * heads), max_kv_len // 128, 16))
 
 
+def _int4_tiles(what, q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_lens, tables, heads, sink, dtype):
+    """What the launches over tiles of queries take, checked: addresses and sizes."""
+    _, device = _first(what, q, "q")
+    q_rows, out_rows = _rows_on(q, "q", dtype, device), _rows_on(out, "out", dtype, device)
+    shape = _, columns = q.shape
+    k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, columns, heads, device)
+    if out.shape != shape:
+        raise KernelError(f"{what}: q and out rows must hold heads x head_dim values")
+    index = (_dense(tile_item, "tile_item", torch.int32, 1, device), _dense(tile_q0, "tile_q0", torch.int32, 1, device),
+             _dense(cu_tokens, "cu_tokens", torch.int32, 1, device), _dense(kv_lens, "kv_lens", torch.int32, 1, device),
+             _dense(tables, "tables", torch.int32, 2, device))
+    tiles, items = tile_item.numel(), kv_lens.numel()
+    rows, width = tables.shape
+    if tile_q0.numel() != tiles or cu_tokens.numel() != items + 1 or rows != items:
+        raise KernelError(f"{what}: inconsistent tile or item arrays")
+    sink_at = 0
+    if sink is not None:
+        sink_at = _check_sink(sink, heads)
+        _dense(sink, "sink", torch.float32, 1, device)
+    addresses = (q_rows[0], q_rows[1], k_at, v_at, out_rows[0], out_rows[1], index[0], index[1], tiles, index[2], index[3],
+                 index[4], width)
+    return addresses, (heads, kv_heads, head_dim, page_size, pages), sink_at, device
+
+
 def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_lens, tables, heads, scale,
                            window=0, max_kv_len=0, query_tile=PREFILL_TILE, sink=None, softcap=0.0, block_heads=None, ranges=None, partial=None):
     """``attention_prefill`` over a cache in 4 bits (bfloat16 queries, head sizes in multiples of 16).
@@ -1536,24 +1563,10 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
     every tile, joined by a second launch (None: ``prefill_int4_ranges(...)``, one where ``max_kv_len`` is not given); with more than one ``partial`` is float scratch of
     ``tiles * heads * ranges * query_tile * (head_dim + 2)`` values, allocated for the call where it is None."""
     _check_prefill_constants()
-    _, device = _first("attention_prefill_int4", q, "q")
-    q_at, q_stride = _rows_on(q, "q", torch.bfloat16, device)
-    out_at, out_stride = _rows_on(out, "out", torch.bfloat16, device)
-    shape = _, columns = q.shape
-    k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, columns, heads, device)
-    if out.shape != shape:
-        raise KernelError("attention_prefill_int4: q and out rows must hold heads x head_dim values")
-    index = (_dense(tile_item, "tile_item", torch.int32, 1, device), _dense(tile_q0, "tile_q0", torch.int32, 1, device),
-             _dense(cu_tokens, "cu_tokens", torch.int32, 1, device), _dense(kv_lens, "kv_lens", torch.int32, 1, device))
-    tables_at = _dense(tables, "tables", torch.int32, 2, device)
-    tiles, items = tile_item.numel(), kv_lens.numel()
-    table_rows, table_width = tables.shape
-    if tile_q0.numel() != tiles or cu_tokens.numel() != items + 1 or table_rows != items:
-        raise KernelError("attention_prefill_int4: inconsistent tile or item arrays")
-    sink_at = 0
-    if sink is not None:
-        sink_at = _check_sink(sink, heads)
-        _dense(sink, "sink", torch.float32, 1, device)
+    addresses, sizes, sink_at, device = _int4_tiles("attention_prefill_int4", q, k_pool, v_pool, out, tile_item, tile_q0,
+                                                    cu_tokens, kv_lens, tables, heads, sink, torch.bfloat16)
+    _, kv_heads, head_dim, _, _ = sizes
+    tiles = addresses[8]
     max_kv_len, query_tile = int(max_kv_len), int(query_tile)
     if block_heads is None:
         block_heads = prefill_int4_block_heads(tiles, heads, kv_heads, head_dim, query_tile)
@@ -1566,10 +1579,18 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
         if partial is None:
             partial = torch.empty(tiles * heads * ranges * query_tile * (head_dim + 2), dtype=torch.float32, device=q.device)
         partial_at, floats = _dense(partial, "partial", torch.float32, None, device), partial.numel()
-    _call("ps_attention_prefill_int4", q_at, q_stride, k_at, v_at, out_at, out_stride, index[0], index[1], tiles, index[2],
-          index[3], tables_at, table_width, heads, kv_heads, head_dim, page_size, pages, float(scale),
-          int(window), max_kv_len, query_tile, sink_at, _check_cap(softcap), int(block_heads), int(ranges),
-          partial_at, floats, _stream())
+    _call("ps_attention_prefill_int4", *addresses, *sizes, float(scale), int(window), max_kv_len, query_tile, sink_at,
+          _check_cap(softcap), int(block_heads), int(ranges), partial_at, floats, _stream())
+    return out
+
+
+def attention_tiled_f32_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_lens, tables, heads, scale,
+                             window=0, sink=None, softcap=0.0, query_tile=PREFILL_TILE, paired=False):
+    """``attention_tiled_f32`` over a cache in 4 bits (``tiled_f32_supported``, ``tiled_f32_shape``)."""
+    addresses, sizes, sink_at, _ = _int4_tiles("attention_tiled_f32_int4", q, k_pool, v_pool, out, tile_item, tile_q0,
+                                               cu_tokens, kv_lens, tables, heads, sink, torch.float32)
+    _call("ps_attention_tiled_f32_int4", *addresses, *sizes, float(scale), int(window), sink_at, _check_cap(softcap),
+          int(query_tile), int(paired), _stream())
     return out
 
 

@@ -409,6 +409,12 @@ class Attention(Mixer):
                                            self.heads, self.scale, window=self.span, max_kv_len=ctx.max_kv_len,
                                            query_tile=size, sink=self.sink, softcap=self.score_cap, block_heads=pair,
                                            ranges=ranges, partial=self._int4_tile_records(ctx) if ranges > 1 else None)
+        elif singles < tokens and kernels.tiled_f32_supported(self.dtype, self.head_dim):
+            size, paired = kernels.tiled_f32_shape(self.heads, self.head_dim, ctx.query_tiles[kernels.PREFILL_TILE][0].numel(),
+                                                   ctx.query_tiles[kernels.PREFILL_SMALL_TILE][0].numel(), ctx.max_kv_len)
+            kernels.attention_tiled_f32_int4(q, cache.k_pool, cache.v_pool, context, *ctx.query_tiles[size], ctx.cu_tokens,
+                                             ctx.kv_lens, tables, self.heads, self.scale, window=self.span, sink=self.sink,
+                                             softcap=self.score_cap, query_tile=size, paired=paired)
         elif singles < tokens:
             kernels.attention_decode_int4(q, cache.k_pool, cache.v_pool, context, ctx.tok_item, ctx.positions, tables,
                                           self.heads, self.scale, 1, window=self.span, tok_list=ctx.portion_tokens,

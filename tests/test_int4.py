@@ -60,6 +60,12 @@ def _prompt(**changed):
     return args
 
 
+def _float_prompt(**changed):
+    args = _prompt(q=torch.zeros(3, 256), out=torch.zeros(3, 256))
+    args.update(changed)
+    return args
+
+
 def _logprobs(**changed):
     args = dict(logits=torch.zeros(3, 50), tokens=_ints(3), out=torch.zeros(3))
     args.update(changed)
@@ -72,8 +78,9 @@ def test_what_they_take(on_gpu):
     kernels.attention_decode_int4(**_decode())
     kernels.attention_prefill_int4(**_prompt())
     kernels.token_logprobs(**_logprobs())
+    kernels.attention_tiled_f32_int4(**_float_prompt())
     assert on_gpu == ["ps_kv_write_int4", "ps_kv_read_int4", "ps_attention_decode_int4", "ps_attention_prefill_int4",
-                      "ps_token_logprobs"]
+                      "ps_token_logprobs", "ps_attention_tiled_f32_int4"]
 
 
 @pytest.mark.parametrize("changed,message", [
@@ -104,6 +111,7 @@ def test_tensors_on_two_devices(on_gpu):
                            (kernels.attention_decode_int4, _decode(tok_list=_ints(2), sink=torch.zeros(4), splits=2,
                                                                    partial=torch.zeros(4000))),
                            (kernels.attention_prefill_int4, _prompt(sink=torch.zeros(4), ranges=2, partial=torch.zeros(9))),
+                           (kernels.attention_tiled_f32_int4, _float_prompt(sink=torch.zeros(4))),
                            (kernels.token_logprobs, _logprobs(entropy=torch.zeros(3), ranks=_ints(3), top_ids=_ints(3, 2),
                                                               top_logprobs=torch.zeros(3, 2), partial=torch.zeros(9)))):
         names = [name for name, value in args.items() if isinstance(value, torch.Tensor)]
@@ -218,6 +226,34 @@ def test_prompt_refused_by_the_library(changed, message):
     assert status == 1 and message in error
     status, error = _c("ps_attention_prefill_int4", 0, 252, 0, 0, 0, 256, 0, 0, 1, 0, 0, 0, *PORTIONS.values(), 0, 0, 0)
     assert status == 1 and "accesses" in error
+
+
+@pytest.mark.parametrize("changed,message", [
+    ({"q": torch.zeros(3, 256, dtype=BF16), "out": torch.zeros(3, 256, dtype=BF16)}, "float32"), ({"heads": 3}, "do not fit"),
+    ({"out": torch.zeros(3, 128)}, "rows must hold"), ({"tile_q0": _ints(2)}, "inconsistent"), ({"cu_tokens": _ints(3)}, "inconsistent"),
+    ({"tables": _ints(2, 5)}, "inconsistent"), ({"kv_lens": _ints(4)[::2], "cu_tokens": _ints(3), "tables": _ints(2, 5)}, "contiguous"),
+    ({"tile_item": _ints(1).long()}, "int32"), ({"sink": torch.zeros(5)}, "one float per head"), ({"softcap": -1.0}, "score cap")])
+def test_float_prompt_refused(on_gpu, changed, message):
+    with pytest.raises(kernels.KernelError, match=message):
+        kernels.attention_tiled_f32_int4(**_float_prompt(**changed))
+    assert not on_gpu
+
+
+FLOATS = dict(table_width=5, heads=4, kv_heads=2, head_dim=64, page_size=16, num_pages=4, scale=0.125, window=0, sink=0, softcap=0.0,
+              query_tile=64, paired=0)
+
+
+@pytest.mark.parametrize("changed,message", [
+    ({"heads": 5}, "multiple of kv_heads"), ({"head_dim": 66}, "multiple of 4"), ({"head_dim": 132}, "up to 128"),
+    ({"page_size": 20}, "multiple of 8"), ({"query_tile": 128}, "queries"), ({"query_tile": 32, "paired": 1}, "queries"),
+    ({"scale": 0.0}, "positive"), ({"table_width": 0}, "bad sizes")])
+def test_float_prompt_refused_by_the_library(changed, message):
+    sizes = dict(FLOATS, **changed)
+    status, error = _c("ps_attention_tiled_f32_int4", 0, 256, 0, 0, 0, 256, 0, 0, 1, 0, 0, 0, *sizes.values(), 0)
+    assert status == 1 and message in error
+    status, error = _c("ps_attention_tiled_f32_int4", 0, 254, 0, 0, 0, 256, 0, 0, 1, 0, 0, 0, *FLOATS.values(), 0)
+    assert status == 1 and "accesses" in error
+    assert _c("ps_attention_tiled_f32_int4", 0, 256, 0, 0, 0, 256, 0, 0, 0, 0, 0, 0, *FLOATS.values(), 0)[0] == 0
 
 
 @pytest.mark.parametrize("args,message", [

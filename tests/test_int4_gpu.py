@@ -348,6 +348,62 @@ def test_prompt_portions(kv_heads, group, dim, page, counts, starts, window, sin
     assert bool(((out.double().cpu() - expected[0]).abs() <= limit).all())
 
 
+FLOAT = [
+    # kv_heads, group, dim, page, counts, starts, window, sink, softcap
+    (3, 1, 64, 16, (65, 130), (0, 0), 0, False, 0.0), (2, 4, 128, 16, (33, 70, 2), (100, 0, 31), 0, False, 0.0),
+    (1, 2, 16, 8, (40,), (3,), 0, True, 0.0), (2, 1, 48, 24, (100, 20), (0, 50), 0, False, 30.0),
+    (1, 3, 96, 16, (64,), (10,), 40, False, 0.0), (1, 2, 80, 8, (35,), (5,), -16, False, 0.0), (1, 2, 20, 8, (50, 3), (0, 61), 0, False, 0.0),
+    (2, 1, 32, 8, (129,), (200,), 0, True, 0.0), (1, 1, 124, 40, (60,), (8,), 25, False, 20.0), (1, 1, 4, 8, (33,), (1,), 0, False, 0.0)]
+
+
+@pytest.mark.parametrize("kv_heads,group,dim,page,counts,starts,window,sink,softcap", FLOAT)
+def test_prompt_portions_in_float(kv_heads, group, dim, page, counts, starts, window, sink, softcap):
+    """Float queries, in every form of tile; the row behind the last token stays."""
+    from pagedserve_amd.ops import kernels
+
+    heads = kv_heads * group
+    tables, pages, _, positions = _requests(counts, starts, page, 47)
+    lengths = [a + b for a, b in zip(counts, starts)]
+    pools, kept = _cache(tables, pages, lengths, kv_heads, dim, page, 48)
+    tokens = sum(counts)
+    g = torch.Generator().manual_seed(49)
+    q = torch.randn((tokens, heads * dim), generator=g) * 1.5
+    sinks = torch.randn(heads, generator=g).cuda() if sink else None
+    cu = [sum(counts[:i]) for i in range(len(counts) + 1)]
+    parts = [list(plain.attention(q[cu[i]:cu[i + 1]], *kept[i], positions[cu[i]:cu[i + 1]], heads, dim ** -0.5, window, sinks,
+                                  softcap)) for i in range(len(counts))]
+    expected = [torch.cat([part[which] for part in parts]) for which in range(3)]
+    limit = plain.allowed(*expected, F32, False)
+    for size, paired in ((32, False), (64, False), (64, True)):
+        tiles = [(item, q0) for item, count in enumerate(counts) for q0 in range(0, count, size)]
+        out = torch.full((tokens + 1, heads * dim), -9.0).cuda()
+        kernels.attention_tiled_f32_int4(q.cuda(), *pools, out[:tokens], _ints([t[0] for t in tiles]),
+                                         _ints([t[1] for t in tiles]), _ints(cu), _ints(lengths), tables.cuda(), heads,
+                                         dim ** -0.5, window, sinks, softcap, size, paired)
+        assert bool(((out[:tokens].double().cpu() - expected[0]).abs() <= limit).all()), (size, paired)
+        assert bool((out[tokens] == -9.0).all())
+
+
+@pytest.mark.parametrize("bad", ["key", "value"])
+def test_a_later_nan_reaches_no_earlier_float_query(bad):
+    from pagedserve_amd.ops import kernels
+
+    tables, pages, _, positions = _requests((40,), (100,), 8, 54)
+    (k_pool, v_pool), kept = _cache(tables, pages, (140,), 1, 64, 8, 55)
+    rows = [torch.zeros(2, 64), torch.zeros(2, 64)]
+    rows[bad == "value"][:, 5] = math.nan
+    kernels.kv_write_int4(rows[0].cuda(), rows[1].cuda(), k_pool, v_pool, _ints([0, 0]), _ints([139, 110]), tables.cuda())
+    q = torch.randn((40, 64), generator=torch.Generator().manual_seed(56))
+    expected = list(plain.attention(q[:10], kept[0][0][:110], kept[0][1][:110], positions[:10], 1, 0.125))
+    for size, paired in ((32, False), (64, False), (64, True)):
+        tiles = list(range(0, 40, size))
+        out = torch.zeros(40, 64).cuda()
+        kernels.attention_tiled_f32_int4(q.cuda(), k_pool, v_pool, out, _ints([0] * len(tiles)), _ints(tiles), _ints([0, 40]),
+                                         _ints([140]), tables.cuda(), 1, 0.125, query_tile=size, paired=paired)
+        assert bool(((out[:10].double().cpu() - expected[0]).abs() <= plain.allowed(*expected, F32, False)).all())
+        assert bool(out[10:].isnan().any(1).all())
+
+
 LONG = [
     # kv_heads, group, dim, page, counts, starts, window, sink, softcap, query_tile
     (2, 2, 64, 16, (70, 3), (1500, 40), 0, True, 0.0, 64), (1, 4, 64, 24, (130,), (900,), 300, False, 0.0, 128),
