@@ -38,6 +38,7 @@ typedef uint32_t int4_u32x4 __attribute__((ext_vector_type(4)));
 #define I4_TILE 32           // keys of a wave at a time
 #define I4_HEADS 16          // heads of a block, at most
 #define I4_OFFSET 24.f       // what a code is held as, less what it stands for
+#define I4_OWN 80            // words for a token's own rows: 8 of codes and 1 of steps to a group, up to a multiple of 64 bytes
 #define I4_SLACK 8.f         // how far (in units of log 2) a score may pass the exponentials' reference
 
 // Reads from LDS, at constant distances from an address, that have arrived when they return.  (Written as assembly: the
@@ -130,20 +131,28 @@ struct Int4Decode {
   int table_width, heads, kv_heads, parts, block_heads, head_dim, page_size, page_shift, num_pages, window, splits, wide_q;
   float scale_log2, softcap_log2;
   const float* sink;
+  const bf16_t* new_k;         // the tokens' own rows, stored first (STORES)
+  const bf16_t* new_v;
+  int64_t new_k_stride, new_v_stride;
 };
 
 // EVEN: pages of a power of two, 16 or more: 16 keys from a multiple of 16 on lie in one page (else 8 from a multiple of 8), whose
 // place the scalar unit works out for the wave.
-// dynamic LDS: the waves' maxima and sums [WAVES][16] each, the block's maxima [16], then the waves' pairs of tiles, in
+// STORES: a token's own key and value are stored first.  The wave whose tile holds them works out their codes, which go to LDS,
+// from where they replace what that tile's loads have found in their place, and at the end to the page, for later calls.
+//
+// dynamic LDS: the waves' maxima and sums [WAVES][16] each, the block's maxima [16], the token's own rows, then the waves' pairs of tiles, in
 // whose place the accumulators [WAVES][heads of the block][32 G] meet at the end
-template <int G, int WAVES, bool EVEN>
-__global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel(const Int4Decode a) {
+// (of heads up to 64 five waves fit a unit's SIMD with 96 registers, two less than the form that stores takes by itself)
+template <int G, int WAVES, bool EVEN, bool STORES>
+__global__ __launch_bounds__(64 * WAVES, G == 2 && EVEN ? 5 : 1) void attention_decode_int4_heads_kernel(const Int4Decode a) {
   typedef Int4Stage<G> Stage;
   extern __shared__ __attribute__((aligned(1024))) float lds[];
   float* s_m = lds;
   float* s_l = lds + WAVES * I4_HEADS;
   float* s_block = lds + 2 * WAVES * I4_HEADS;
-  float* s_acc = s_block + I4_HEADS;
+  uint32_t* s_own = reinterpret_cast<uint32_t*>(s_block + I4_HEADS);      // codes of key and value, then their steps
+  float* s_acc = s_block + I4_HEADS + I4_OWN;
   unsigned char* stages = reinterpret_cast<unsigned char*>(s_acc);      // (the accumulators come when no tile is left)
   const int index = blockIdx.x, split = blockIdx.z;
   const int kv_head = blockIdx.y / a.parts, part = blockIdx.y - kv_head * a.parts;
@@ -190,6 +199,21 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
     chunk = (chunk + I4_TILE * WAVES - 1) / (I4_TILE * WAVES) * (I4_TILE * WAVES);
     begin += split * chunk;
     if (begin + chunk < end) end = begin + chunk;
+  }
+
+  // the token's own rows, by the wave whose tile holds them: 8 dimensions to a lane, of the key and then of the value
+  const bool own = STORES && pos >= begin && pos < end;
+  const bool mine = own && wave == (pos - begin) / I4_TILE % WAVES;
+  float row[1][8];
+  if (STORES && mine && lane < 8 * G) {
+    const bool is_value = lane >= 4 * G;
+    const bf16_t* from = (is_value ? a.new_v + t * a.new_v_stride : a.new_k + t * a.new_k_stride) + (int64_t)kv_head * a.head_dim;
+    const int d0 = 8 * (lane % (4 * G));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float value = to_float(from[d0 + i < a.head_dim ? d0 + i : a.head_dim - 1]);
+      row[0][i] = d0 + i < a.head_dim ? value : 0.f;
+    }
   }
 
   // the pages of a tile's units of 8 (EVEN: 16) keys, and which of them exist
@@ -279,6 +303,20 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
   if (base < end) {
     entries = ask(base);
     send(0);
+  }
+
+  if (STORES && mine && lane < 8 * G) {
+    uint32_t word[1], step[1];
+    int4_code_row<1, true>(row, false, word, step);            // (a group to four lanes)
+    const int g = lane % (4 * G) / 4, quarter = lane & 3;
+    unsigned char* at = reinterpret_cast<unsigned char*>(s_own);
+    if (lane < 4 * G) {
+      s_own[quarter * G + g] = word[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) at[16 * G + (4 * quarter + i) * G + g] = (unsigned char)(word[0] >> (8 * i));
+    }
+    if (quarter == 0) reinterpret_cast<uint16_t*>(at + 32 * G)[lane / 4] = (uint16_t)step[0];
   }
 
   // the queries, column n of the products: dimensions 32 g + 8 c + (0, 4, 1, 5, ..), the order of a word's nibbles
@@ -409,6 +447,17 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
     const unsigned units = exist & 15u;
     const bool whole = base >= first && base + I4_TILE <= end && units == (1u << UNITS) - 1;
     const uint32_t stage = pair_at + slot * Stage::BYTES;
+    if (STORES && own && base <= pos && pos < base + I4_TILE) {
+      unsigned char* at = pair + slot * Stage::BYTES;
+      const int within = pos - base;
+      int lane = threadIdx.x & 63;
+      asm volatile("" : "+v"(lane));       // (worked out here, once: kept through the loop it takes a register too many)
+      if (lane < 8 * G)
+        reinterpret_cast<uint32_t*>(at + (lane >= 4 * G ? Stage::CODES : 0) + within * (16 * G))[lane % (4 * G)] = s_own[lane];
+      if (lane < 2 * G)
+        reinterpret_cast<uint16_t*>(at + 2 * Stage::CODES + (lane >= G ? Stage::STEPS : 0) + within * (2 * G))[lane % G] =
+            reinterpret_cast<const uint16_t*>(s_own + 8 * G)[lane];
+    }
     float s[8];
     score(s, stage);
     if (a.softcap_log2 > 0.f) {
@@ -482,6 +531,20 @@ __global__ __launch_bounds__(64 * WAVES) void attention_decode_int4_heads_kernel
       record[a.head_dim + 1] = total;
     }
   }
+  if (STORES && mine) {
+    // the codes to their page (here, where nothing waits for that)
+    const int logical = logical_of(pos), within = pos - logical * a.page_size;
+    const int page = scalar_load(table + logical);
+    if ((unsigned)page < (unsigned)a.num_pages) {
+      const int64_t at = int4_page_at(page, a.kv_heads, kv_head, a.page_size, G);
+      if (lane < 8 * G)
+        reinterpret_cast<uint32_t*>((uint8_t*)(lane >= 4 * G ? a.v_pool : a.k_pool) + at + within * (16 * G))[lane % (4 * G)] =
+            s_own[lane];
+      if (lane < 2 * G)
+        reinterpret_cast<uint16_t*>((uint8_t*)(lane >= G ? a.v_pool : a.k_pool) + at + a.page_size * (16 * G) +
+                                    within * (2 * G))[lane % G] = reinterpret_cast<const uint16_t*>(s_own + 8 * G)[lane];
+    }
+  }
 }
 
 // (beyond the 64 KB that a kernel may ask for without saying so)
@@ -497,12 +560,17 @@ static void launch_heads(const Int4Decode& a, int count, int waves, hipStream_t 
   // 1,024 keys 32.7 us with two, 34.0 with three and 36.4 with four, 128 of 12 over 1,000 29.7, 32.0 and 33.2; 64 of 32 heads
   // of 128 over 8 and 1,500 keys 28.8 with two, 32 with three; 48 of 20 heads of 96 over 2,000 53 and 63.)
   const int pairs = waves * 2 * Int4Stage<G>::BYTES, meet = waves * a.block_heads * 32 * G * 4;
-  const int bytes = (I4_HEADS + waves * 2 * I4_HEADS) * 4 + (pairs > meet ? pairs : meet);
+  const int bytes = (I4_HEADS + waves * 2 * I4_HEADS + I4_OWN) * 4 + (pairs > meet ? pairs : meet);
   const bool even = a.page_size >= 16 && a.page_shift >= 0;
-#define PS_LAUNCH_H4E(WAVES, EVEN)                                                                              \
-  do {                                                                                                          \
-    int4_allow_lds(reinterpret_cast<const void*>(attention_decode_int4_heads_kernel<G, WAVES, EVEN>), bytes); \
-    hipLaunchKernelGGL((attention_decode_int4_heads_kernel<G, WAVES, EVEN>), grid, dim3(64 * WAVES), bytes, s, a); \
+#define PS_LAUNCH_H4S(WAVES, EVEN, STORES)                                                                          \
+  do {                                                                                                              \
+    int4_allow_lds(reinterpret_cast<const void*>(attention_decode_int4_heads_kernel<G, WAVES, EVEN, STORES>), bytes); \
+    hipLaunchKernelGGL((attention_decode_int4_heads_kernel<G, WAVES, EVEN, STORES>), grid, dim3(64 * WAVES), bytes, s, a); \
+  } while (0)
+#define PS_LAUNCH_H4E(WAVES, EVEN)                                  \
+  do {                                                              \
+    if (a.new_k != nullptr) PS_LAUNCH_H4S(WAVES, EVEN, true);       \
+    else PS_LAUNCH_H4S(WAVES, EVEN, false);                         \
   } while (0)
 #define PS_LAUNCH_H4(WAVES)                \
   do {                                     \
@@ -516,6 +584,7 @@ static void launch_heads(const Int4Decode& a, int count, int waves, hipStream_t 
     }
   }
   PS_LAUNCH_H4(4);
+#undef PS_LAUNCH_H4S
 #undef PS_LAUNCH_H4E
 #undef PS_LAUNCH_H4
 }
@@ -720,11 +789,12 @@ __global__ __launch_bounds__(64) void attention_decode_int4_merge_kernel(const f
   }
 }
 
-extern "C" int ps_attention_decode_int4(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool,
-                                        void* out, int64_t out_stride, float* partial, int64_t partial_floats,
-                                        const int* tok_list, const int* tok_item, const int* tok_pos,
-                                        const int* tables, int table_width, int count, int heads, int kv_heads,
-                                        int head_dim, int page_size, int num_pages, float scale, int window,
+extern "C" int ps_attention_decode_int4(const void* q, int64_t q_stride, const void* new_k, const void* new_v,
+                                        int64_t new_k_stride, int64_t new_v_stride, const void* k_pool,
+                                        const void* v_pool, void* out, int64_t out_stride, float* partial,
+                                        int64_t partial_floats, const int* tok_list, const int* tok_item,
+                                        const int* tok_pos, const int* tables, int table_width, int count, int heads,
+                                        int kv_heads, int head_dim, int page_size, int num_pages, float scale, int window,
                                         int splits, const float* sink, float softcap, int dtype, void* stream) {
   PS_REQUIRE(count >= 0 && heads > 0 && kv_heads > 0 && page_size > 0 && num_pages > 0 && table_width > 0,
              "ps_attention_decode_int4: bad sizes");
@@ -741,6 +811,8 @@ extern "C" int ps_attention_decode_int4(const void* q, int64_t q_stride, const v
                              partial_floats >= (int64_t)count * heads * splits * (head_dim + 2)),
              "ps_attention_decode_int4: %lld floats of scratch are too few for %d ranges", (long long)partial_floats,
              splits);
+  PS_REQUIRE((new_k == nullptr) == (new_v == nullptr) && (new_k == nullptr || (dtype == PS_BF16 && scale > 0.f && tok_item == nullptr && tok_list == nullptr)),
+             "ps_attention_decode_int4: rows to be stored are keys and values in bfloat16, a request's to a token, under a positive scale");
   if (count == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid(count, heads, splits);
@@ -770,7 +842,8 @@ extern "C" int ps_attention_decode_int4(const void* q, int64_t q_stride, const v
     const Int4Decode a{(const bf16_t*)q, q_stride, (const uint8_t*)k_pool, (const uint8_t*)v_pool, (bf16_t*)out, out_stride,
                        partial, tok_list, tok_item, tok_pos, tables, table_width, heads, kv_heads,
                        (kv_group + block_heads - 1) / block_heads, block_heads, head_dim, page_size, page_shift, num_pages, window, splits,
-                       wide_q, scale * 1.4426950408889634f, softcap * 1.4426950408889634f, sink};
+                       wide_q, scale * 1.4426950408889634f, softcap * 1.4426950408889634f, sink,
+                       (const bf16_t*)new_k, (const bf16_t*)new_v, new_k_stride, new_v_stride};
     const int64_t blocks = (int64_t)count * kv_heads * a.parts;
     int waves = splits == 1 && blocks <= ps_compute_units() && groups <= 4 && block_heads * groups <= 32 ? 8 : 4;
     switch (groups) {

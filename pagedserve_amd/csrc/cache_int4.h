@@ -85,3 +85,115 @@ __device__ inline void int4_codes(const float* x, float step, float* codes) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) codes[i] = fminf(fmaxf(codes[i], -8.f), 7.f);
 }
+
+// The quarter of a value's row holds byte i of group g's word as its byte i G + g: from the words of the groups, and back.
+template <int G, bool BACK>
+__device__ inline void int4_turn_bytes(uint32_t* words) {
+  uint32_t turned[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) turned[g] = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int at = i * G + g;
+      if (BACK) turned[g] |= (words[at / 4] >> (8 * (at % 4)) & 0xffu) << (8 * i);
+      else turned[at / 4] |= (words[g] >> (8 * i) & 0xffu) << (8 * (at % 4));
+    }
+#pragma unroll
+  for (int g = 0; g < G; ++g) words[g] = turned[g];
+}
+
+// N words from or to an address that is a multiple of the largest power of two in 4 N bytes, 16 at most.
+template <int N>
+__device__ inline void int4_load_words(const uint8_t* from, uint32_t* words) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(from)[i];
+      words[4 * i] = v.x;
+      words[4 * i + 1] = v.y;
+      words[4 * i + 2] = v.z;
+      words[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 v = reinterpret_cast<const uint2*>(from)[i];
+      words[2 * i] = v.x;
+      words[2 * i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) words[i] = reinterpret_cast<const uint32_t*>(from)[i];
+  }
+}
+template <int N>
+__device__ inline void int4_store_words(uint8_t* to, const uint32_t* words) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      reinterpret_cast<uint4*>(to)[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) reinterpret_cast<uint2*>(to)[i] = make_uint2(words[2 * i], words[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) reinterpret_cast<uint32_t*>(to)[i] = words[i];
+  }
+}
+
+// What lane c of four that share a row holds of it: the words of its codes in the page's order and the row's steps (the
+// lane's 8 dimensions of each group in x; BF16: numbers of 8 bits).
+template <int G, bool BF16>
+__device__ inline void int4_code_row(const float (&x)[G][8], bool values, uint32_t (&words)[G],
+                                     uint32_t (&steps)[(G + 1) / 2]) {
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    float high = x[g][0], low = x[g][0], finite = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      high = fmaxf(high, x[g][i]);
+      low = fminf(low, x[g][i]);
+      finite = fmaf(x[g][i], 0.f, finite);                   // (NaN by an infinity or a NaN, which an extreme passes over)
+    }
+    high = lanes_max<4>(high);
+    low = -lanes_max<4>(-low);
+    const bool all_finite = lanes_max<4>(finite == 0.f ? 0.f : 1.f) == 0.f;
+    const float step = all_finite ? int4_step(high, low) : __uint_as_float(0x7fc00000u);
+    words[g] = 0x88888888u;
+    if (all_finite && step != 0.f) {
+      float codes[8];
+      int4_codes<BF16>(x[g], step, codes);
+      uint32_t halves[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // four codes less 8 as the digits of a number to the base of 16, and 8 to each
+        float digits = 0.f;
+#pragma unroll
+        for (int i = 3; i >= 0; --i) digits = fmaf(digits, 16.f, codes[4 * h + i]);
+        halves[h] = (uint32_t)(digits + 34952.f);
+      }
+      words[g] = halves[0] | halves[1] << 16;
+    }
+    const uint32_t bits = __float_as_uint(step) >> 16;
+    steps[g / 2] = g % 2 ? steps[g / 2] | bits << 16 : bits;
+  }
+  if (values) int4_turn_bytes<G, false>(words);
+}
+
+// That into place `within` of a page.
+template <int G>
+__device__ inline void int4_store_row(uint8_t* page, int page_size, int within, int c, const uint32_t (&words)[G],
+                                      const uint32_t (&steps)[(G + 1) / 2]) {
+  int4_store_words<G>(page + within * (16 * G) + c * (4 * G), words);
+  if (c == 0) {
+    uint8_t* to = page + page_size * (16 * G) + within * (2 * G);
+    if constexpr (G % 2 == 0) {
+      int4_store_words<G / 2>(to, steps);
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g) reinterpret_cast<uint16_t*>(to)[g] = (uint16_t)(steps[g / 2] >> (16 * (g % 2)));
+    }
+  }
+}

@@ -301,8 +301,11 @@ int ps_kv_read_int4(const void* k_pool, const void* v_pool, void* k, void* v, in
                     int table_width, int tokens, int kv_heads, int head_dim, int page_size,
                     int num_pages, int dtype, void* stream);
 // ps_attention_decode over such a cache (q and out of `dtype`; no gate, no logistic weights): `partial` is scratch of
-// count * heads * splits * (head_dim + 2) floats, unused with one range.  A token that sees nothing gets zeros.
-int ps_attention_decode_int4(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool,
+// count * heads * splits * (head_dim + 2) floats, unused with one range.  A token that sees nothing gets zeros.  new_k, new_v:
+// null, or the tokens' own rows of keys and values (bfloat16, by token number), stored first as ps_kv_write_int4 does (without tok_item and
+// tok_list: no token sees what another one stores).
+int ps_attention_decode_int4(const void* q, int64_t q_stride, const void* new_k, const void* new_v,
+                             int64_t new_k_stride, int64_t new_v_stride, const void* k_pool, const void* v_pool,
                              void* out, int64_t out_stride, float* partial, int64_t partial_floats,
                              const int* tok_list, const int* tok_item, const int* tok_pos,
                              const int* tables, int table_width, int count, int heads, int kv_heads,

@@ -376,7 +376,7 @@ class Attention(Mixer):
         return q
 
     def _forward_int4(self, x, residual, ctx, cache, tables):
-        """The same layer over a cache in 4 bits: one launch more, which stores the step's keys and values as codes."""
+        """The same layer over a cache in 4 bits.  Prompt portions take one launch more, which stores the step's keys and values."""
         if self.prepared:
             raise NotImplementedError("attention with prepared queries and keys takes no cache in 4 bits")
         tokens = ctx.tokens
@@ -386,10 +386,12 @@ class Attention(Mixer):
                        memo=site_memo(self._memo_qkv, ctx.workspace), shared=ctx.shared_calls)
         if self.position is not None and self.position.transforms_qk:
             self.position.apply_to_qk(q, k, ctx)
-        if cache.writes:
-            kernels.kv_write_int4(k, v, cache.k_pool, cache.v_pool, ctx.tok_item, ctx.positions, tables)
         context = ctx.workspace.first_rows("attn", self.q_cols, self.dtype, tokens)
         singles = ctx.single_tokens.numel() if ctx.single_tokens is not None else 0
+        # a decode step's attention stores its tokens' rows itself
+        store = (k, v) if cache.writes and singles == tokens and self.dtype == torch.bfloat16 and self.scale > 0 else None
+        if cache.writes and store is None:
+            kernels.kv_write_int4(k, v, cache.k_pool, cache.v_pool, ctx.tok_item, ctx.positions, tables)
         if singles:
             splits = kernels.int4_decode_splits(self.dtype, singles, self.heads, self.kv_heads, self.head_dim,
                                                 self._visible(ctx.max_kv_len))
@@ -397,7 +399,7 @@ class Attention(Mixer):
                                           ctx.positions, tables, self.heads, self.scale, splits,
                                           partial=self._int4_records(ctx) if splits > 1 else None, window=self.span,
                                           tok_list=None if singles == tokens else ctx.single_tokens, sink=self.sink,
-                                          softcap=self.score_cap)
+                                          softcap=self.score_cap, store=store)
         if singles < tokens and kernels.prefill_int4_supported(self.dtype, self.head_dim, tables.shape[1]):
             size = kernels.prefill_int4_tile(self.heads, self.head_dim,
                                              {size: lists[0].numel() for size, lists in ctx.query_tiles.items()},

@@ -139,7 +139,13 @@ def test_tensors_that_are_not_on_the_current_device(on_gpu):
     ({"splits": 2, "partial": torch.zeros(9, dtype=BF16)}, "partial"), ({"splits": 2, "partial": torch.zeros(9, 2)[:, 0]}, "contiguous"),
     ({"tok_item": None}, "row per token"), ({"tok_list": _ints(3).long()}, "int32"), ({"tok_list": _ints(6)[::2]}, "contiguous"),
     ({"sink": torch.zeros(3)}, "one float per head"), ({"softcap": -1.0}, "score cap"), ({"softcap": float("inf")}, "score cap"),
-    ({"k_pool": _pools(dim=128)[0], "v_pool": _pools(dim=128)[0]}, "do not fit")])
+    ({"k_pool": _pools(dim=128)[0], "v_pool": _pools(dim=128)[0]}, "do not fit"),
+    ({"store": (torch.zeros(3, 128), torch.zeros(3, 128))}, "bfloat16"), ({"store": (torch.zeros(2, 128, dtype=BF16),) * 2}, "stored are"),
+    ({"store": (torch.zeros(3, 64, dtype=BF16),) * 2}, "stored are"), ({"store": (torch.zeros(3, 128, dtype=BF16),) * 2, "scale": -1.0, "tok_item": None}, "row per token"),
+    ({"store": (torch.zeros(3, 128, dtype=BF16),) * 2}, "stored are"),
+    ({"store": (torch.zeros(3, 128, dtype=BF16),) * 2, "tok_item": None, "tables": _ints(3, 5), "scale": -1.0}, "stored are"),
+    ({"store": (torch.zeros(3, 128, dtype=BF16),) * 2, "tok_item": None, "tables": _ints(3, 5), "tok_list": _ints(3)}, "stored are"),
+    ({"store": (torch.zeros(3, 128, dtype=BF16), torch.zeros(2, 128, dtype=BF16))}, "stored are")])
 def test_decode_refused(on_gpu, changed, message):
     with pytest.raises(kernels.KernelError, match=message):
         kernels.attention_decode_int4(**_decode(**changed))
@@ -205,7 +211,7 @@ ATTEND = dict(table_width=5, count=3, heads=4, kv_heads=2, head_dim=64, page_siz
     ({"table_width": 1 << 26}, "block tables")])
 def test_decode_refused_by_the_library(changed, message):
     sizes = dict(ATTEND, **changed)
-    status, error = _c("ps_attention_decode_int4", 0, 256, 0, 0, 0, 256, 0, 0, 0, 0, 0, 0, *sizes.values(), 0, 0.0, 1, 0)
+    status, error = _c("ps_attention_decode_int4", 0, 256, 0, 0, 0, 0, 0, 0, 0, 256, 0, 0, 0, 0, 0, 0, *sizes.values(), 0, 0.0, 1, 0)
     assert status == 1 and message in error
 
 
@@ -271,7 +277,7 @@ def test_nothing_to_do_is_no_launch():
     assert _c("ps_kv_write_int4", 0, 0, 128, 128, 0, 0, 0, 0, 0, *sizes.values(), 0)[0] == 0
     assert _c("ps_token_logprobs", 0, 50, 0, 50, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)[0] == 0
     sizes = dict(ATTEND, count=0)
-    assert _c("ps_attention_decode_int4", 0, 256, 0, 0, 0, 256, 0, 0, 0, 0, 0, 0, *sizes.values(), 0, 0.0, 1, 0)[0] == 0
+    assert _c("ps_attention_decode_int4", 0, 256, 0, 0, 0, 0, 0, 0, 0, 256, 0, 0, 0, 0, 0, 0, *sizes.values(), 0, 0.0, 1, 0)[0] == 0
     assert _c("ps_attention_prefill_int4", 0, 256, 0, 0, 0, 256, 0, 0, 0, 0, 0, 0, *PORTIONS.values(), 0, 0, 0)[0] == 0
 
 

@@ -300,6 +300,63 @@ def test_sinks_of_minus_infinity(kind, splits):
     assert bool(((out[1:].double().cpu() - expected[0]).abs() <= plain.allowed(*expected, kind, kind == BF16)).all())
 
 
+STORED = [
+    # kv_heads, group, dim, page, lengths (the stored key among them), window, splits
+    (3, 1, 64, 16, (1, 32, 33, 200, 129), 0, 1), (2, 8, 128, 32, (700, 64, 5, 128), 0, 4), (1, 4, 32, 8, (90, 8, 9), 40, 2),
+    (2, 2, 96, 24, (50, 500), 0, 3), (1, 1, 256, 16, (300, 1), -64, 1), (2, 1, 33, 40, (41, 40, 260), 0, 8),
+    (1, 20, 64, 16, (140, 77), 0, 2), (1, 2, 160, 8, (66,), 0, 1), (1, 12, 192, 16, (150, 31), 0, 2), (2, 1, 7, 16, (17, 400), 0, 5),
+    (1, 1, 224, 64, (64, 65), 0, 1)]
+
+
+@pytest.mark.parametrize("kv_heads,group,dim,page,lengths,window,splits", STORED)
+def test_tokens_that_store_their_own_rows(kv_heads, group, dim, page, lengths, window, splits):
+    """One launch does what storing and attending do, bit for bit, in the pools too; a token in front of its context, one
+    behind the table and one whose page does not exist store nothing."""
+    from pagedserve_amd.ops import kernels
+
+    heads, items = kv_heads * group, len(lengths) + 3
+    tables, pages, _, _ = _requests((*lengths, 20, 20, 20), (0,) * items, page, 71)
+    pools, _ = _cache(tables, pages, [max(1, length - 1) for length in lengths] + [20, 20, 19], kv_heads, dim, page, 72)
+    tables[-1, 19 // page] = -1
+    g = torch.Generator().manual_seed(73)
+    both = torch.randn((items, (heads + 2 * kv_heads) * dim + 3), generator=g).to(BF16)
+    both[0, heads * dim + 2] = 1e4                           # (a step far above the others)
+    both = both.cuda()
+    q, k, v = both[:, :-3].split([heads * dim, kv_heads * dim, kv_heads * dim], 1)
+    positions = _ints([length - 1 for length in lengths] + [-1, tables.shape[1] * page + 3, 19])
+    results = []
+    for together in (False, True):
+        mine = [pool.clone() for pool in pools]
+        out = torch.full((items, heads * dim), 7.0, dtype=BF16).cuda()
+        partial = torch.full((items * heads * splits * (dim + 2),), math.nan).cuda()
+        if not together:
+            kernels.kv_write_int4(k, v, *mine, _ints(list(range(items))), positions, tables.cuda())
+        kernels.attention_decode_int4(q, *mine, out, None, positions, tables.cuda(), heads, dim ** -0.5, splits, partial, window,
+                                      store=(k, v) if together else None)
+        results.append((out, *mine))
+    # (the token behind the table sees places that nobody filled)
+    torch.testing.assert_close(results[1][0], results[0][0], rtol=0, atol=0, equal_nan=True)
+    assert torch.equal(results[0][1], results[1][1]) and torch.equal(results[0][2], results[1][2])
+    assert bool((results[1][0][-3] == 0).all()) and not bool(results[1][0][:-2].isnan().any() or results[1][0][-1].isnan().any())
+
+
+def test_a_stored_row_that_is_no_number():
+    """A NaN in the token's own value makes its group's result one, a NaN in its key the head's, and nothing else."""
+    from pagedserve_amd.ops import kernels
+
+    tables, pages, _, _ = _requests((40, 40, 40), (0, 0, 0), 16, 74)
+    pools, _ = _cache(tables, pages, (39, 39, 39), 2, 64, 16, 75)
+    rows = torch.randn((3, 384), generator=torch.Generator().manual_seed(76)).to(BF16).cuda()
+    rows[1, 128 + 3] = math.nan                              # a key's first head
+    rows[2, 256 + 64 + 40] = math.inf                        # a value's second head, second group
+    out = torch.zeros(3, 128, dtype=BF16).cuda()
+    kernels.attention_decode_int4(rows[:, :128], *pools, out, None, _ints([39, 39, 39]), tables.cuda(), 2, 0.125, 1,
+                                  store=(rows[:, 128:256], rows[:, 256:]))
+    bad = out.isnan().cpu()
+    assert not bad[0].any() and bad[1, :64].all() and not bad[1, 64:].any()
+    assert bad[2, 96:].all() and not bad[2, :96].any()
+
+
 PROMPT = [
     # kv_heads, group, dim, page, counts, starts, window, sink, softcap
     (1, 1, 64, 8, (2,), (0,), 0, False, 0.0), (3, 1, 64, 16, (65, 130), (0, 0), 0, False, 0.0),
