@@ -143,9 +143,11 @@ struct Int4Decode {
 //
 // dynamic LDS: the waves' maxima and sums [WAVES][16] each, the block's maxima [16], the token's own rows, then the waves' pairs of tiles, in
 // whose place the accumulators [WAVES][heads of the block][32 G] meet at the end
-// (of heads up to 64 five waves fit a unit's SIMD with 96 registers, two less than the form that stores takes by itself)
+// (registers for five waves to a SIMD of heads up to 64 and for four of heads up to 96, a few less than some forms take by
+// themselves: pages of 24, 64 requests of 25 heads of 64 over 1,024 keys 44.2 -> 43.0 us, 48 of 20 heads of 96 over 2,000
+// 71 -> 63; where that would spill, heads up to 64 that store over such pages, they take what they take)
 template <int G, int WAVES, bool EVEN, bool STORES>
-__global__ __launch_bounds__(64 * WAVES, G == 2 && EVEN ? 5 : 1) void attention_decode_int4_heads_kernel(const Int4Decode a) {
+__global__ __launch_bounds__(64 * WAVES, G == 2 && (EVEN || !STORES) ? 5 : G == 3 ? 4 : 1) void attention_decode_int4_heads_kernel(const Int4Decode a) {
   typedef Int4Stage<G> Stage;
   extern __shared__ __attribute__((aligned(1024))) float lds[];
   float* s_m = lds;
