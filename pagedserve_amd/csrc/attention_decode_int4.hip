@@ -391,9 +391,19 @@ __global__ __launch_bounds__(64 * WAVES, G == 2 && (EVEN || !STORES) ? 5 : G == 
           acc[g][1][r] *= correction;
         }
     }
+    float unit = factor;
+    if (__builtin_amdgcn_ballot_w64(fabsf(reference) > 1048576.f)) {
+      // (of such a product the part that rounding takes is an exponent of its own: all are rounded as the reference was)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s[i] *= factor;
+        asm volatile("" : "+v"(s[i]));
+      }
+      unit = 1.f;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], factor, -reference));
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], unit, -reference));
       l += s[i];
     }
   };

@@ -555,14 +555,27 @@ __device__ __forceinline__ void attention_prefill_block(
         // are all -inf and their exponentials 0.  Other lanes of the wave may differ, so the
         // products below run in any case.
         const float reference = (m_new == -INFINITY) ? 0.f : m_new;
+        float unit = scale_log2;
+        if (Pages::INT4 && __builtin_amdgcn_ballot_w64(fabsf(reference) > 1048576.f)) {
+          // (of such a product the part that rounding takes is an exponent of its own: all are rounded as the reference was)
+#pragma unroll
+          for (int r = 0; r < KR; ++r)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float product = s[r][e] * scale_log2;
+              asm volatile("" : "+v"(product));
+              s[r][e] = product;
+            }
+          unit = 1.f;
+        }
         float tile_sum = 0.f;
 #pragma unroll
         for (int r = 0; r < KR; ++r) {
           uint32_t words[8];
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r][e], scale_log2, -reference));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[r][e + 1], scale_log2, -reference));
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r][e], unit, -reference));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[r][e + 1], unit, -reference));
             tile_sum += p0 + p1;
             words[e >> 1] = pack2_bf16(p0, p1);
           }

@@ -340,6 +340,44 @@ def test_tokens_that_store_their_own_rows(kv_heads, group, dim, page, lengths, w
     assert bool((results[1][0][-3] == 0).all()) and not bool(results[1][0][:-2].isnan().any() or results[1][0][-1].isnan().any())
 
 
+@pytest.mark.parametrize("kind", [BF16, F32])
+@pytest.mark.parametrize("size", [1e9, 1e25])
+def test_scores_of_any_size(kind, size):
+    """Keys so large that the best score alone counts: its value, whatever the score's rounding."""
+    from pagedserve_amd.ops import kernels
+
+    tables, pages, items, positions = _requests((90,), (0,), 16, 77)
+    pools = [_garbage(pages, 1, 16, 64, 78 + which) for which in range(2)]
+    pools = [pool.cuda() for pool in pools]
+    g = torch.Generator().manual_seed(79)
+    k = torch.randn((90, 64), generator=g)
+    k[:, 0] = torch.randperm(90, generator=g) - 45.0
+    k[17, 0], k[71, 0] = 90.0, -90.0                         # (the scores' ends)
+    v = torch.randn((90, 64), generator=g)
+    kernels.kv_write_int4((k * size).cuda(), v.cuda(), *pools, _ints(items), _ints(positions), tables.cuda())
+    kept = [torch.zeros(90, 64).cuda() for _ in range(2)]
+    kernels.kv_read_int4(*pools, *kept, _ints(items), _ints(positions), tables.cuda())
+    q = torch.zeros(2, 64)
+    q[0, 0], q[1, 0] = 3.0, -3.0
+    best = [17, 71]
+    for splits in (1, 2):
+        out = torch.zeros(2, 64, dtype=kind).cuda()
+        kernels.attention_decode_int4(q.to(kind).cuda(), *pools, out, _ints([0, 0]), _ints([89, 89]), tables.cuda(), 1, 0.125,
+                                      splits, torch.zeros(2 * splits * 66).cuda())
+        expected = kept[1][best]
+        assert bool(((out.float() - expected).abs() <= 2.0 ** -7 * expected.abs().amax(1, keepdim=True)).all())
+    tiles = (_ints([0]), _ints([0]), _ints([0, 2]), _ints([90]), tables.cuda(), 1, 0.125)
+    q = q.to(kind).cuda()                                    # (positions 88 and 89, behind both ends)
+    out = torch.zeros(2, 64, dtype=kind).cuda()
+    if kind == F32:
+        kernels.attention_tiled_f32_int4(q, *pools, out, *tiles)
+        assert bool(((out - expected).abs() <= 2.0 ** -7 * expected.abs().amax(1, keepdim=True)).all())
+    else:
+        for query_tile, ranges in ((64, 1), (128, 1), (64, 2)):
+            kernels.attention_prefill_int4(q, *pools, out, *tiles, query_tile=query_tile, ranges=ranges)
+            assert bool(((out.float() - expected).abs() <= 2.0 ** -7 * expected.abs().amax(1, keepdim=True)).all())
+
+
 def test_a_stored_row_that_is_no_number():
     """A NaN in the token's own value makes its group's result one, a NaN in its key the head's, and nothing else."""
     from pagedserve_amd.ops import kernels
