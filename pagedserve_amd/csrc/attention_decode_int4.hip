@@ -18,9 +18,9 @@
 //
 // Bound by memory where there are blocks enough (4.5 bits a value), else by the trip block table -> codes: a tile's codes
 // are asked for one tile ahead (Int4Stage), its table entries, which are the same for a wave and come through the scalar
-// unit, two.  32 requests over 8,192 keys, 12 heads of 64: 51 us, 4.4 TB/s, 90 % of a large copy's rate (64: 92 us, 4.9 TB/s); 64 over
-// 768 to 1,024, 25 heads that share no keys: 29.4 us, 3.5 TB/s; 24 over up to 6,000, 16 heads of 128 over 2: 16.1 us; 1
-// over 900: 5.0 us and 2.0 for the merge.
+// unit, two.  32 requests over 8,192 keys, 12 heads of 64: 51 to 54 us, 4.2 to 4.4 TB/s, 85 to 90 % of a large copy's rate
+// (64: 92 us, 4.9 TB/s); 64 over 768 to 1,024, 25 heads that share no keys: 29.4 to 31 us, 3.4 TB/s; 24 over up to 6,000,
+// 16 heads of 128 over 2: 16.1 us; 1 over 900: 5.0 us and 2.0 for the merge.
 //
 // float queries, and scales that are not positive, take the kernel on the vector unit: LPK lanes share a key, a lane holds
 // eight dimensions of the query and takes one word of the key's codes; a conversion of the code and a multiply-add to a
@@ -141,13 +141,14 @@ struct Int4Decode {
 // STORES: a token's own key and value are stored first.  The wave whose tile holds them works out their codes, which go to LDS,
 // from where they replace what that tile's loads have found in their place, and at the end to the page, for later calls.
 //
-// dynamic LDS: the waves' maxima and sums [WAVES][16] each, the block's maxima [16], the token's own rows, then the waves' pairs of tiles, in
-// whose place the accumulators [WAVES][heads of the block][32 G] meet at the end
+// dynamic LDS: the waves' maxima and sums [WAVES][16] each, the block's maxima [16], the token's own rows, then the waves'
+// pairs of tiles, in whose place the accumulators [WAVES][heads of the block][32 G] meet at the end
 // (registers for five waves to a SIMD of heads up to 64 and for four of heads up to 96, a few less than some forms take by
 // themselves: pages of 24, 64 requests of 25 heads of 64 over 1,024 keys 44.2 -> 43.0 us, 48 of 20 heads of 96 over 2,000
 // 71 -> 63; where that would spill, heads up to 64 that store over such pages, they take what they take)
 template <int G, int WAVES, bool EVEN, bool STORES>
-__global__ __launch_bounds__(64 * WAVES, G == 2 && (EVEN || !STORES) ? 5 : G == 3 ? 4 : 1) void attention_decode_int4_heads_kernel(const Int4Decode a) {
+__global__ __launch_bounds__(64 * WAVES, G == 2 && (EVEN || !STORES) ? 5 : G == 3 ? 4 : 1) void
+attention_decode_int4_heads_kernel(const Int4Decode a) {
   typedef Int4Stage<G> Stage;
   extern __shared__ __attribute__((aligned(1024))) float lds[];
   float* s_m = lds;
@@ -363,7 +364,8 @@ __global__ __launch_bounds__(64 * WAVES, G == 2 && (EVEN || !STORES) ? 5 : G == 
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const uint32_t w = codes[sub][g];
-        const int4_u32x4 row = {int4_pair<0>(w, mask, sixteens), int4_pair<1>(w, mask, sixteens), int4_pair<2>(w, mask, sixteens), int4_pair<3>(w, mask, sixteens)};
+        const int4_u32x4 row = {int4_pair<0>(w, mask, sixteens), int4_pair<1>(w, mask, sixteens),
+                                int4_pair<2>(w, mask, sixteens), int4_pair<3>(w, mask, sixteens)};
         const int4_f32x4 dot = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(int4_bf16x8, row), query[g],
                                                                        start[g], 0, 0, 0);
 #pragma unroll
@@ -823,8 +825,10 @@ extern "C" int ps_attention_decode_int4(const void* q, int64_t q_stride, const v
                              partial_floats >= (int64_t)count * heads * splits * (head_dim + 2)),
              "ps_attention_decode_int4: %lld floats of scratch are too few for %d ranges", (long long)partial_floats,
              splits);
-  PS_REQUIRE((new_k == nullptr) == (new_v == nullptr) && (new_k == nullptr || (dtype == PS_BF16 && scale > 0.f && tok_item == nullptr && tok_list == nullptr)),
-             "ps_attention_decode_int4: rows to be stored are keys and values in bfloat16, a request's to a token, under a positive scale");
+  PS_REQUIRE((new_k == nullptr) == (new_v == nullptr) &&
+                 (new_k == nullptr || (dtype == PS_BF16 && scale > 0.f && tok_item == nullptr && tok_list == nullptr)),
+             "ps_attention_decode_int4: rows to be stored are keys and values in bfloat16, a request's to a token, under a "
+             "positive scale");
   if (count == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid(count, heads, splits);
@@ -853,7 +857,8 @@ extern "C" int ps_attention_decode_int4(const void* q, int64_t q_stride, const v
     const bool wide_q = head_dim % 8 == 0 && q_stride % 8 == 0 && (uintptr_t)q % 16 == 0;
     const Int4Decode a{(const bf16_t*)q, q_stride, (const uint8_t*)k_pool, (const uint8_t*)v_pool, (bf16_t*)out, out_stride,
                        partial, tok_list, tok_item, tok_pos, tables, table_width, heads, kv_heads,
-                       (kv_group + block_heads - 1) / block_heads, block_heads, head_dim, page_size, page_shift, num_pages, window, splits,
+                       (kv_group + block_heads - 1) / block_heads, block_heads, head_dim, page_size, page_shift,
+                       num_pages, window, splits,
                        wide_q, scale * 1.4426950408889634f, softcap * 1.4426950408889634f, sink,
                        (const bf16_t*)new_k, (const bf16_t*)new_v, new_k_stride, new_v_stride};
     const int64_t blocks = (int64_t)count * kv_heads * a.parts;

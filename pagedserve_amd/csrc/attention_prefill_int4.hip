@@ -163,7 +163,8 @@ extern "C" int ps_attention_prefill_int4(const void* q, int64_t q_stride, const 
 #undef PS_LAUNCH_P4
   PS_CHECK_LAUNCH("ps_attention_prefill_int4");
   if (ranges > 1) {
-    hipLaunchKernelGGL(attention_prefill_int4_join_kernel, dim3(heads, tiles, (query_tile * (head_dim / 4) + 255) / 256), dim3(256), 0, s,
+    hipLaunchKernelGGL(attention_prefill_int4_join_kernel,
+                       dim3(heads, tiles, (query_tile * (head_dim / 4) + 255) / 256), dim3(256), 0, s,
                        partial, states, (bf16_t*)out, out_stride, tile_item, tile_q0, cu_tokens, heads, head_dim, query_tile, ranges);
     PS_CHECK_LAUNCH("ps_attention_prefill_int4(join)");
   }

@@ -7,8 +7,8 @@
 // rounded to five significant bits, ties to even: e itself is code 0 up to that rounding, all sixteen codes are
 // used, and (code - 8) d, three bits times five, is a bfloat16 number without rounding, so that
 // attention over this cache is attention over a bfloat16 cache which holds these values.  (Root mean
-// square error of normal values 8.62 % of theirs, 8.60 % with the step unrounded; codes -7 .. 7 of the magnitude 9.7 %.)  A step that is still
-// below the normal floats becomes 0, and the group zeros; a group that holds an infinity or a NaN
+// square error of normal values 8.62 % of theirs, 8.60 % with the step unrounded; codes -7 .. 7 of the magnitude 9.7 %.)
+// A step that is still below the normal floats becomes 0, and the group zeros; a group that holds an infinity or a NaN
 // gets a NaN for its step and is NaN as a whole, as a cache in the model's type would show it.
 //
 // A page of one head: the codes of its keys, 16 G bytes each (G groups), then their steps, G bfloat16

@@ -10,7 +10,8 @@
 // logits, T, bounds the alternatives from below, and about `top` threads have any logit that reaches it: the shares of
 // these are read again (out of the cache), a share by a wave, and what reaches T goes to one wave, which sorts.  So
 // alternatives cost no second pass over the row.  Logits and ids are compared as one 64-bit number, in which no two are
-// equal: a row of equal logits costs a second round for that bound, no more, and the results do not depend on the order in which candidates arrive.
+// equal: a row of equal logits costs a second round for that bound, no more, and the results do not depend on the order in
+// which candidates arrive.
 //
 // Long rows are cut into parts, whose records a second launch joins.
 //

@@ -311,8 +311,8 @@ int ps_attention_decode_int4(const void* q, int64_t q_stride, const void* new_k,
                              const int* tables, int table_width, int count, int heads, int kv_heads,
                              int head_dim, int page_size, int num_pages, float scale, int window,
                              int splits, const float* sink, float softcap, int dtype, void* stream);
-// ps_attention_prefill over such a cache (bfloat16 q and out), block_heads (1 or 2) heads of a key/value head to a block, the keys of every tile cut into `ranges` where units would
-// stay idle over long contexts.  With more than one, partial (from a multiple of 16 bytes on) is scratch of
+// ps_attention_prefill over such a cache (bfloat16 q and out), block_heads (1 or 2) heads of a key/value head to a block, the
+// keys of every tile cut into `ranges` where units would stay idle over long contexts.  With more than one, partial (from a multiple of 16 bytes on) is scratch of
 // tiles x heads x ranges x query_tile x (head_dim + 2) floats.
 int ps_attention_prefill_int4(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool,
                               void* out, int64_t out_stride, const int* tile_item, const int* tile_q0,

@@ -1439,8 +1439,8 @@ def int4_decode_splits(dtype, count, heads, kv_heads, head_dim, visible) -> int:
       9.3 and 8.1, over 4,000 in 8 and 16 12.9 and 13.9; 24 of 16 heads of 128 over 2 and 6,000 keys in 8 and 16 20.2
       and 19.2, 16 of 16 over 4 and 2,000 11.7 and 14.5).
     * More blocks: one range up to 2,048 keys (20 of 12 heads over 1,000 in 1 and 2 9.1 and 11.1), beyond of 512 keys or more,
-      eight at most, until nine blocks come to a unit, of bfloat16 heads beyond 64, fewer of whose blocks a unit holds, three (32 of 12 over 8,192
-      keys in 1, 4, 6 and 8 81, 53.6, 50.8 and 52.6, 64 in 2, 3 and 4 101, 91.7 and 92.6; 64 of 32 heads of 128 over 4 and 4,096
+      eight at most, until nine blocks come to a unit, of bfloat16 heads beyond 64, fewer of whose blocks a unit holds,
+      three (32 of 12 over 8,192 keys in 1, 4, 6 and 8 81, 53.6, 50.8 and 52.6, 64 in 2, 3 and 4 101, 91.7 and 92.6; 64 of 32 heads of 128 over 4 and 4,096
       in 3 and 6 38.6 and 41.1)."""
     units = compute_units()
     group = 1 if dtype == torch.float32 else heads // kv_heads
@@ -1569,11 +1569,12 @@ def _int4_tiles(what, q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_
 
 
 def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_lens, tables, heads, scale,
-                           window=0, max_kv_len=0, query_tile=PREFILL_TILE, sink=None, softcap=0.0, block_heads=None, ranges=None, partial=None):
+                           window=0, max_kv_len=0, query_tile=PREFILL_TILE, sink=None, softcap=0.0, block_heads=None,
+                           ranges=None, partial=None):
     """``attention_prefill`` over a cache in 4 bits (bfloat16 queries, head sizes in multiples of 16).
     ``block_heads``: 1 or 2 heads to a block (None: ``prefill_int4_block_heads(...)``).  ``ranges``: parts of the keys of
-    every tile, joined by a second launch (None: ``prefill_int4_ranges(...)``, one where ``max_kv_len`` is not given); with more than one ``partial`` is float scratch of
-    ``tiles * heads * ranges * query_tile * (head_dim + 2)`` values, allocated for the call where it is None."""
+    every tile, joined by a second launch (None: ``prefill_int4_ranges(...)``, one where ``max_kv_len`` is not given); with
+    more than one ``partial`` is float scratch of ``tiles * heads * ranges * query_tile * (head_dim + 2)`` values, allocated for the call where it is None."""
     _check_prefill_constants()
     addresses, sizes, sink_at, device = _int4_tiles("attention_prefill_int4", q, k_pool, v_pool, out, tile_item, tile_q0,
                                                     cu_tokens, kv_lens, tables, heads, sink, torch.bfloat16)
