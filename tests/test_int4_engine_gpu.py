@@ -85,6 +85,25 @@ def test_bfloat16_runs_under_every_cut(models, which):
     assert max(errors) < 0.15, errors
 
 
+@pytest.mark.parametrize("dtype,limit", [("bfloat16", 0.15), ("float32", 2e-3)])
+def test_long_contexts(tmp_path, dtype, limit):
+    """Portions and single tokens behind hundreds of keys, where both are cut into ranges, with and without graphs.  (In
+    32-bit a code that turns moves a logit by some thousandth; tests with margins hold the rest to rounding.)"""
+    config = dict(helpers.TINY_A, n_positions=1024)
+    folder = helpers.write_folder(os.path.join(str(tmp_path), "long"), config, helpers.lively_tensors(config, 5))
+    requests = {i: helpers.random_tokens(n, config["vocab_size"], 950 + i) for i, n in enumerate((900, 640, 3))}
+    raw, weights = plain_gpt2.read_model_folder(folder)
+    with int4_models.cache_in_4_bits():
+        reference = {rid: plain_gpt2.forward_logits(raw, weights, tokens) for rid, tokens in requests.items()}
+    for graphs in (True, False):
+        engine = _engine(folder, 16, dtype, use_graphs=graphs, num_pages=120)
+        rows = helpers.replay_in_process(engine, helpers.trace_mixed(requests, portion=(60, 33, 129, 2), decode_tail=24))
+        difference = torch.stack([row - reference[rid][at] for (rid, at), row in rows.items()])
+        expected = torch.stack([reference[rid][at] for rid, at in rows])
+        assert float(difference.norm() / expected.norm()) < limit
+        assert len(rows) == 1543 and not engine.cache.requests
+
+
 def test_generated_tokens_are_the_plain_models(models):
     """Greedy decoding through the scheduler, its graphs and the entry point, in 32-bit."""
     from pagedserve_amd.engine.llm import LLM
