@@ -148,7 +148,7 @@ class Engine:
         self.max_layouts_remembered = 512
         self._graphs = {}        # key -> StepGraph
         self._graph_seen = {}     # layout -> steps that ran without a graph (buffers exist now)
-        self._layouts = {}        # (tokens, items, wanted, singles, tiles) -> offsets, size, device views
+        self._layouts = {}        # (tokens, items, wanted, singles, tiles of every size) -> offsets, size, device views
         self._graph_failures = {}
         self._workspace_moved = 0
         self._graph_retired = []  # (event, graph): dropped, destroyed once the event has happened
@@ -317,7 +317,7 @@ class Engine:
     def _pack(self, entries, select=None):
         """Fill the packed index buffer on the host, copy it, and return the step context.
 
-        The layout depends only on (tokens, items, wanted rows, one-token items)."""
+        The layout depends only on (tokens, items, wanted rows, one-token items, query tiles of every size)."""
         cache = self.cache
         counts = [len(entry.tokens) for entry in entries]
         tokens = sum(counts)
@@ -508,7 +508,7 @@ class Engine:
 
     def _run_step(self, entries, greedy=False) -> StepOutput:
         """Steps of one layout (numbers of tokens, items, wanted rows, one-token items and
-        query tiles, and how tokens are chosen) issue the same launches with the same
+        query tiles of every size, and how tokens are chosen) issue the same launches with the same
         arguments: everything else lies in the packed index buffer.  The first step of a
         layout runs directly (buffers get allocated), the second is recorded as a HIP graph,
         later ones copy their indices and replay it."""
@@ -525,7 +525,7 @@ class Engine:
             # every entry brings one token and wants its logits: the lean path
             requests = self.cache.requests
             longest = 1 + max(requests[entry.request_id].length for entry in entries)
-            key = (items, items, items, items, 0, mode, self._context_class(longest))
+            key = (items, items, items, items, (0,) * len(self.query_tiles), mode, self._context_class(longest))
             plan = self._graphs.get(key)
             if (plan is not None and plan.logits.data_ptr() == self._logit_buffer(items).data_ptr()
                     and all(len(e.tokens) == 1 and len(e.want) == 1 for e in entries)):
@@ -536,7 +536,8 @@ class Engine:
         logits = self._logit_buffer(wanted)
         singles = ctx.single_tokens.numel()
         kv_class = self._context_class(ctx.max_kv_len)
-        tiles = sum(lists[0].numel() for lists in ctx.query_tiles.values())
+        # (of every size for itself: the index arrays lie behind one another, and launches take a size's count)
+        tiles = tuple(lists[0].numel() for lists in ctx.query_tiles.values())
         graph_key = (ctx.tokens, items, wanted, singles, tiles, mode, kv_class)
         if not self.use_graphs or graph_key in self._graph_failures:
             out, tokens = self._forward(ctx, rows, logits, wanted, greedy)
