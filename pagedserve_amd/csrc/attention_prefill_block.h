@@ -4,6 +4,7 @@
 #pragma once
 #include <math.h>
 
+#include "attention_prefill_keys.h"
 #include "cache_int4.h"
 #include "common.h"
 
@@ -142,23 +143,21 @@ __device__ __forceinline__ void attention_prefill_block(
   // (over a cache in 4 bits positions behind the block table see what the table has)
   const int64_t table_room = Pages::INT4 ? (int64_t)table_width * page_size : INT32_MAX;
   const int room = table_room < INT32_MAX ? (int)table_room : INT32_MAX;
-  const int key_end = start + tile_last_q + 1 < room ? start + tile_last_q + 1 : room;
+  PrefillKeys keys = prefill_keys(start, q0, tile_last_q, window, room, page_size, page_shift, AP_KEYS);
+  const int key_begin = keys.begin, key_end = keys.end;
   const int q_last = q_pos < room ? q_pos : room - 1;
-  const int key_begin = first_visible_key(start + q0, window);
   // the first keys that the wave's first and last query see
   const int first_of_first = first_visible_key(wave_first, window);
   const int first_of_last = wave_active ? first_visible_key(wave_last, window) : 0;
 
   // the block-table entries of keys key_begin .. key_end - 1
-  const int first_logical = page_shift >= 0 ? (key_begin >> page_shift) : key_begin / page_size;
-  const int last_logical = page_shift >= 0 ? ((key_end - 1) >> page_shift) : (key_end - 1) / page_size;
   // kept as the number of the page's first key row of this head within the pool (a row: one
   // key's HD values; the host checks that the pool has fewer than 2^32 of them), so that a
   // load's address is one multiplication away
   const uint32_t page_rows = (uint32_t)kv_heads * (uint32_t)page_size;
   const uint32_t head_rows = (uint32_t)kv_head * (uint32_t)page_size;
-  for (int i = tid; i <= last_logical - first_logical && i < AP_TABLE_MAX; i += 64 * QW * KS) {
-    const int logical = first_logical + i;
+  for (int i = tid; i < keys.entries && i < AP_TABLE_MAX; i += 64 * QW * KS) {
+    const int logical = keys.first_entry + i;
     int page = logical < table_width ? table[logical] : 0;
     page = (page >= 0 && page < num_pages) ? page : 0;         // never an address outside the pool
     s_table[i] = (uint32_t)page * page_rows + head_rows;
@@ -194,16 +193,10 @@ __device__ __forceinline__ void attention_prefill_block(
   auto place_of = [&](int key, uint32_t& page_row, int& within) {
     // keys outside the tile's visible range are fetched from a visible key instead: they
     // are masked below, and whatever lies in pages that were given back is never read
-    key = key < key_begin ? key_begin : (key >= key_end ? key_end - 1 : key);
-    int logical;
-    if (page_shift >= 0) {
-      logical = key >> page_shift;
-      within = key & page_mask;
-    } else {
-      logical = key / page_size;
-      within = key - logical * page_size;
-    }
-    page_row = s_table[logical - first_logical];
+    key = prefill_key(keys, key);
+    const int logical = prefill_entry(key, page_size, page_shift);
+    within = page_shift >= 0 ? key & page_mask : key - logical * page_size;
+    page_row = s_table[logical - keys.first_entry];
   };
   auto issue = [&](int tile_number, int k0) {
     if constexpr (!Pages::INT4) {
@@ -430,14 +423,8 @@ __device__ __forceinline__ void attention_prefill_block(
       }
   }
 
-  int k_first = key_begin / AP_KEYS * AP_KEYS;
-  int tiles = (key_end - k_first + AP_KEYS - 1) / AP_KEYS;
-  if (Pages::INT4 && part.ranges > 1) {
-    const int per = (tiles + part.ranges - 1) / part.ranges;
-    k_first += part.range * per * AP_KEYS;
-    tiles -= part.range * per;
-    tiles = tiles < per ? tiles : per;      // (none or fewer: a range without keys)
-  }
+  if (Pages::INT4 && part.ranges > 1) prefill_range(keys, part.range, part.ranges, AP_KEYS);
+  const int k_first = keys.first, tiles = keys.tiles;
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the table is in LDS
   // the queries have arrived with that; a use here keeps the compiler from waiting for them
   // (and with them for every tile in flight) inside the loop
