@@ -16,6 +16,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 #define AP_QUERIES 64      // queries per block (32 with QW = 1, 128 with QW = 4)
 #define AP_TABLE_MAX 2048  // block-table entries that a tile may need
 #define AP_LARGE_HEAD_DIM 64   // largest head size of the blocks of 128 queries
+#define AP_NO_PAGE 0xffffffffu // in the place of a page's first row (a cache in 4 bits): the table names none
 
 typedef const __attribute__((address_space(1))) void* ap_global_ptr;
 typedef __attribute__((address_space(3))) void* ap_lds_ptr;
@@ -156,12 +157,19 @@ __device__ __forceinline__ void attention_prefill_block(
   // load's address is one multiplication away
   const uint32_t page_rows = (uint32_t)kv_heads * (uint32_t)page_size;
   const uint32_t head_rows = (uint32_t)kv_head * (uint32_t)page_size;
+  bool missing = false;
   for (int i = tid; i < keys.entries && i < AP_TABLE_MAX; i += 64 * QW * KS) {
     const int logical = keys.first_entry + i;
     int page = logical < table_width ? table[logical] : 0;
-    page = (page >= 0 && page < num_pages) ? page : 0;         // never an address outside the pool
-    s_table[i] = (uint32_t)page * page_rows + head_rows;
+    const bool there = page >= 0 && page < num_pages;
+    missing |= !there;
+    page = there ? page : 0;                                   // never an address outside the pool
+    s_table[i] = Pages::INT4 && !there ? AP_NO_PAGE : (uint32_t)page * page_rows + head_rows;
   }
+  // (what the waves found lies where nothing is stored before the loop's first barrier)
+  uint32_t* found = reinterpret_cast<uint32_t*>(stages + STAGE_BYTES);
+  if (Pages::INT4 && __builtin_amdgcn_ballot_w64(missing) != 0) missing = true;
+  if (Pages::INT4 && lane == 0) found[wave] = missing;
 
   // queries as column operand of the first product: lane (query sub, dims step*16 + half*8 ..)
   bf16x8 qf[NDB];
@@ -197,6 +205,7 @@ __device__ __forceinline__ void attention_prefill_block(
     const int logical = prefill_entry(key, page_size, page_shift);
     within = page_shift >= 0 ? key & page_mask : key - logical * page_size;
     page_row = s_table[logical - keys.first_entry];
+    if constexpr (Pages::INT4) page_row = page_row == AP_NO_PAGE ? head_rows : page_row;     // (a place that exists)
   };
   auto issue = [&](int tile_number, int k0) {
     if constexpr (!Pages::INT4) {
@@ -430,7 +439,11 @@ __device__ __forceinline__ void attention_prefill_block(
   // (and with them for every tile in flight) inside the loop
 #pragma unroll
   for (int step = 0; step < NDB; ++step) asm volatile("" : "+v"(qf[step]));
+  // Over a cache in 4 bits keys without a page are masked: whether there are any is known to all waves, and which ones is
+  // looked up only then.
+  bool holes = false;
   if constexpr (Pages::INT4) {
+    holes = __builtin_amdgcn_ballot_w64(lane < AP_WAVES && found[lane % AP_WAVES] != 0) != 0;
     if (tiles > 0) {
       fetch(k_first);
       store(0);
@@ -488,12 +501,24 @@ __device__ __forceinline__ void attention_prefill_block(
       }
     }
   };
+  // scores of a wave's keys that have no page, eight at a time (pages hold a multiple of 8)
+  auto hide_absent = [&](const int kw, f32x16 (&s)[KR]) {
+#pragma unroll
+    for (int r = 0; r < KR; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int entry = prefill_entry(prefill_key(keys, kw + 32 * r + 8 * i), page_size, page_shift) - keys.first_entry;
+        if (__builtin_amdgcn_readfirstlane(s_table[entry]) != AP_NO_PAGE) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r][4 * i + e] = -INFINITY;
+      }
+  };
   // softmax of a wave's scores of one tile and the second product (the values' reads may
   // still be in flight when it starts)
   auto weigh = [&](const int kw, f32x16 (&s)[KR], ValueRegs& vr) {
     // all of these keys are visible to every query of the wave: no mask
       const bool masked = kw + WAVE_KEYS - 1 > wave_first || kw + WAVE_KEYS > key_end ||
-                          kw < first_of_last || !q_valid;
+                          kw < first_of_last || !q_valid || holes;
       // scores stay unscaled until the exponential: p = 2^(s c - m), with m kept in scaled units
       if (extra.softcap > 0.f) {
         // a cap on the scaled scores, in the unscaled scores' units
@@ -506,6 +531,7 @@ __device__ __forceinline__ void attention_prefill_block(
       float tile_max = -INFINITY;
       if (__builtin_amdgcn_readfirstlane(__any(masked) ? 1 : 0)) {
         const int q_first = q_valid ? first_visible_key(q_pos, window) : 0;
+        if (Pages::INT4 && holes) hide_absent(kw, s);
 #pragma unroll
         for (int r = 0; r < KR; ++r)
 #pragma unroll

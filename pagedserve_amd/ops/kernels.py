@@ -1574,7 +1574,9 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
     """``attention_prefill`` over a cache in 4 bits (bfloat16 queries, head sizes in multiples of 16).
     ``block_heads``: 1 or 2 heads to a block (None: ``prefill_int4_block_heads(...)``).  ``ranges``: parts of the keys of
     every tile, joined by a second launch (None: ``prefill_int4_ranges(...)``, one where ``max_kv_len`` is not given); with
-    more than one ``partial`` is float scratch of ``tiles * heads * ranges * query_tile * (head_dim + 2)`` values, allocated for the call where it is None."""
+    more than one ``partial`` is float scratch of ``tiles * heads * ranges * query_tile * (head_dim + 2)`` values, allocated for the call where it is None.
+    As for single tokens, keys whose table entry lies outside the pool are seen by nobody, and positions behind the block table
+    see what the table has."""
     _check_prefill_constants()
     addresses, sizes, sink_at, device = _int4_tiles("attention_prefill_int4", q, k_pool, v_pool, out, tile_item, tile_q0,
                                                     cu_tokens, kv_lens, tables, heads, sink, torch.bfloat16)

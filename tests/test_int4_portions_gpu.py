@@ -1,6 +1,7 @@
 """Prompt portions over a cache in 4 bits where a table or a page ends: against plain formulas in 64 bits."""
 
 import math
+from unittest import mock
 
 import pytest
 import torch
@@ -13,9 +14,9 @@ pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
 
 
-def _portions(kind, dim):
+def _portions(kind, dim, group=1):
     """(what it is, a call ``(q, pools, out, counts, lengths, tables, heads, window=0, sink=None)``) for every form of tile that
-    takes the head size, in one range and in several."""
+    takes the head size and as many heads to a key/value head, in one range and in several."""
     from pagedserve_amd.ops import kernels
 
     def call(size, name, **options):
@@ -31,8 +32,11 @@ def _portions(kind, dim):
         return [((size, paired), call(size, "attention_tiled_f32_int4", paired=paired))
                 for size, paired in ((32, False), (64, False), (64, True))]
     sizes = (64, 128) if dim <= 128 else (64,)
-    return [((size, ranges, most), call(size, "attention_prefill_int4", ranges=ranges, max_kv_len=most))
-            for size in sizes for ranges, most in ((1, 0), (1, 100), (3, 0))]
+    forms = [((size, ranges, most), call(size, "attention_prefill_int4", ranges=ranges, max_kv_len=most))
+             for size in sizes for ranges, most in ((1, 0), (1, 100), (3, 0))]
+    if group % 2 == 0 and 64 < dim <= 128:
+        forms += [((64, ranges, "pairs"), call(64, "attention_prefill_int4", ranges=ranges, block_heads=2)) for ranges in (1, 3)]
+    return forms
 
 
 @pytest.mark.parametrize("kind", [BF16, F32])
@@ -66,3 +70,57 @@ def test_windows_that_begin_behind_the_table(kind, dim, page, width, window):
         off = (out[:tokens].double().cpu() - expected[0]).abs() <= limit
         assert bool(off[sees].all()), form
         assert bool((out[tokens] == -9.0).all())
+
+
+def _check(out, expected, kind, what):
+    """NaN where the formula has one, and nowhere else; the rest within bounds."""
+    out, limit = out.double().cpu(), plain.allowed(*expected, kind, kind == BF16)
+    bad = expected[0].isnan()
+    assert torch.equal(out.isnan(), bad), (what, (out.isnan() != bad).nonzero()[:4].tolist())
+    assert bool(((out - expected[0]).abs()[~bad] <= limit[~bad]).all()), what
+
+
+MISSING = [
+    # group, dim, page, counts, starts, window, sink, logical pages of every request that the table does not have
+    (1, 64, 16, (70,), (100,), 0, False, ((0, 4, 5, 9),)), (2, 128, 8, (66, 20), (30, 150), 0, False, ((1, 2, 11), (18, 19, 20, 21))),
+    (1, 64, 24, (130, 3), (0, 50), 40, False, ((1, 4), (2,))), (2, 48, 16, (40, 33), (60, 0), 0, True, ((5,), (0, 1, 2))),
+    (1, 256, 32, (70,), (200,), -64, False, ((3, 7),)), (2, 128, 64, (129,), (300,), 0, False, ((1, 5),)),
+    (1, 16, 8, (65,), (8,), 0, False, (tuple(range(8)),))]
+
+
+@pytest.mark.parametrize("kind", [BF16, F32])
+@pytest.mark.parametrize("group,dim,page,counts,starts,window,sink,missing", MISSING)
+def test_pages_that_the_table_does_not_have(kind, group, dim, page, counts, starts, window, sink, missing):
+    """Keys whose entry lies outside the pool are seen by nobody, as single tokens have it: not those of another page."""
+    from pagedserve_amd.ops import kernels
+
+    if kind == F32 and dim > 128:
+        pytest.skip("float portions of such heads go token by token")
+    heads = 2 * group
+    lengths = [a + b for a, b in zip(counts, starts)]
+    tables, pages, items, positions = _requests(counts, starts, page, 81)
+    pools, kept = _cache(tables, pages, lengths, 2, dim, page, 82)
+    for item, gone in enumerate(missing):
+        for turn, logical in enumerate(gone):
+            tables[item, logical] = (-1, pages, 1 << 30)[turn % 3]
+    q = torch.randn((sum(counts), heads * dim), generator=torch.Generator().manual_seed(83)).to(kind)
+    sinks = torch.randn(heads, generator=torch.Generator().manual_seed(84)).cuda() if sink else None
+    parts = []
+    for item, part in enumerate(q.split(list(counts))):
+        seen = plain.visible
+        with mock.patch.object(plain, "visible", lambda at, key, window: seen(at, key, window)
+                               and key // page not in missing[item]):
+            parts.append(list(plain.attention(part, *kept[item], list(range(starts[item], lengths[item])), heads, dim ** -0.5,
+                                              window, sinks)))
+    expected = [torch.cat([part[which] for part in parts]) for which in range(3)]
+    for form, run in _portions(kind, dim, group):
+        print(form, flush=True)
+        out = torch.full((len(items) + 1, heads * dim), -9.0, dtype=kind).cuda()
+        run(q.cuda(), pools, out[:-1], counts, lengths, tables.cuda(), heads, window, sinks)
+        blind = torch.cat([part[0] for part in parts]).eq(0).all(1)
+        _check(out[:-1][~blind], [e[~blind] for e in expected], kind, form)
+        assert bool((out[-1] == -9.0).all())
+    out = torch.zeros((len(items), heads * dim), dtype=kind).cuda()
+    kernels.attention_decode_int4(q.cuda(), *pools, out, _ints(items), _ints(positions), tables.cuda(), heads, dim ** -0.5, 1,
+                                  None, window, sink=sinks)
+    _check(out, expected, kind, "single tokens")
