@@ -4,6 +4,8 @@
 #pragma once
 #include <math.h>
 
+#include <type_traits>
+
 #include "attention_prefill_keys.h"
 #include "cache_int4.h"
 #include "common.h"
@@ -243,8 +245,7 @@ __device__ __forceinline__ void attention_prefill_block(
     if constexpr (ROW_ITEMS % THREADS == 0) return j * THREADS >= ROW_ITEMS;
     else return j * THREADS + wave * 64 >= ROW_ITEMS;
   };
-  uint32_t codes[Pages::INT4 ? ITEMS : 1][GROUPS], steps[Pages::INT4 ? ITEMS : 1][STEP_WORDS],
-      value_steps[Pages::INT4 ? ITEMS : 1][STEP_WORDS];
+  uint32_t codes[Pages::INT4 ? ITEMS : 1][GROUPS], steps[Pages::INT4 ? ITEMS : 1][STEP_WORDS];
   // Which key an item is of: of every 16 in an order that spreads the stores of 16 lanes over the banks, whose rows are
   // turned by the key's number (rows of 64 dimensions: keys 0, 1, 8, 9, .., of 128: 0, 4, 8, 12, ..).
   auto key_of = [&](int item) {
@@ -285,8 +286,8 @@ __device__ __forceinline__ void attention_prefill_block(
         uint32_t page_row;
         int within;
         place_of(k0 + key_local, page_row, within);
-        const uint64_t at = (uint64_t)page_row * (18 * GROUPS);
-        const uint8_t* from = (is_value ? v_pool : k_pool) + at + within * (16 * GROUPS) + c * (4 * GROUPS);
+        const uint8_t* page = (is_value ? v_pool : k_pool) + (uint64_t)page_row * (18 * GROUPS);
+        const uint8_t* from = page + within * (16 * GROUPS) + c * (4 * GROUPS);
         if constexpr (GROUPS % 4 == 0) {
 #pragma unroll
           for (int i = 0; i < GROUPS / 4; ++i) {
@@ -307,9 +308,7 @@ __device__ __forceinline__ void attention_prefill_block(
 #pragma unroll
           for (int i = 0; i < GROUPS; ++i) codes[j][i] = reinterpret_cast<const uint32_t*>(from)[i];
         }
-        const int step_at = page_size * (16 * GROUPS) + within * (2 * GROUPS);
-        load_steps(v_pool + at + step_at, value_steps[j]);
-        if (!is_value) load_steps(k_pool + at + step_at, steps[j]);
+        load_steps(page + page_size * (16 * GROUPS) + within * (2 * GROUPS), steps[j]);
       }
     }
   };
@@ -326,6 +325,10 @@ __device__ __forceinline__ void attention_prefill_block(
                             fmaf((float)(odd >> (8 * i) & 0xffu), step, base));
     return words;
   };
+  // A value that is no number must not reach the queries that do not see its key: their weight of 0 would still make it one.
+  // It is 0 in LDS, and that the thread has met such a value is kept for the block's end.  (By its step, which is finite or
+  // NaN; nobody knows what it is in a page that was never written, which stands in for one that the table does not name.)
+  float no_number = 0.f;
   auto store = [&](int tile_number) {
     if constexpr (Pages::INT4) {
       unsigned char* stage = stages + (tile_number % STAGES) * STAGE_BYTES;
@@ -336,41 +339,41 @@ __device__ __forceinline__ void attention_prefill_block(
         const int key_local = key_of(item), c = item & 3;
         const int turn = (key_local / SPREAD) % CH;
         unsigned char* row = stage + (is_value ? TILE_BYTES : 0) + key_local * ROW;
+        // (a branch, which a wave takes one way: the compiler would make both kinds of words and choose)
+        auto store_row = [&](auto turned) __attribute__((always_inline)) {
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          const int piece = 4 * g + c;
-          if (CH % 4 != 0 && piece >= CH) continue;           // (behind the last dimension)
-          // A value that is no number must not reach the queries that do not see its key, whose weight of 0 would
-          // still make it one: it is 0 here, and the key takes its place, whose scores are masked.
-          const float v_step = __uint_as_float(value_steps[j][g / 2] >> (16 * (g % 2)) << 16);
-          uint32_t word;
-          float step;
-          if (is_value) {
-            // byte b of the word for this group is byte b GROUPS + g of the row's quarter
-            if constexpr (GROUPS == 1) word = codes[j][0];
-            else if constexpr (GROUPS == 2)
-              word = __builtin_amdgcn_perm(codes[j][1], codes[j][0], g ? 0x07050301u : 0x06040200u);
-            else if constexpr (GROUPS == 4)
-              word = __builtin_amdgcn_perm(codes[j][1], codes[j][0], 0x0c0c0400u + 0x0101u * g) |
-                     __builtin_amdgcn_perm(codes[j][3], codes[j][2], 0x04000c0cu + 0x01010000u * g);
-            else {
-              word = 0;
+          for (int g = 0; g < GROUPS; ++g) {
+            const int piece = 4 * g + c;
+            if (CH % 4 != 0 && piece >= CH) continue;         // (behind the last dimension)
+            uint32_t word = codes[j][g];
+            if constexpr (turned.value && GROUPS > 1) {
+              // byte b of the word for this group is byte b GROUPS + g of the row's quarter
+              if constexpr (GROUPS == 2)
+                word = __builtin_amdgcn_perm(codes[j][1], codes[j][0], g ? 0x07050301u : 0x06040200u);
+              else if constexpr (GROUPS == 4)
+                word = __builtin_amdgcn_perm(codes[j][1], codes[j][0], 0x0c0c0400u + 0x0101u * g) |
+                       __builtin_amdgcn_perm(codes[j][3], codes[j][2], 0x04000c0cu + 0x01010000u * g);
+              else {
+                word = 0;
 #pragma unroll
-              for (int b = 0; b < 4; ++b) {
-                const int byte = b * GROUPS + g;
-                word |= (codes[j][byte / 4] >> (8 * (byte % 4)) & 0xffu) << (8 * b);
+                for (int b = 0; b < 4; ++b) {
+                  const int byte = b * GROUPS + g;
+                  word |= (codes[j][byte / 4] >> (8 * (byte % 4)) & 0xffu) << (8 * b);
+                }
               }
             }
-            step = v_step == v_step ? v_step : 0.f;
-          } else {
-            word = codes[j][g];
-            // (0 times a step, which is finite or no number)
-            step = fmaf(v_step, 0.f, __uint_as_float(steps[j][g / 2] >> (16 * (g % 2)) << 16));
+            float step = __uint_as_float(steps[j][g / 2] >> (16 * (g % 2)) << 16);
+            if constexpr (turned.value) {
+              no_number = fmaf(step, 0.f, no_number);
+              step = __builtin_isfinite(step) ? step : 0.f;
+            }
+            int slot = piece + turn;
+            slot = slot >= CH ? slot - CH : slot;
+            *reinterpret_cast<u32x4*>(row + slot * 16) = values_of(word, step);
           }
-          int slot = piece + turn;
-          slot = slot >= CH ? slot - CH : slot;
-          *reinterpret_cast<u32x4*>(row + slot * 16) = values_of(word, step);
-        }
+        };
+        if (is_value) store_row(std::true_type());
+        else store_row(std::false_type());
       }
     }
   };
@@ -501,17 +504,17 @@ __device__ __forceinline__ void attention_prefill_block(
       }
     }
   };
-  // scores of a wave's keys that have no page, eight at a time (pages hold a multiple of 8)
-  auto hide_absent = [&](const int kw, f32x16 (&s)[KR]) {
+  // which eights of a wave's keys have no page (pages hold a multiple of 8), a bit each
+  auto absent_keys = [&](const int kw) {
+    uint32_t absent = 0;
+    if (Pages::INT4 && __builtin_expect(holes, 0)) {
 #pragma unroll
-    for (int r = 0; r < KR; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int entry = prefill_entry(prefill_key(keys, kw + 32 * r + 8 * i), page_size, page_shift) - keys.first_entry;
-        if (__builtin_amdgcn_readfirstlane(s_table[entry]) != AP_NO_PAGE) continue;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[r][4 * i + e] = -INFINITY;
+      for (int i = 0; i < WAVE_KEYS / 8; ++i) {
+        const int entry = prefill_entry(prefill_key(keys, kw + 8 * i), page_size, page_shift) - keys.first_entry;
+        absent |= (uint32_t)(__builtin_amdgcn_readfirstlane(s_table[entry]) == AP_NO_PAGE) << i;
       }
+    }
+    return absent;
   };
   // softmax of a wave's scores of one tile and the second product (the values' reads may
   // still be in flight when it starts)
@@ -531,7 +534,17 @@ __device__ __forceinline__ void attention_prefill_block(
       float tile_max = -INFINITY;
       if (__builtin_amdgcn_readfirstlane(__any(masked) ? 1 : 0)) {
         const int q_first = q_valid ? first_visible_key(q_pos, window) : 0;
-        if (Pages::INT4 && holes) hide_absent(kw, s);
+        const uint32_t absent = absent_keys(kw);
+        if (Pages::INT4 && __builtin_expect(absent != 0, 0)) {
+#pragma unroll
+          for (int r = 0; r < KR; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if ((absent >> (4 * r + i) & 1u) == 0) continue;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[r][4 * i + e] = -INFINITY;
+            }
+        }
 #pragma unroll
         for (int r = 0; r < KR; ++r)
 #pragma unroll
@@ -685,6 +698,17 @@ __device__ __forceinline__ void attention_prefill_block(
     weigh(kw, s, vr);
   }
 
+  // over a cache in 4 bits: whether any thread of the block met a value that is no number
+  bool any_no_number = false;
+  if constexpr (Pages::INT4) {
+    ap_wait_loads_and_sync<0>();               // every wave is past its last operand reads
+    const bool wave_no_number = __builtin_amdgcn_ballot_w64(no_number != no_number) != 0;
+    if (lane == 0) found[wave] = wave_no_number;
+    __syncthreads();
+    any_no_number = __builtin_amdgcn_ballot_w64(lane < AP_WAVES && found[lane % AP_WAVES] != 0) != 0;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // (read, before states take its place)
+  }
+
   // ---- the KS states of a query are merged by the wave with the first run of keys.  The
   // accumulators of waves with the same queries have the same layout, so lane meets lane.
   if (KS > 1) {
@@ -718,6 +742,40 @@ __device__ __forceinline__ void attention_prefill_block(
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           acc[db][e] = acc[db][e] * c_mine + theirs[(2 + db * 16 + e) * 64] * c_theirs;
+    }
+  }
+
+  if constexpr (Pages::INT4) {
+    if (__builtin_expect(any_no_number, 0)) {
+      // The values' steps once more, of 64 keys at a time: the sums of a query that sees one which is no number are none in
+      // its group's dimensions.
+      const int q_first = q_valid ? first_visible_key(q_pos, window) : 0;
+      const int from = k_first > key_begin ? k_first : key_begin;
+      const int behind = k_first + tiles * AP_KEYS < key_end ? k_first + tiles * AP_KEYS : key_end;
+      uint32_t bad = 0;
+#pragma unroll 1
+      for (int base = from; base < behind; base += 64) {
+        const int key = base + lane < behind ? base + lane : behind - 1;
+        uint32_t page_row, mine = 0;
+        int within;
+        place_of(key, page_row, within);
+        const bool there = s_table[prefill_entry(key, page_size, page_shift) - keys.first_entry] != AP_NO_PAGE;
+        const uint16_t* at = reinterpret_cast<const uint16_t*>(v_pool + (uint64_t)page_row * (18 * GROUPS) +
+                                                               page_size * (16 * GROUPS)) + within * GROUPS;
+#pragma unroll 1
+        for (int g = 0; g < GROUPS; ++g) mine |= (uint32_t)(there && (at[g] & 0x7fffu) >= 0x7f80u) << g;
+        uint64_t left = __builtin_amdgcn_ballot_w64(mine != 0 && base + lane < behind);
+        while (left != 0) {
+          const int i = __builtin_ctzll(left);
+          left &= left - 1;
+          const uint32_t groups = __builtin_amdgcn_readlane(mine, i);
+          bad |= base + i <= q_last && base + i >= q_first ? groups : 0u;
+        }
+      }
+#pragma unroll
+      for (int db = 0; db < NDB32; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[db][e] = bad >> db & 1u ? __uint_as_float(0x7fc00000u) : acc[db][e];
     }
   }
 

@@ -124,3 +124,64 @@ def test_pages_that_the_table_does_not_have(kind, group, dim, page, counts, star
     kernels.attention_decode_int4(q.cuda(), *pools, out, _ints(items), _ints(positions), tables.cuda(), heads, dim ** -0.5, 1,
                                   None, window, sink=sinks)
     _check(out, expected, kind, "single tokens")
+
+
+NO_NUMBER = [
+    # group, dim, page, count, start, window, (position, head, group of dimensions; None: a key's) of what is no number
+    (1, 64, 16, 70, 100, 0, ((3, 0, 1), (150, 1, 0))), (2, 128, 8, 66, 30, 0, ((95, 0, 3), (40, 1, 2), (41, 1, 0))),
+    (1, 64, 24, 130, 0, 40, ((60, 0, 0), (61, 0, 1))), (2, 48, 16, 40, 60, 0, ((70, 1, 1), (99, 0, 0))),
+    (1, 256, 32, 70, 200, -64, ((210, 0, 7), (255, 1, 4), (256, 1, 0))), (2, 128, 64, 129, 300, 0, ((310, 0, 1), (0, 1, 3))),
+    (1, 16, 8, 65, 8, 0, ((20, 0, 0), (72, 1, 0))), (1, 96, 16, 50, 70, 0, ((90, 0, 2), (100, 0, None), (33, 1, 1))),
+    (1, 32, 8, 70, 0, 0, ((0, 0, 0), (35, 1, None)))]
+
+
+def _no_number(kind, group, dim, page, count, start, window, bad):
+    from pagedserve_amd.ops import kernels
+
+    heads, length = 2 * group, start + count
+    tables, pages, items, positions = _requests((count,), (start,), page, 91)
+    pools, ((k, v),) = _cache(tables, pages, (length,), 2, dim, page, 92)
+    rows = [k.float(), v.float()]
+    for position, head, which in bad:
+        rows[which is not None][position, head * dim + 32 * (which or 0) + 5] = math.nan
+    index = (_ints([0] * length), _ints(list(range(length))), tables.cuda())
+    kernels.kv_write_int4(rows[0].cuda(), rows[1].cuda(), *pools, *index)
+    kept = [plain.held(part, 2)[2] for part in rows]
+    q = torch.randn((count, heads * dim), generator=torch.Generator().manual_seed(93)).to(kind)
+    expected = list(plain.attention(q, *kept, positions, heads, dim ** -0.5, window))
+    share = float(expected[0].isnan().double().mean())
+    assert 0 < share < 0.9
+    for form, run in _portions(kind, dim, group):
+        print(form, flush=True)
+        out = torch.full((count, heads * dim), -9.0, dtype=kind).cuda()
+        run(q.cuda(), pools, out, (count,), (length,), tables.cuda(), heads, window)
+        _check(out, expected, kind, form)
+    out = torch.zeros((count, heads * dim), dtype=kind).cuda()
+    kernels.attention_decode_int4(q.cuda(), *pools, out, _ints(items), _ints(positions), tables.cuda(), heads, dim ** -0.5, 1,
+                                  None, window)
+    _check(out, expected, kind, "single tokens")
+
+
+@pytest.mark.parametrize("group,dim,page,count,start,window,bad", NO_NUMBER)
+def test_what_is_no_number_stays_where_it_is(group, dim, page, count, start, window, bad):
+    """A value's group that is no number makes these dimensions of its head so, for the queries that see it; a key, the head's."""
+    _no_number(BF16, group, dim, page, count, start, window, bad)
+
+
+def test_infinities_in_the_place_of_a_missing_page():
+    """What nobody wrote may be anything, steps that are infinite among them, and page 0 may be such a page."""
+    dim, page, count, start = 64, 16, 70, 40
+    tables, pages, _, positions = _requests((count,), (start,), page, 85)
+    tables[(tables >= 0) & (tables < pages)] += 1                           # (page 0 is nobody's)
+    pools, ((k, v),) = _cache(tables, pages + 1, (start + count,), 2, dim, page, 86)
+    for pool in pools:
+        pool[0].view(2, -1)[:, page * 32:] = torch.tensor([0x80, 0x7f], dtype=torch.uint8).repeat(page * 2).cuda()
+    tables[0, 3] = -1
+    q = torch.randn((count, 2 * dim), generator=torch.Generator().manual_seed(87)).to(BF16)
+    seen = plain.visible
+    with mock.patch.object(plain, "visible", lambda at, key, window: seen(at, key, window) and key // page != 3):
+        expected = list(plain.attention(q, k, v, positions, 2, dim ** -0.5))
+    for form, run in _portions(BF16, dim):
+        out = torch.full((count, 2 * dim), -9.0, dtype=BF16).cuda()
+        run(q.cuda(), pools, out, (count,), (start + count,), tables.cuda(), 2)
+        _check(out, expected, BF16, form)
