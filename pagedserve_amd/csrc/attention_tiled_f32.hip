@@ -58,8 +58,10 @@ struct AfPool<true> {
 
 // DF: 32 head dimensions each; RAGGED: the head size is not 32 DF; PAIRS: one block takes the 64 queries of a tile,
 // two waves to 32 of them; `parts`: else, blocks to a listed tile (of 32 queries each); INT4: a cache in 4 bits
+// (over codes heads of 65 to 96 dimensions get registers for two waves to a SIMD, eight fewer than they would take: 2 x 1,024
+// tokens of 12 heads of 96 96 us, with one wave 109)
 template <int DF, bool RAGGED, bool PAIRS, bool INT4>
-__global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
+__global__ __launch_bounds__(64 * AF_WAVES, INT4 && DF == 3 ? 2 : 1) void attention_tiled_f32_kernel(
     const float* __restrict__ q, int64_t q_stride, const typename AfPool<INT4>::Element* __restrict__ k_pool,
     const typename AfPool<INT4>::Element* __restrict__ v_pool, float* __restrict__ out, int64_t out_stride,
     const int* __restrict__ tile_item, const int* __restrict__ tile_q0,
@@ -125,7 +127,7 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
     const int logical = key / page_size, within = key - logical * page_size;
     const bool there = key < key_end && logical < table_width && page >= 0 && page < num_pages;
     if constexpr (INT4) {
-      to_steps = there ? page_size * (16 * DF) - within * (14 * DF) : 0;
+      to_steps = page_size * (16 * DF) - (there ? within * (14 * DF) : 0);
       const int64_t row = int4_page_at(page, kv_heads, kv_head, page_size, DF) + within * (16 * DF);
       return there ? row : -1;
     }
@@ -134,10 +136,10 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
   };
   af_f32x4 key_values[INT4 ? 1 : STEPS];
   float values[DF][16];
-  // a key's words, its steps and those of its value; of 16 values a byte per group and the steps
+  // a key's words and its steps; of 16 values a byte per group and the steps
   constexpr int BYTES = DF == 3 ? 3 : 1, STEP_WORDS = DF == 4 ? 2 : DF == 3 ? 3 : 1;
   uint4 key_codes[INT4 ? DF : 1];
-  uint32_t key_steps[INT4 ? STEP_WORDS : 1], poison[INT4 ? STEP_WORDS : 1];
+  uint32_t key_steps[INT4 ? STEP_WORDS : 1];
   uint32_t value_codes[INT4 ? 16 : 1][BYTES], value_steps[INT4 ? 16 : 1][STEP_WORDS];
   auto load_steps = [&](const uint8_t* from, uint32_t (&words)[STEP_WORDS]) {
     if constexpr (DF == 4) {
@@ -162,7 +164,6 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
 #pragma unroll
       for (int g = 0; g < DF; ++g) key_codes[g] = reinterpret_cast<const uint4*>(source)[g];
       load_steps(source + to_steps, key_steps);
-      load_steps(v_pool + (row < 0 ? 0 : row) + to_steps, poison);
     } else {
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
@@ -177,9 +178,7 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
       const int g = s / 4, w = (s % 4) * DF + g;
       const uint32_t words[4] = {key_codes[w / 4].x, key_codes[w / 4].y, key_codes[w / 4].z, key_codes[w / 4].w};
       const uint32_t codes = words[w % 4] >> (16 * half);
-      // A value that is no number must not reach the queries that do not see its key, whose weight of 0 would still make
-      // it one: it is 0 below, and the key takes its place here, whose scores are masked.
-      const float step = fmaf(step_of(poison, g), 0.f, step_of(key_steps, g)), base = -8.f * step;
+      const float step = step_of(key_steps, g), base = -8.f * step;
       af_f32x4 piece;
 #pragma unroll
       for (int i = 0; i < 4; ++i) piece[i] = fmaf((float)(codes >> (4 * i) & 15u), step, base);
@@ -216,8 +215,17 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
       }
     }
   };
+  // A value that is no number must not reach the queries that do not see its key: their weight of 0 would still make it one.
+  // It is 0 in the product, and the largest magnitude of all steps, as a number of its bits, says at the end that there was one.
+  typedef uint16_t two __attribute__((ext_vector_type(2)));
+  two largest = {0, 0};
   auto convert_values = [&]() {
     if constexpr (INT4) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+#pragma unroll
+        for (int w = 0; w < STEP_WORDS; ++w)
+          largest = __builtin_elementwise_max(largest, __builtin_bit_cast(two, value_steps[e][w] & 0x7fff7fffu));
 #pragma unroll
       for (int e = 0; e < 16; ++e)
 #pragma unroll
@@ -336,6 +344,37 @@ __global__ __launch_bounds__(64 * AF_WAVES) void attention_tiled_f32_kernel(
     for (int g = 0; g < 4; ++g)
       *reinterpret_cast<float4*>(mine + 32 * f + 8 * g + 4 * half) =
           make_float4(acc[f][4 * g], acc[f][4 * g + 1], acc[f][4 * g + 2], acc[f][4 * g + 3]);
+  if constexpr (INT4) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(largest.x > 0x7f80 || largest.y > 0x7f80) != 0, 0)) {
+      // The steps of the wave's values once more: the sums of a query that sees one which is no number are none in its
+      // group's dimensions.
+      uint32_t bad = 0;
+#pragma unroll 1
+      for (int from = key_begin + turn * AF_ROWS; from < key_end; from += TURNS * AF_ROWS) {
+        int to_steps = 0;
+        const int64_t row = row_of(from, page_of(from), to_steps);
+        const uint16_t* at = reinterpret_cast<const uint16_t*>(v_pool + (row < 0 ? 0 : row) + to_steps);
+        uint32_t found = 0;
+#pragma unroll
+        for (int g = 0; g < DF; ++g) found |= (uint32_t)(row >= 0 && (at[g] & 0x7fffu) > 0x7f80u) << g;
+        uint32_t left = (uint32_t)__builtin_amdgcn_ballot_w64(found != 0);      // (both halves ask for the same keys)
+        while (left != 0) {
+          const int i = __builtin_ctz(left);
+          left &= left - 1;
+          const uint32_t groups = __builtin_amdgcn_readlane(found, i);
+          bad |= from + i <= q_pos && from + i >= q_first ? groups : 0u;
+        }
+      }
+      const float none = __uint_as_float(0x7fc00000u);
+#pragma unroll 1
+      for (int f = 0; f < DF; ++f) {
+        if ((bad >> f & 1u) == 0) continue;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(mine + 32 * f + 8 * g + 4 * half) = make_float4(none, none, none, none);
+      }
+    }
+  }
   if (half == 0) {
     s_max[wave * AF_ROWS + column] = run_max;
     s_sum[wave * AF_ROWS + column] = run_sum;

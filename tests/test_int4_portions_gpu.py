@@ -185,3 +185,8 @@ def test_infinities_in_the_place_of_a_missing_page():
         out = torch.full((count, 2 * dim), -9.0, dtype=BF16).cuda()
         run(q.cuda(), pools, out, (count,), (start + count,), tables.cuda(), 2)
         _check(out, expected, BF16, form)
+
+
+@pytest.mark.parametrize("group,dim,page,count,start,window,bad", [case for case in NO_NUMBER if case[1] <= 128])
+def test_what_is_no_number_stays_where_it_is_in_float(group, dim, page, count, start, window, bad):
+    _no_number(F32, group, dim, page, count, start, window, bad)
