@@ -797,8 +797,9 @@ __device__ __forceinline__ void attention_prefill_block(
     return;
   }
   // element e of an accumulator: head dimension db*32 + (e/4)*8 + half*4 + e%4 of query `sub`
-  if (q_valid && l != 0.f) {
-    const float inv = gate_factor(extra, tok0 + qi, head) / l;
+  // (of a query that sees nothing: over a cache in 4 bits zeros, as single tokens get them, else nothing)
+  if (q_valid && (Pages::INT4 || l != 0.f)) {
+    const float inv = Pages::INT4 && l == 0.f ? 0.f : gate_factor(extra, tok0 + qi, head) / l;
     bf16_t* dst = out + (int64_t)(tok0 + qi) * out_stride + (int64_t)head * HD;
 #pragma unroll
     for (int db = 0; db < NDB32; ++db)

@@ -69,8 +69,7 @@ __global__ __launch_bounds__(256) void attention_prefill_int4_join_kernel(
     x[2] = fmaf(v.z, c, x[2]);
     x[3] = fmaf(v.w, c, x[3]);
   }
-  if (total == 0.f) return;                // (a query that sees nothing: its row stays, as without ranges)
-  const float inv = 1.f / total;
+  const float inv = total == 0.f ? 0.f : 1.f / total;        // (a query that sees nothing: zeros)
   *reinterpret_cast<uint2*>(out + (tok0 + row) * out_stride + (int64_t)head * head_dim + d) =
       make_uint2(pack2_bf16(x[0] * inv, x[1] * inv), pack2_bf16(x[2] * inv, x[3] * inv));
 }

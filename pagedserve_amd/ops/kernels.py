@@ -1575,8 +1575,8 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
     ``block_heads``: 1 or 2 heads to a block (None: ``prefill_int4_block_heads(...)``).  ``ranges``: parts of the keys of
     every tile, joined by a second launch (None: ``prefill_int4_ranges(...)``, one where ``max_kv_len`` is not given); with
     more than one ``partial`` is float scratch of ``tiles * heads * ranges * query_tile * (head_dim + 2)`` values, allocated for the call where it is None.
-    As for single tokens, keys whose table entry lies outside the pool are seen by nobody, and positions behind the block table
-    see what the table has."""
+    As for single tokens, keys whose table entry lies outside the pool are seen by nobody, positions behind the block table
+    see what the table has, and a query that sees no key gets zeros."""
     _check_prefill_constants()
     addresses, sizes, sink_at, device = _int4_tiles("attention_prefill_int4", q, k_pool, v_pool, out, tile_item, tile_q0,
                                                     cu_tokens, kv_lens, tables, heads, sink, torch.bfloat16)
@@ -1601,7 +1601,8 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
 
 def attention_tiled_f32_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_lens, tables, heads, scale,
                              window=0, sink=None, softcap=0.0, query_tile=PREFILL_TILE, paired=False):
-    """``attention_tiled_f32`` over a cache in 4 bits (``tiled_f32_supported``, ``tiled_f32_shape``)."""
+    """``attention_tiled_f32`` over a cache in 4 bits (``tiled_f32_supported``, ``tiled_f32_shape``); missing pages, positions
+    behind the block table and queries that see no key as in ``attention_prefill_int4``."""
     addresses, sizes, sink_at, _ = _int4_tiles("attention_tiled_f32_int4", q, k_pool, v_pool, out, tile_item, tile_q0,
                                                cu_tokens, kv_lens, tables, heads, sink, torch.float32)
     _call("ps_attention_tiled_f32_int4", *addresses, *sizes, float(scale), int(window), sink_at, _check_cap(softcap),

@@ -190,3 +190,20 @@ def test_infinities_in_the_place_of_a_missing_page():
 @pytest.mark.parametrize("group,dim,page,count,start,window,bad", [case for case in NO_NUMBER if case[1] <= 128])
 def test_what_is_no_number_stays_where_it_is_in_float(group, dim, page, count, start, window, bad):
     _no_number(F32, group, dim, page, count, start, window, bad)
+
+
+@pytest.mark.parametrize("kind", [BF16, F32])
+@pytest.mark.parametrize("dim,sink", [(64, False), (128, False), (64, True)])
+def test_queries_that_see_nothing(kind, dim, sink):
+    """Windows behind the table's end, pages that it does not have, a sink of minus infinity: zeros, as single tokens get them."""
+    tables, pages, _, _ = _requests((1, 1), (79, 79), 16, 95)
+    tables = tables[:, :5].contiguous()
+    pools, _ = _cache(tables, pages, (80, 80), 2, dim, 16, 96)
+    tables[1] = -1
+    q = torch.randn((140, 2 * dim), generator=torch.Generator().manual_seed(97)).to(kind)
+    sinks = torch.full((2,), -math.inf).cuda() if sink else None
+    for form, run in _portions(kind, dim):
+        out = torch.full((141, 2 * dim), -9.0, dtype=kind).cuda()
+        run(q.cuda(), pools, out[:140], (70, 70), (160, 80), tables.cuda(), 2, 12, sinks)      # (at 90 .. and 10 ..)
+        assert torch.equal(out[1:140], torch.zeros_like(out[1:140])), form
+        assert bool((out[:1] != 0).any()) and bool((out[140] == -9.0).all()), form
