@@ -633,12 +633,10 @@ __global__ __launch_bounds__(256) void attention_decode_int4_kernel(
   const int word = has_word ? w : 0;
   const int key_at = int4_key_word(word, groups);
   float query[8];
-  float query_sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int d = 8 * w + i;
     query[i] = d < head_dim ? to_float(q[t * q_stride + (int64_t)head * head_dim + d]) : 0.f;
-    query_sum += query[i];
   }
 
   // (a token in front of its context sees nothing, and reads no entry of the table)

@@ -599,3 +599,29 @@ def test_as_a_bfloat16_cache_of_the_values_held():
         limit = plain.allowed(*e, BF16, True)
         for out in outs:
             assert bool(((out[t:t + 1] - e[0]).abs() <= limit).all())
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,window,sink,softcap", [
+    (16, 2, 1, 0, False, 0.0), (32, 1, 2, 0, True, 0.0), (48, 2, 3, 30, False, 0.0), (64, 1, 4, -16, False, 20.0),
+    (128, 2, 1, 0, True, 0.0), (250, 1, 2, 0, False, 0.0)])
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+@pytest.mark.parametrize("kind", [BF16, F32])
+def test_scales_that_are_not_positive(kind, scale, dim, kv_heads, group, window, sink, softcap):
+    """Bfloat16 queries take another kernel under such a scale, a head to a block."""
+    from pagedserve_amd.ops import kernels
+
+    heads, lengths, page = kv_heads * group, (1, 17, 200, 530), 16
+    tables, pages, _, _ = _requests([1] * len(lengths), [length - 1 for length in lengths], page, 101)
+    pools, kept = _cache(tables, pages, lengths, kv_heads, dim, page, 102)
+    q = torch.randn((len(lengths), heads * dim), generator=torch.Generator().manual_seed(103)).to(kind)
+    sinks = torch.randn(heads, generator=torch.Generator().manual_seed(104)).cuda() if sink else None
+    expected = [list(plain.attention(q[i:i + 1], *kept[i], [length - 1], heads, scale, window, sinks, softcap))
+                for i, length in enumerate(lengths)]
+    expected = [torch.cat([e[which] for e in expected]) for which in range(3)]
+    limit = plain.allowed(*expected, kind, False)
+    for splits in (1, 3):
+        out = torch.full((len(lengths), heads * dim), -9.0, dtype=kind).cuda()
+        kernels.attention_decode_int4(q.cuda(), *pools, out, None, _ints([length - 1 for length in lengths]), tables.cuda(), heads,
+                                      scale, splits, torch.full((len(lengths) * heads * splits * (dim + 2),), math.nan).cuda(),
+                                      window, sink=sinks, softcap=softcap)
+        assert bool(((out.double().cpu() - expected[0]).abs() <= limit).all()), splits
