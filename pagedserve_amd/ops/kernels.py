@@ -1334,7 +1334,7 @@ def _rows_on(tensor, name, dtype, device):
     try:
         if tensor.dtype is dtype and tensor.get_device() == device:
             stride, step = tensor.stride()
-            if step == 1 and tensor.numel() > stride:         # (more than one row)
+            if step == 1 and tensor.numel() > stride >= tensor.size(1):       # (more than one row, which do not overlap)
                 return tensor.data_ptr(), stride
             return tensor.data_ptr(), _rows(tensor, name)
     except (AttributeError, ValueError):

@@ -1,0 +1,31 @@
+"""Rows of unusual strides at the faces of the operators of a cache in 4 bits and of the log probabilities, without a GPU."""
+
+from unittest import mock
+
+import pytest
+import torch
+
+from pagedserve_amd.ops import kernels
+from test_int4 import BF16, _c, _decode, _float_prompt, _ints, _logprobs, _prompt, _write, on_gpu  # noqa: F401
+
+
+def _calls(function, args):
+    found = []
+    with mock.patch.object(kernels, "_call", lambda name, *given: found.append(given)):
+        function(**args)
+    return found[0]
+
+
+def test_a_single_row_is_as_long_as_its_stride(on_gpu):  # noqa: F811
+    """The stride of a single row means nothing: a column that was turned has 1."""
+    def turned(n, kind=torch.float32):
+        row = torch.zeros(n, dtype=kind).view(n, 1).t()
+        assert row.shape == (1, n) and row.stride() == (1, 1)
+        return row
+
+    given = _calls(kernels.kv_write_int4, _write(k=turned(128), v=turned(128), tok_item=_ints(1), tok_pos=_ints(1)))
+    assert given[2:4] == (128, 128)
+    given = _calls(kernels.attention_decode_int4, _decode(q=turned(256, BF16), out=turned(256, BF16), tok_item=_ints(1), tok_pos=_ints(1)))
+    assert given[1] == given[9] == 256
+    given = _calls(kernels.token_logprobs, _logprobs(logits=turned(50), tokens=_ints(1), out=torch.zeros(1)))
+    assert given[1:4] == (50, 1, 50)
