@@ -1469,6 +1469,8 @@ def attention_decode_int4(q, k_pool, v_pool, out, tok_item, tok_pos, tables, hea
     k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, columns, heads, device)
     if out.shape != shape:
         raise KernelError("attention_decode_int4: q and out rows must hold heads x head_dim values")
+    if out_stride < columns:
+        raise KernelError("attention_decode_int4: rows of out overlap")
     item_at, pos_at, tables_at, width = _token_index(tok_item, tok_pos, tables, tokens, device, direct_items=True)
     list_at, count = 0, tokens
     if tok_list is not None:
@@ -1552,6 +1554,8 @@ def _int4_tiles(what, q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens, kv_
     k_at, v_at, pages, kv_heads, page_size, head_dim = _int4_pools(k_pool, v_pool, columns, heads, device)
     if out.shape != shape:
         raise KernelError(f"{what}: q and out rows must hold heads x head_dim values")
+    if out_rows[1] < columns:
+        raise KernelError(f"{what}: rows of out overlap")
     index = (_dense(tile_item, "tile_item", torch.int32, 1, device), _dense(tile_q0, "tile_q0", torch.int32, 1, device),
              _dense(cu_tokens, "cu_tokens", torch.int32, 1, device), _dense(kv_lens, "kv_lens", torch.int32, 1, device),
              _dense(tables, "tables", torch.int32, 2, device))

@@ -29,3 +29,17 @@ def test_a_single_row_is_as_long_as_its_stride(on_gpu):  # noqa: F811
     assert given[1] == given[9] == 256
     given = _calls(kernels.token_logprobs, _logprobs(logits=turned(50), tokens=_ints(1), out=torch.zeros(1)))
     assert given[1:4] == (50, 1, 50)
+
+
+@pytest.mark.parametrize("function,args,kind", [(kernels.attention_decode_int4, _decode, BF16),
+                                                (kernels.attention_prefill_int4, _prompt, BF16),
+                                                (kernels.attention_tiled_f32_int4, _float_prompt, torch.float32)])
+def test_results_that_overlap_are_refused(on_gpu, function, args, kind):  # noqa: F811
+    """Queries may share a row, results may not."""
+    row = torch.zeros(256, dtype=kind)
+    function(**args(q=row.expand(3, 256)))
+    assert len(on_gpu) == 1
+    for out in (row.expand(3, 256), torch.zeros(600, dtype=kind).as_strided((3, 256), (8, 1))):
+        with pytest.raises(kernels.KernelError, match="overlap"):
+            function(**args(out=out))
+    assert len(on_gpu) == 1
