@@ -407,7 +407,7 @@ extern "C" int ps_token_logprobs(const void* logits, int64_t ld, int rows, int v
                                  float* logprobs, float* entropy, int* ranks, int* top_ids, float* top_logprobs,
                                  int top, float* partial, int64_t partial_floats, int dtype, void* stream) {
   const char* who = "ps_token_logprobs";
-  PS_REQUIRE(rows >= 0 && vocab > 0 && ld >= vocab, "%s: bad sizes", who);
+  PS_REQUIRE(rows >= 0 && vocab > 0 && (ld >= vocab || ld == 0), "%s: bad sizes", who);     // (0: one row for all tokens)
   PS_REQUIRE(dtype == PS_F32 || dtype == PS_BF16, "%s: unknown dtype %d", who, dtype);
   PS_REQUIRE(top >= 0 && top <= LP_MAX_TOP && top <= vocab, "%s: 0 to %d alternatives out of a vocabulary of %d, not %d",
              who, LP_MAX_TOP, vocab, top);

@@ -2739,7 +2739,8 @@ def logprob_scratch(rows, vocab, top) -> int:
 
 
 def token_logprobs(logits, tokens, out, entropy=None, ranks=None, top_ids=None, top_logprobs=None, partial=None):
-    """out[r] = log softmax(logits[r])[tokens[r]] (float or bfloat16 logits, rows of any stride, one token each).
+    """out[r] = log softmax(logits[r])[tokens[r]] (float or bfloat16 logits, rows of any stride that does not make them overlap, or
+    one row expanded to all, one token each).
 
     ``entropy``: the entropy of each row's distribution, in natural units.  ``ranks``: how many tokens of the row are
     more likely than the given one (among equals the lower ids are).  ``top_ids`` and ``top_logprobs`` ([rows, top], int32 and float, top

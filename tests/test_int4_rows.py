@@ -43,3 +43,13 @@ def test_results_that_overlap_are_refused(on_gpu, function, args, kind):  # noqa
         with pytest.raises(kernels.KernelError, match="overlap"):
             function(**args(out=out))
     assert len(on_gpu) == 1
+
+
+def test_a_row_of_logits_for_many_tokens(on_gpu):  # noqa: F811
+    """One distribution, several tokens asked about: the library takes rows that are all the same one."""
+    given = _calls(kernels.token_logprobs, _logprobs(logits=torch.zeros(50).expand(3, 50)))
+    assert given[1:4] == (0, 3, 50)
+    # (scratch, which is missing, is asked for after the sizes)
+    for ld, vocab, message in ((0, 200000, "too few"), (200000, 200000, "too few"), (199999, 200000, "bad sizes"), (-50, 50, "bad sizes")):
+        status, error = _c("ps_token_logprobs", 0, ld, 3, vocab, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        assert status == 1 and message in error
