@@ -1578,7 +1578,8 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
     """``attention_prefill`` over a cache in 4 bits (bfloat16 queries, head sizes in multiples of 16).
     ``block_heads``: 1 or 2 heads to a block (None: ``prefill_int4_block_heads(...)``).  ``ranges``: parts of the keys of
     every tile, joined by a second launch (None: ``prefill_int4_ranges(...)``, one where ``max_kv_len`` is not given); with
-    more than one ``partial`` is float scratch of ``tiles * heads * ranges * query_tile * (head_dim + 2)`` values, allocated for the call where it is None.
+    more than one ``partial`` is float scratch of ``tiles * heads * ranges * query_tile * (head_dim + 2)`` values, allocated for the call where
+    it is None (an error while a ``StepGraph`` is recorded, whose replays would write to memory that was given back).
     As for single tokens, keys whose table entry lies outside the pool are seen by nobody, positions behind the block table
     see what the table has, and a query that sees no key gets zeros."""
     _check_prefill_constants()
@@ -1596,6 +1597,9 @@ def attention_prefill_int4(q, k_pool, v_pool, out, tile_item, tile_q0, cu_tokens
         if query_tile not in (PREFILL_TILE, PREFILL_LARGE_TILE):
             raise KernelError(f"attention_prefill_int4: tiles of {PREFILL_TILE} or {PREFILL_LARGE_TILE} queries, not {query_tile}")
         if partial is None:
+            if StepGraph.recording:
+                raise KernelError("attention_prefill_int4: a recorded call with ranges needs scratch that its replays find "
+                                  "unused by anybody else: give it as partial")
             partial = torch.empty(tiles * heads * ranges * query_tile * (head_dim + 2), dtype=torch.float32, device=q.device)
         partial_at, floats = _dense(partial, "partial", torch.float32, None, device), partial.numel()
     _call("ps_attention_prefill_int4", *addresses, *sizes, float(scale), int(window), max_kv_len, query_tile, sink_at,
@@ -2787,6 +2791,8 @@ class StepGraph:
     """An executable HIP graph of the launches issued between ``begin`` and ``end`` on the
     current (non-default) stream."""
 
+    recording = False      # between ``begin`` and ``end`` (or ``abort``)
+
     def __init__(self):
         self.handle = None
         self.nodes = 0
@@ -2799,8 +2805,10 @@ class StepGraph:
         lib.ps_graph_begin.restype = c_int
         if lib.ps_graph_begin(_stream()) != 0:
             raise KernelError(lib.ps_last_error().decode())
+        StepGraph.recording = True
 
     def end(self):
+        StepGraph.recording = False
         lib = load_library()
         lib.ps_graph_end.argtypes = [c_void_p, ctypes.POINTER(c_void_p), ctypes.POINTER(c_int)]
         lib.ps_graph_end.restype = c_int
@@ -2813,6 +2821,7 @@ class StepGraph:
 
     @staticmethod
     def abort():
+        StepGraph.recording = False
         lib = load_library()
         lib.ps_graph_abort.argtypes = [c_void_p]
         lib.ps_graph_abort(_stream())
