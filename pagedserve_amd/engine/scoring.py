@@ -56,8 +56,9 @@ class _Rows:
             self.partial = torch.empty(needed, dtype=torch.float32, device=logits.device)
         ids = self.top_ids[:rows * top].view(rows, top) if top else None
         best = self.top_logprobs[:rows * top].view(rows, top) if top else None
-        kernels.token_logprobs(logits, self.tokens[:rows], self.floats[0, :rows], self.floats[1, :rows], self.ranks[:rows],
-                               ids, best, self.partial)
+        with torch.cuda.device_of(logits):         # (the engine's, which need not be the current one)
+            kernels.token_logprobs(logits, self.tokens[:rows], self.floats[0, :rows], self.floats[1, :rows], self.ranks[:rows],
+                                   ids, best, self.partial)
         alternatives = [None] * rows
         if top:
             alternatives = [list(zip(*pair)) for pair in zip(ids.tolist(), best.tolist())]
