@@ -172,6 +172,8 @@ class CacheManager:
                 raise ValueError(f"pages of a cache in 4 bits hold a multiple of 8 keys, not {page_size}")
             if any(group.values_in_keys or group.value_head_dim != group.head_dim for group in groups):
                 raise ValueError("a cache in 4 bits holds values of their own, of the keys' head size")
+            if any(group.head_dim > 256 for group in groups):
+                raise ValueError(f"a cache in 4 bits holds heads of up to 256 dimensions, not {max(g.head_dim for g in groups)}")
         self.cache_format = cache_format
         if max_slots <= 0:
             raise ValueError("max_slots must be positive")
