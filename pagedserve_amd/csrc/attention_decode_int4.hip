@@ -13,14 +13,16 @@
 //            score passes it by more than 2^8, so that most tiles need no exchange between lanes and no rescaling.
 //   values   O^T[dimension][head] = V^T P^T over the 32 keys, which are the lane's own 8 and those of three others: no
 //            exchange here either.  The weights are multiplied by the group's step before they are rounded to bfloat16 (2^-9 of
-//            each on average); the codes are 16 + code again, and a product of ones with the same weights gives what
-//            is to be taken off, 24 times, at the end.
+//            each on average); the codes are 16 + code again, and a product of -24 in all places with the same weights
+//            comes first, in every tile, and takes off what that is too much.
 //
 // Bound by memory where there are blocks enough (4.5 bits a value), else by the trip block table -> codes: a tile's codes
 // are asked for one tile ahead (Int4Stage), its table entries, which are the same for a wave and come through the scalar
 // unit, two.  32 requests over 8,192 keys, 12 heads of 64: 51 to 54 us, 4.2 to 4.4 TB/s, 85 to 90 % of a large copy's rate
 // (64: 92 us, 4.9 TB/s); 64 over 768 to 1,024, 25 heads that share no keys: 29.4 to 31 us, 3.4 TB/s; 24 over up to 6,000,
-// 16 heads of 128 over 2: 16.1 us; 1 over 900: 5.0 us and 2.0 for the merge.
+// 16 heads of 128 over 2: 16.1 us; 1 over 900: 5.0 us and 2.0 for the merge.  Storing the tokens' own rows as a decode step
+// does (under the profiler, beside the same without): 32 over 8,192 53.8 and 51.6 us, 64 over 768 to 1,024 of 25 heads 34.2 and
+// 31.5, 1 over 900 6.1 and 5.0.
 //
 // float queries, and scales that are not positive, take the kernel on the vector unit: LPK lanes share a key, a lane holds
 // eight dimensions of the query and takes one word of the key's codes; a conversion of the code and a multiply-add to a

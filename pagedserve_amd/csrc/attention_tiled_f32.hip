@@ -27,8 +27,8 @@
 //
 // Over a cache in 4 bits (cache_int4.h) a lane reads its key's whole row of codes, 16 bytes a group, and of a value the
 // byte of its dimension in every group, with the keys' steps; they become floats, exactly, where they are multiplied:
-// 2 x 1,024 tokens of 12 heads of 64 66.5 us (floats 61.8), 512 behind 3,500 keys 161 (128), 512 of 16 heads of 128 over 4
-// behind 2,000 157 (139); token by token 366, 609 and 975.
+// 2 x 1,024 tokens of 12 heads of 64 65.3 us (floats 59.0), 512 behind 3,500 keys 163 (127), 512 of 16 heads of 128 over 4
+// behind 2,000 154 (138); token by token 371, 620 and 983.
 //
 // Head sizes that are multiples of 4 up to 128; others stay with the one-wave-per-token
 // kernel.
@@ -59,7 +59,7 @@ struct AfPool<true> {
 // DF: 32 head dimensions each; RAGGED: the head size is not 32 DF; PAIRS: one block takes the 64 queries of a tile,
 // two waves to 32 of them; `parts`: else, blocks to a listed tile (of 32 queries each); INT4: a cache in 4 bits
 // (over codes heads of 65 to 96 dimensions get registers for two waves to a SIMD, eight fewer than they would take: 2 x 1,024
-// tokens of 12 heads of 96 96 us, with one wave 109)
+// tokens of 12 heads of 96 95 us, with one wave 109)
 template <int DF, bool RAGGED, bool PAIRS, bool INT4>
 __global__ __launch_bounds__(64 * AF_WAVES, INT4 && DF == 3 ? 2 : 1) void attention_tiled_f32_kernel(
     const float* __restrict__ q, int64_t q_stride, const typename AfPool<INT4>::Element* __restrict__ k_pool,

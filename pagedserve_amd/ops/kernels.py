@@ -1458,7 +1458,8 @@ def attention_decode_int4(q, k_pool, v_pool, out, tok_item, tok_pos, tables, hea
                           window=0, tok_list=None, sink=None, softcap=0.0, store=None):
     """``attention_decode`` over a cache in 4 bits, any head size up to 256, float or bfloat16 queries: the same attention over
     the values that the cache stands for.  ``partial``: float scratch of ``count * heads * splits * (head_dim + 2)``
-    values when ``splits > 1``.  A token that sees no key gets zeros.  ``store = (k, v)``: the tokens' own keys and values
+    values when ``splits > 1``.  A token that sees no key gets zeros; keys whose table entry lies outside the pool are seen by
+    nobody.  ``store = (k, v)``: the tokens' own keys and values
     (bfloat16 rows as of ``q``'s tokens), stored first as ``kv_write_int4`` would, in the same launch (8 requests of 12 heads
     of 64 over 130 keys: 6.1 us, in two launches 7.5).  Every token is a request of its own then (neither ``tok_item`` nor
     ``tok_list``: no token sees what another one stores), and the scale is positive."""
