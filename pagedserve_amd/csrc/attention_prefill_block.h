@@ -204,8 +204,15 @@ __device__ __forceinline__ void attention_prefill_block(
     // keys outside the tile's visible range are fetched from a visible key instead: they
     // are masked below, and whatever lies in pages that were given back is never read
     key = prefill_key(keys, key);
-    const int logical = prefill_entry(key, page_size, page_shift);
-    within = page_shift >= 0 ? key & page_mask : key - logical * page_size;
+    // (both in one branch: asked twice, it cost 2 x 4,096 tokens of 12 heads of 64 over bfloat16 pages 89.5 us instead of 84.6)
+    int logical;
+    if (page_shift >= 0) {
+      logical = key >> page_shift;
+      within = key & page_mask;
+    } else {
+      logical = key / page_size;
+      within = key - logical * page_size;
+    }
     page_row = s_table[logical - keys.first_entry];
     if constexpr (Pages::INT4) page_row = page_row == AP_NO_PAGE ? head_rows : page_row;     // (a place that exists)
   };
