@@ -21,8 +21,8 @@
 // unit, two.  32 requests over 8,192 keys, 12 heads of 64: 51 to 54 us, 4.2 to 4.4 TB/s, 85 to 90 % of a large copy's rate
 // (64: 92 us, 4.9 TB/s); 64 over 768 to 1,024, 25 heads that share no keys: 29.4 to 31 us, 3.4 TB/s; 24 over up to 6,000,
 // 16 heads of 128 over 2: 16.1 us; 1 over 900: 5.0 us and 2.0 for the merge.  Storing the tokens' own rows as a decode step
-// does (under the profiler, beside the same without): 32 over 8,192 53.8 and 51.6 us, 64 over 768 to 1,024 of 25 heads 34.2 and
-// 31.5, 1 over 900 6.1 and 5.0.
+// does (under the profiler, beside the same without): 32 over 8,192 53.6 and 52.5 us, 64 over 768 to 1,024 of 25 heads 34.1 and
+// 31.3, 1 over 900 6.1 and 4.9.
 //
 // float queries, and scales that are not positive, take the kernel on the vector unit: LPK lanes share a key, a lane holds
 // eight dimensions of the query and takes one word of the key's codes; a conversion of the code and a multiply-add to a

@@ -7,13 +7,13 @@
 // Bound: the vector instructions of the conversion (3.5 to a value: four bits to a float, one product, half a packing;
 // every block converts what it reads) come on top of those of the softmax, which bound the other cache's kernel.  So a
 // block multiplies what it has converted with as many queries as its registers allow: 128 rows, of one head, or of two
-// that share a key/value head, where the blocks fill the units.  2 x 4,096 tokens of 12 heads of 64: 110 us, 470 TFLOP/s
-// (the other cache 90); 4,096 of 16 heads of 128 142 us, 484 TFLOP/s (64 rows: 188); 16 heads of 128 behind 5,000 keys,
-// 962 tokens, 99 us, 410 TFLOP/s, by pairs of heads and 115 by one (the other cache 92).
+// that share a key/value head, where the blocks fill the units.  2 x 4,096 tokens of 12 heads of 64: 108 us, 478 TFLOP/s
+// (the other cache 85); 4,096 of 16 heads of 128 141 us, 487 TFLOP/s (64 rows: 184); 16 heads of 128 behind 5,000 keys,
+// 962 tokens, 98 us, 415 TFLOP/s, by pairs of heads and 112 by one (the other cache 90).
 //
 // Where the blocks are fewer than the compute units, keys are cut into ranges, whose records a second launch joins: 512
-// tokens of 12 heads behind 3,500 keys 29.6 us (the other cache, without ranges, 42), 64 of 8 heads of 128 behind 8,000
-// 23.7 (126), 1,024 of 8 heads of 256 40 (52).
+// tokens of 12 heads behind 3,500 keys 29 us (the other cache, without ranges, 40), 64 of 8 heads of 128 behind 8,000
+// 23.6 (117), 1,024 of 8 heads of 256 40 (48).
 //
 // Keys whose page the table does not name are masked, and values that are no number stay in their own dimensions: both
 // are looked for by a bit to a block, and cost the blocks without any 0 to 3 % (2 x 1,024 tokens of 12 heads of 64 21.1 and
@@ -21,7 +21,7 @@
 //
 // Blocks of 64 rows: 8 waves, four along the keys, for heads of up to 128 (16 heads of 128: 4,096 tokens 180 us, of four
 // waves, two along the keys, 258), but many blocks of smaller heads, whose four waves fit a unit more often (2 x 4,096 tokens of 12
-// heads of 64 126 us), and heads beyond 128, whose accumulators take the registers of eight.
+// heads of 64 122 us), and heads beyond 128, whose accumulators take the registers of eight.
 #include <math.h>
 
 #include "common.h"

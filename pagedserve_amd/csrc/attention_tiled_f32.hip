@@ -27,8 +27,8 @@
 //
 // Over a cache in 4 bits (cache_int4.h) a lane reads its key's whole row of codes, 16 bytes a group, and of a value the
 // byte of its dimension in every group, with the keys' steps; they become floats, exactly, where they are multiplied:
-// 2 x 1,024 tokens of 12 heads of 64 65.3 us (floats 59.0), 512 behind 3,500 keys 163 (127), 512 of 16 heads of 128 over 4
-// behind 2,000 154 (138); token by token 371, 620 and 983.
+// 2 x 1,024 tokens of 12 heads of 64 65 us (floats 59), 512 behind 3,500 keys 163 (126), 512 of 16 heads of 128 over 4
+// behind 2,000 153 (138); token by token 370, 618 and 982.
 //
 // Head sizes that are multiples of 4 up to 128; others stay with the one-wave-per-token
 // kernel.
